@@ -170,7 +170,24 @@ SIGNATURES = {
     "cign_gamma_residual_bwd": (c_int, [c_int64, c_int64, _P, _P, _P, c_float, c_uint64, _P, _P, _P,
                                         _P, c_size_t, _P]),
     "cign_block_dropout_mask": (c_int, [c_int64, c_float, c_uint64, _P, _P, _P]),
+    "cign_layer_norm_fwd": (c_int, [c_int64, c_int64, c_int32, c_int32, _P, c_int64, _P, _P,
+                                    c_float, _P, _P, _P, _P]),
+    "cign_layer_norm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "cign_layer_norm_bwd": (c_int, [c_int64, c_int64, c_int32, c_int32, _P, c_int64, _P, c_int64,
+                                    _P, _P, _P, _P, _P, _P, _P, c_size_t, _P]),
+    "cign_node_log_probs_fwd": (c_int, [c_int64, c_int64, c_int32, _P, c_int64, _P, c_int32, _P,
+                                        _P, _P, _P, _P, _P]),
+    "cign_node_log_probs_bwd": (c_int, [c_int64, c_int64, c_int32, _P, c_int64, _P, _P, _P,
+                                        c_int32, _P, _P, c_int64, _P, c_int64, _P, _P, _P]),
+    "cign_distill_fwd": (c_int, [c_int64, c_int64, c_int32, _P, c_int64, c_int32, c_int32, _P,
+                                 c_int64, c_int32, _P, c_int64, c_float, c_int32, _P, _P, _P]),
+    "cign_distill_bwd": (c_int, [c_int64, c_int64, c_int32, _P, c_int64, c_int32, c_int32, _P,
+                                 c_int64, c_int32, _P, c_int64, c_float, c_int32, _P, _P, c_int64,
+                                 _P, _P]),
 }
+
+# element types of the class-row operators (CIGN_F32, CIGN_BF16, CIGN_F16)
+TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 def load_library(path: Path | str | None = None):
@@ -237,6 +254,19 @@ def ptr_array(ts) -> "ctypes.Array":
     for i, t in enumerate(ts):
         arr[i] = 0 if t is None else t.data_ptr()
     return arr
+
+
+def rows_of(t: torch.Tensor) -> tuple:
+    """(t, row stride) of a 2-D tensor as a kernel reads it: unit stride within
+    a row, rows apart by at least their width; copied if it is not so."""
+    n, c = t.shape
+    if t.stride(1) == 1 or c == 1:
+        ld = t.stride(0)
+        if n <= 1:
+            return t, c
+        if ld >= c:
+            return t, ld
+    return t.contiguous(), c
 
 
 def stream_of(t: torch.Tensor) -> c_void_p:

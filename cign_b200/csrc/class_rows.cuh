@@ -1,0 +1,123 @@
+// Shared device code of the row operators over float32, bfloat16 and float16
+// matrices (layer_norm.cu, node_log_probs.cu, distill.cu): element types and
+// conversions, block reductions, and the running softmax statistics of a row.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace cign {
+
+// ---------------------------------------------------------------- types
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);  // to nearest, ties to even
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+inline bool known_type(int32_t t) { return t == CIGN_F32 || t == CIGN_BF16 || t == CIGN_F16; }
+inline size_t type_size(int32_t t) { return t == CIGN_F32 ? 4 : 2; }
+
+// CALL with `T` bound to the element type named by the run-time code `TYPE`.
+#define CIGN_TYPE_DISPATCH(TYPE, T, ...)                              \
+  do {                                                                \
+    if ((TYPE) == CIGN_F32) { using T = float; __VA_ARGS__; }         \
+    else if ((TYPE) == CIGN_BF16) { using T = __nv_bfloat16; __VA_ARGS__; } \
+    else { using T = __half; __VA_ARGS__; }                           \
+  } while (0)
+
+// ---------------------------------------------------------------- block sums
+// Sum of v over the block, in lane order then warp order (fixed, so runs
+// repeat bit for bit); every thread gets it.  `part` holds one float per warp.
+template <int WARPS>
+__device__ __forceinline__ float block_sum(float v, float* part) {
+  v = warp_sum(v);
+  __syncthreads();  // part may still be read from an earlier call
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = 0.0f;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) s += part[w];
+  return s;
+}
+
+// ---------------------------------------------------------------- softmax
+// Running statistics of the values seen so far, relative to their maximum m:
+//   s = sum e^(x - m) - 1   (without the maximum's own e^0)
+//   t = sum e^(x - m) (x - m)
+// so lse = m + log1p(s) and the entropy is log1p(s) - t / (1 + s), a sum of
+// two terms that are not negative.  Keeping the 1 out of the sum keeps the
+// digits of log1p(s) where one class has nearly all of the probability.
+// Nothing seen: m = -inf, s = -1.  Values -inf count as probability 0; a NaN
+// makes s NaN.
+struct RowStat {
+  float m = -INFINITY, s = -1.0f, t = 0.0f;
+};
+
+__device__ __forceinline__ void stat_add(RowStat& a, float x) {
+  if (x > a.m) {
+    const float f = expf(a.m - x);  // 0 where nothing (or only -inf) was seen
+    const float all = (1.0f + a.s) * f;
+    a.t = f > 0.0f ? fmaf(all, a.m - x, f * a.t) : 0.0f;
+    a.s = all;
+    a.m = x;
+  } else if (x == a.m) {
+    a.s += 1.0f;
+  } else {
+    const float d = x - a.m;  // NaN where x is NaN
+    const float e = expf(d);
+    a.s += e;
+    if (e > 0.0f) a.t = fmaf(e, d, a.t);
+  }
+}
+
+// The union of two disjoint sets of values.
+__device__ __forceinline__ RowStat stat_merge(const RowStat& a, const RowStat& b) {
+  const bool ge = a.m >= b.m;
+  const RowStat hi = ge ? a : b, lo = ge ? b : a;
+  const bool eq = a.m == b.m;
+  const float dm = eq ? 0.0f : lo.m - hi.m;
+  const float f = eq ? 1.0f : expf(dm);
+  const float n = (1.0f + lo.s) * f;
+  RowStat r;
+  r.m = hi.m;
+  r.s = hi.s + n;
+  r.t = hi.t;
+  if (f > 0.0f) r.t += fmaf(n, dm, f * lo.t);
+  return r;
+}
+
+__device__ __forceinline__ RowStat stat_shfl_xor(const RowStat& a, int o) {
+  RowStat b;
+  b.m = __shfl_xor_sync(kFullMask, a.m, o);
+  b.s = __shfl_xor_sync(kFullMask, a.s, o);
+  b.t = __shfl_xor_sync(kFullMask, a.t, o);
+  return b;
+}
+
+// ---------------------------------------------------------------- ordering
+// Classes are ordered by value, larger first (NaN before everything, as
+// torch.sort orders it), and by index, smaller first: larger keys come first.
+// -0 and +0 are equal.  0 is below every key.
+__device__ __forceinline__ uint64_t class_key(float v, uint32_t index) {
+  uint32_t u = __float_as_uint(v + 0.0f);
+  u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  if (v != v) u = 0xffffffffu;
+  return (static_cast<uint64_t>(u) << 32) | static_cast<uint32_t>(~index);
+}
+__device__ __forceinline__ uint32_t key_index(uint64_t key) {
+  return ~static_cast<uint32_t>(key);
+}
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t u = static_cast<uint32_t>(key >> 32);
+  if (u == 0xffffffffu) return __int_as_float(0x7fffffff);
+  return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+}
+
+}  // namespace cign

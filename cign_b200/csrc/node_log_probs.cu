@@ -1,0 +1,219 @@
+// Log probabilities of given classes, entropy and best classes of the rows of
+// a logit matrix, and the gradient of the logits.  With m the row's maximum,
+// s = sum e^(x - m) - 1 and t = sum e^(x - m) (x - m) (class_rows.cuh):
+//   log p_j = (x_j - m) - log1p(s),   H = log1p(s) - t / (1 + s)
+// and with the upstream gradients gl (label y), gh (entropy) and gt_i (best
+// class idx_i), G = gl + sum_i gt_i and a_j = gl [j = y] + sum_i gt_i [j = idx_i]:
+//   grad_j = a_j - p_j G - gh p_j (log p_j + H)
+// Where a_j is not zero, a_j - p_j G is formed as (a_j - G) - G expm1(log p_j),
+// which keeps its digits for p_j near 1.
+#include "class_rows.cuh"
+
+namespace cign {
+namespace {
+
+constexpr int kLpThreads = 256;
+constexpr int kLpWarps = kLpThreads / 32;
+constexpr int kLpMaxTop = 64;
+
+struct LogProbOut {
+  float* log_prob;
+  float* entropy;
+  float* stats;  // [n, 2]: m, log1p(s)
+  float* top_log_probs;
+  int64_t* top_index;
+};
+
+// log1p(s); NaN for a row that holds +inf, as it has no distribution.
+__device__ __forceinline__ float stat_log(const RowStat& a) {
+  return a.m == INFINITY ? __int_as_float(0x7fffffff) : log1pf(a.s);
+}
+// Every class of the row is masked (-inf): nothing is left to distribute.
+__device__ __forceinline__ bool stat_nothing(const RowStat& a) {
+  return a.m == -INFINITY && a.s == a.s;
+}
+__device__ __forceinline__ float log_prob_of(float x, float m, float logs) {
+  return m == -INFINITY ? (logs == logs ? -INFINITY : logs) : (x - m) - logs;
+}
+
+__device__ __forceinline__ RowStat block_stat(RowStat a, RowStat* part) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a = stat_merge(a, stat_shfl_xor(a, o));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
+  __syncthreads();
+  a = part[0];
+#pragma unroll
+  for (int w = 1; w < kLpWarps; ++w) a = stat_merge(a, part[w]);
+  return a;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLpThreads)
+log_probs_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld,
+                     const int64_t* __restrict__ labels, int top_k, LogProbOut out) {
+  __shared__ RowStat part[kLpWarps];
+  __shared__ unsigned long long best[kLpWarps];
+  const int64_t row = blockIdx.x;
+  const T* x = logits + row * ld;
+  RowStat a;
+  for (int64_t j = threadIdx.x; j < c; j += kLpThreads) stat_add(a, to_f(x[j]));
+  a = block_stat(a, part);
+  const float logs = stat_log(a);
+  if (threadIdx.x == 0) {
+    if (out.stats) {
+      out.stats[2 * row] = a.m;
+      out.stats[2 * row + 1] = logs;
+    }
+    if (out.entropy) out.entropy[row] = stat_nothing(a) ? 0.0f : logs - a.t / (1.0f + a.s);
+    if (out.log_prob) {
+      const int64_t y = labels[row];
+      float lp = 0.0f;
+      if (y >= c) lp = __int_as_float(0x7fffffff);
+      else if (y >= 0) lp = log_prob_of(to_f(x[y]), a.m, logs);
+      out.log_prob[row] = lp;
+    }
+  }
+  uint64_t last = ~0ull;
+  for (int i = 0; i < top_k; ++i) {
+    uint64_t key = 0;
+    for (int64_t j = threadIdx.x; j < c; j += kLpThreads) {
+      const uint64_t q = class_key(to_f(x[j]), static_cast<uint32_t>(j));
+      if (q < last && q > key) key = q;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const uint64_t q = __shfl_xor_sync(kFullMask, key, o);
+      if (q > key) key = q;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) best[threadIdx.x >> 5] = key;
+    __syncthreads();
+    for (int w = 0; w < kLpWarps; ++w)
+      if (best[w] > key) key = best[w];
+    last = key;
+    if (threadIdx.x == 0) {
+      out.top_index[row * top_k + i] = key_index(key);
+      out.top_log_probs[row * top_k + i] = log_prob_of(key_value(key), a.m, logs);
+    }
+  }
+}
+
+struct LogProbGrads {
+  const float* log_prob;  // element r at r * stride; NULL = no such gradient
+  int64_t log_prob_stride;
+  const float* entropy;
+  int64_t entropy_stride;
+  const float* top;  // [n, top_k] contiguous
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kLpThreads)
+log_probs_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld,
+                     const int64_t* __restrict__ labels, const float* __restrict__ stats,
+                     const float* __restrict__ entropy, int top_k,
+                     const int64_t* __restrict__ top_index, LogProbGrads g,
+                     T* __restrict__ grad) {
+  const int64_t row = blockIdx.x;
+  const T* x = logits + row * ld;
+  T* out = grad + row * c;
+  const float nan = __int_as_float(0x7fffffff);
+  const int64_t y = (g.log_prob && labels) ? labels[row] : -1;
+  const float gl = y >= 0 ? (y < c ? g.log_prob[row * g.log_prob_stride] : nan) : 0.0f;
+  const float gh = g.entropy ? g.entropy[row * g.entropy_stride] : 0.0f;
+  const float m = stats[2 * row], logs = stats[2 * row + 1];
+  float G = gl;
+  bool any = !(gl == 0.0f) || !(gh == 0.0f);
+  if (g.top)
+    for (int i = 0; i < top_k; ++i) {
+      const float v = g.top[row * top_k + i];
+      G += v;
+      any |= !(v == 0.0f);
+    }
+  const float H = g.entropy ? entropy[row] : 0.0f;
+  // no gradient reaches the row, or it has no distribution
+  const bool zero = !any || (m == -INFINITY && logs == logs);
+  for (int64_t j = threadIdx.x; j < c; j += kLpThreads) {
+    float v = 0.0f;
+    if (!zero) {
+      const float lp = (to_f(x[j]) - m) - logs;
+      const float p = expf(lp);
+      const float spread = p > 0.0f ? gh * p * (lp + H) : gh * p;
+      float a = 0.0f;
+      bool special = j == y;
+      if (special) a = gl;
+      if (g.top)
+        for (int i = 0; i < top_k; ++i)
+          if (top_index[row * top_k + i] == j) {
+            a += g.top[row * top_k + i];
+            special = true;
+          }
+      v = special ? (a - G) - G * expm1f(lp) - spread : -p * G - spread;
+    }
+    out[j] = from_f<T>(v);
+  }
+}
+
+int lp_check(int64_t n, int64_t c, int32_t x_type, int64_t ld, int32_t top_k, const char* name) {
+  CIGN_REQUIRE(n >= 0 && c > 0, CIGN_ERR_INVALID_ARGUMENT, "%s: bad sizes", name);
+  CIGN_REQUIRE(known_type(x_type), CIGN_ERR_INVALID_ARGUMENT, "%s: unknown element type", name);
+  CIGN_REQUIRE(ld >= c, CIGN_ERR_INVALID_ARGUMENT, "%s: row stride below the class count", name);
+  CIGN_REQUIRE(top_k >= 0 && top_k <= c, CIGN_ERR_INVALID_ARGUMENT,
+               "%s: top_k must be between 0 and the class count", name);
+  CIGN_REQUIRE(top_k <= kLpMaxTop, CIGN_ERR_UNSUPPORTED, "%s: top_k is at most %d", name,
+               kLpMaxTop);
+  CIGN_REQUIRE(n < (1ll << 31) && c < (1ll << 31), CIGN_ERR_UNSUPPORTED,
+               "%s: at most 2^31 - 1 rows and classes", name);
+  return CIGN_OK;
+}
+
+}  // namespace
+}  // namespace cign
+
+using namespace cign;
+
+extern "C" {
+
+int cign_node_log_probs_fwd(int64_t n, int64_t c, int32_t x_type, const void* logits, int64_t ld,
+                            const int64_t* labels, int32_t top_k, float* log_prob, float* entropy,
+                            float* stats, float* top_log_probs, int64_t* top_index,
+                            cign_stream_t stream) {
+  int rc = lp_check(n, c, x_type, ld, top_k, "node_log_probs_fwd");
+  if (rc) return rc;
+  if (n == 0) return CIGN_OK;
+  CIGN_REQUIRE(logits != nullptr && (log_prob == nullptr || labels != nullptr) &&
+                   (top_k == 0 || (top_log_probs && top_index)),
+               CIGN_ERR_NULL_POINTER, "node_log_probs_fwd: NULL argument");
+  const LogProbOut out{log_prob, entropy, stats, top_log_probs, top_index};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  CIGN_TYPE_DISPATCH(x_type, T,
+      log_probs_fwd_kernel<T><<<static_cast<unsigned>(n), kLpThreads, 0, s>>>(
+          n, c, static_cast<const T*>(logits), ld, labels, top_k, out));
+  CIGN_CHECK_LAUNCH("log_probs_fwd_kernel");
+  return CIGN_OK;
+}
+
+int cign_node_log_probs_bwd(int64_t n, int64_t c, int32_t x_type, const void* logits, int64_t ld,
+                            const int64_t* labels, const float* stats, const float* entropy,
+                            int32_t top_k, const int64_t* top_index, const float* grad_log_prob,
+                            int64_t grad_log_prob_stride, const float* grad_entropy,
+                            int64_t grad_entropy_stride, const float* grad_top, void* grad_logits,
+                            cign_stream_t stream) {
+  int rc = lp_check(n, c, x_type, ld, top_k, "node_log_probs_bwd");
+  if (rc) return rc;
+  if (n == 0) return CIGN_OK;
+  CIGN_REQUIRE(logits && stats && grad_logits && (!grad_log_prob || labels) &&
+                   (!grad_entropy || entropy) && (!grad_top || top_index),
+               CIGN_ERR_NULL_POINTER, "node_log_probs_bwd: NULL argument");
+  const LogProbGrads g{grad_log_prob, grad_log_prob_stride, grad_entropy, grad_entropy_stride,
+                       top_k > 0 ? grad_top : nullptr};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  CIGN_TYPE_DISPATCH(x_type, T,
+      log_probs_bwd_kernel<T><<<static_cast<unsigned>(n), kLpThreads, 0, s>>>(
+          n, c, static_cast<const T*>(logits), ld, labels, stats, entropy, top_k, top_index, g,
+          static_cast<T*>(grad_logits)));
+  CIGN_CHECK_LAUNCH("log_probs_bwd_kernel");
+  return CIGN_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,110 @@
+"""LayerNorm of the last dimension for rows of any width in float32, bfloat16
+or float16, with its backward pass (cign_layer_norm_fwd/_bwd).
+
+``fused_block_ops`` has the block's norms (float32, up to 1024 wide, with
+dropout or an addend) and ``jk_norm`` the output norm over the block states
+(float32, up to 2048 wide); :func:`layer_norm` takes the rows they refuse: a
+deeper model's output norm, half-precision rows, rows of a wider buffer, norms
+without weight or bias.  Statistics and sums are float32 for every type, the
+weight and bias gradients are summed in a fixed order, and y, grad x, grad
+weight and grad bias are rounded once.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+
+def _forward(x, ldx, weight, bias, eps, need_stats):
+    lib = _lib.load_library()
+    n, d = x.shape
+    y = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if need_stats:
+        mean, rstd = torch.empty((2, n), dtype=torch.float32, device=x.device).unbind(0)
+    param = weight if weight is not None else bias
+    with _lib.DeviceGuard(x.device):
+        rc = lib.cign_layer_norm_fwd(n, d, _lib.TYPE_CODES[x.dtype],
+                                     _lib.TYPE_CODES[x.dtype if param is None else param.dtype],
+                                     _lib.ptr(x), ldx, _lib.ptr(weight), _lib.ptr(bias), eps,
+                                     _lib.ptr(y), _lib.ptr(mean), _lib.ptr(rstd),
+                                     _lib.stream_of(x))
+    _lib.check(rc, "cign_layer_norm_fwd")
+    return y, mean, rstd
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        rows, ldx = _lib.rows_of(x)
+        y, mean, rstd = _forward(rows, ldx, weight, bias, eps, True)
+        ctx.save_for_backward(rows, weight, mean, rstd)
+        ctx.ldx = ldx
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        lib = _lib.load_library()
+        x, weight, mean, rstd = ctx.saved_tensors
+        n, d = x.shape
+        dev = x.device
+        gy, ldg = _lib.rows_of(gy)
+        want_x, want_w, want_b, _ = ctx.needs_input_grad
+        gx = torch.empty((n, d), dtype=x.dtype, device=dev) if want_x else None
+        gw = torch.empty((d,), dtype=weight.dtype, device=dev) if want_w else None
+        gb = torch.empty((d,), dtype=ctx.bias_dtype, device=dev) if want_b else None
+        param = x.dtype if weight is None and ctx.bias_dtype is None else (
+            ctx.bias_dtype if weight is None else weight.dtype)
+        ws = _lib.workspace(lib.cign_layer_norm_bwd_workspace_bytes(n, d) if want_w or want_b
+                            else 0, dev)
+        with _lib.DeviceGuard(dev):
+            rc = lib.cign_layer_norm_bwd(n, d, _lib.TYPE_CODES[x.dtype], _lib.TYPE_CODES[param],
+                                         _lib.ptr(gy), ldg, _lib.ptr(x), ctx.ldx,
+                                         _lib.ptr(weight), _lib.ptr(mean), _lib.ptr(rstd),
+                                         _lib.ptr(gx), _lib.ptr(gw), _lib.ptr(gb), _lib.ptr(ws),
+                                         ws.numel(), _lib.stream_of(x))
+        _lib.check(rc, "cign_layer_norm_bwd")
+        return gx, gw, gb, None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    """LayerNorm of x's last dimension: (x - mean) / sqrt(var + eps) * weight + bias.
+
+    x: CUDA float32, bfloat16 or float16, any leading dimensions; the rows may
+    lie in a wider buffer.  weight, bias: [D] or None, both of one type, x's or
+    float32.  Gradients flow to x, weight and bias (once: a second derivative
+    raises)."""
+    if x.device.type != "cuda" or x.dtype not in _lib.TYPE_CODES:
+        raise TypeError("x must be CUDA float32, bfloat16 or float16")
+    if x.dim() < 1 or x.size(-1) < 1:
+        raise ValueError(f"x must be [..., D] with D >= 1, got {tuple(x.shape)}")
+    d = x.size(-1)
+    eps = float(eps)
+    if not (0.0 <= eps < float("inf")):
+        raise ValueError("eps must be finite and not negative")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        if p.device != x.device or p.dtype not in (x.dtype, torch.float32):
+            raise TypeError(f"{name} must be on x's device, of x's type or float32")
+        if p.shape != (d,):
+            raise ValueError(f"{name} must be [{d}], got {tuple(p.shape)}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError("weight and bias must have the same type")
+    rows = x if x.dim() == 2 else x.reshape(-1, d)
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        y = _LayerNormFn.apply(rows, weight, bias, eps)
+    else:
+        rows, ldx = _lib.rows_of(rows)
+        y = _forward(rows, ldx, weight, bias, eps, False)[0]
+    return y if x.dim() == 2 else y.view(x.shape)

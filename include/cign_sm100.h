@@ -5,7 +5,8 @@
  * Conventions
  *   - Every pointer argument is a DEVICE pointer unless stated otherwise;
  *     pointer arrays (float* const* ...) are HOST arrays of device pointers.
- *   - Dense matrices are row-major, fp32, contiguous, rows of the stated width.
+ *   - Dense matrices are row-major, fp32, contiguous, rows of the stated width
+ *     (the class-row operators at the end state their own types and strides).
  *   - CSR indices are int32 (the reference converts to int32 before any
  *     kernel: multihop_csr_pipeline.py:38-48, collapsed_gat.cpp:32-43).
  *   - `stream` is a cudaStream_t passed as void*; 0 = legacy default stream.
@@ -656,6 +657,87 @@ CIGN_API int cign_gamma_residual_bwd(int64_t n, int64_t d, const float* grad_y,
 CIGN_API int cign_block_dropout_mask(int64_t count, float p, uint64_t seed,
                               const uint64_t* seed_ptr,
                             uint8_t* mask, cign_stream_t stream);
+
+/* ------------------------------------------------------------------ class rows
+ * Row operators of the classification head over float32, bfloat16 or float16
+ * matrices: LayerNorm of any width, log probabilities of labels with entropy
+ * and best classes, and distillation from a teacher's kept classes.  The
+ * reference runs these steps on torch (nn.LayerNorm, model_cign.py:1195-1201;
+ * F.cross_entropy on the train mask, train_cign.py:2103-2148); it has no
+ * distillation.
+ *   - `x_type` and `param_type` are CIGN_F32, CIGN_BF16 or CIGN_F16.
+ *   - Matrices are row-major with the stated row stride (in elements, at
+ *     least the width); pointers need the alignment of one element only.
+ *     Outputs have no gaps between rows.
+ *   - Statistics, sums and products are float32 (or wider) for every type;
+ *     outputs are rounded once. */
+enum { CIGN_F32 = 0, CIGN_BF16 = 1, CIGN_F16 = 2 };
+
+/* y = (x - mean) * (var + eps)^-1/2 * w + b per row (biased variance).
+ * x: [n, d], row stride ldx; w, b: [d] or NULL (1 and 0); mean, rstd: [n]
+ * for the backward, or both NULL.  n < 2^31, d < 2^24. */
+CIGN_API int cign_layer_norm_fwd(int64_t n, int64_t d, int32_t x_type, int32_t param_type,
+                        const void* x, int64_t ldx, const void* w, const void* b, float eps,
+                        void* y, float* mean, float* rstd, cign_stream_t stream);
+
+CIGN_API size_t cign_layer_norm_bwd_workspace_bytes(int64_t n, int64_t d);
+
+/* grad_x [n, d] (x_type), grad_w = sum_n grad_y * xhat and grad_b = sum_n
+ * grad_y [d] (param_type); each may be NULL when it is not wanted.  ws
+ * (16-byte aligned) is used for grad_w and grad_b only. */
+CIGN_API int cign_layer_norm_bwd(int64_t n, int64_t d, int32_t x_type, int32_t param_type,
+                        const void* grad_y, int64_t ldg, const void* x, int64_t ldx,
+                        const void* w, const float* mean, const float* rstd, void* grad_x,
+                        void* grad_w, void* grad_b, void* ws, size_t ws_bytes,
+                        cign_stream_t stream);
+
+/* Per row of logits [n, c]: log_prob = log softmax at labels[row], entropy of
+ * the softmax, and the top_k (0..64, at most c) classes by value (ties: the
+ * lower class; NaN before everything) with their log probabilities.
+ *   labels: int64 [n]; negative = no label (log_prob 0, no gradient);
+ *     >= c = log_prob NaN.  labels and log_prob may both be NULL.
+ *   entropy, stats ([n, 2], for the backward) may be NULL.
+ *   A class with logit -inf has probability 0.  A row of -inf only has
+ *     log_prob -inf (0 without a label), entropy 0 and gradient 0; a row with
+ *     a NaN or +inf gives NaN. */
+CIGN_API int cign_node_log_probs_fwd(int64_t n, int64_t c, int32_t x_type, const void* logits,
+                            int64_t ld, const int64_t* labels, int32_t top_k, float* log_prob,
+                            float* entropy, float* stats, float* top_log_probs,
+                            int64_t* top_index, cign_stream_t stream);
+
+/* grad_logits [n, c] (x_type) from the upstream gradients of log_prob,
+ * entropy (element r at r * stride) and top_log_probs ([n, top_k], no gaps);
+ * each may be NULL.  stats, entropy, top_index: the forward's. */
+CIGN_API int cign_node_log_probs_bwd(int64_t n, int64_t c, int32_t x_type, const void* logits,
+                            int64_t ld, const int64_t* labels, const float* stats,
+                            const float* entropy, int32_t top_k, const int64_t* top_index,
+                            const float* grad_log_prob, int64_t grad_log_prob_stride,
+                            const float* grad_entropy, int64_t grad_entropy_stride,
+                            const float* grad_top, void* grad_logits, cign_stream_t stream);
+
+/* Per row: T^2 times the divergence KL(teacher || student) over the teacher's
+ * k (1..256) kept classes, student p = softmax(logits / T).
+ *   values [n, k] (value_type), index [n, k] (index_type 0: int32, 1: int64),
+ *     with their row strides.  An entry with a negative index or value -inf
+ *     is absent; an index >= c makes the row NaN; a class may occur twice.
+ *   tail 0 ("drop"): the teacher is softmax(values / T) over the entries.
+ *   tail 1 ("bucket"): values are the teacher's log probabilities at T; what
+ *     they leave of 1 is one more class, compared with the student's
+ *     probability of all classes that are not kept.
+ *   A row without entries has loss 0 and gradient 0.
+ *   loss [n]; stats [n, 8] (16-byte aligned, for the backward) or NULL.
+ *   c <= 2^20. */
+CIGN_API int cign_distill_fwd(int64_t n, int64_t c, int32_t x_type, const void* logits, int64_t ld,
+                     int32_t k, int32_t value_type, const void* values, int64_t ld_values,
+                     int32_t index_type, const void* index, int64_t ld_index, float temperature,
+                     int32_t tail, float* loss, float* stats, cign_stream_t stream);
+
+/* grad_logits [n, c] (x_type); grad_loss: element r at r * stride. */
+CIGN_API int cign_distill_bwd(int64_t n, int64_t c, int32_t x_type, const void* logits, int64_t ld,
+                     int32_t k, int32_t value_type, const void* values, int64_t ld_values,
+                     int32_t index_type, const void* index, int64_t ld_index, float temperature,
+                     int32_t tail, const float* stats, const float* grad_loss,
+                     int64_t grad_loss_stride, void* grad_logits, cign_stream_t stream);
 
 #ifdef __cplusplus
 }
