@@ -101,6 +101,50 @@ __device__ __forceinline__ RowStat stat_shfl_xor(const RowStat& a, int o) {
   return b;
 }
 
+// ---------------------------------------------------------------- narrow rows
+// Rows of at most 8 G classes are held by a group of G lanes (a power of two,
+// G <= 32), class lane + G i in register i: the loads and stores of a group
+// cover G neighbouring elements at a time, a row is read once, and the 32 / G
+// rows of a warp are neighbours.  8 loads in flight per lane are what covers
+// the memory latency at full occupancy.
+constexpr int kNarrowElems = 8;
+constexpr int kNarrowThreads = 256;
+constexpr int64_t kNarrowMax = 32 * kNarrowElems;
+
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+  return v;
+}
+template <int G>
+__device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFullMask, v, o));
+  return v;
+}
+// The lanes of this lane's group, as a warp mask.
+template <int G>
+__device__ __forceinline__ unsigned group_mask() {
+  if (G == 32) return kFullMask;
+  return ((1u << (G & 31)) - 1u) << ((threadIdx.x & 31) & ~(G - 1));
+}
+
+inline unsigned narrow_grid(int64_t n, int G) {
+  return static_cast<unsigned>((n + kNarrowThreads / G - 1) / (kNarrowThreads / G));
+}
+
+// CALL with `G` bound to the lanes of a row of c <= kNarrowMax classes.
+#define CIGN_GROUP_DISPATCH(c, G, ...)                               \
+  do {                                                                \
+    if ((c) <= 8) { constexpr int G = 1; __VA_ARGS__; }               \
+    else if ((c) <= 16) { constexpr int G = 2; __VA_ARGS__; }         \
+    else if ((c) <= 32) { constexpr int G = 4; __VA_ARGS__; }         \
+    else if ((c) <= 64) { constexpr int G = 8; __VA_ARGS__; }         \
+    else if ((c) <= 128) { constexpr int G = 16; __VA_ARGS__; }       \
+    else { constexpr int G = 32; __VA_ARGS__; }                       \
+  } while (0)
+
 // ---------------------------------------------------------------- ordering
 // Classes are ordered by value, larger first (NaN before everything, as
 // torch.sort orders it), and by index, smaller first: larger keys come first.

@@ -129,6 +129,56 @@ __device__ __forceinline__ double log_q(float v, const DistillRow& r, bool bucke
   return (static_cast<double>(v) - r.tmax) * it.full - static_cast<double>(r.tlog);
 }
 
+// W p - q of a kept class: q the sum of its entries.
+__device__ __forceinline__ float kept_gradient(const Teacher& te, int64_t row, int64_t c,
+                                               int64_t idx, float v, double lp,
+                                               const DistillRow& r, bool bucket, const InvT& it) {
+  const double lq = log_q(v, r, bucket, it);
+  if (r.dup == 0.0f) {
+    const float d = static_cast<float>(lq - lp);
+    return expf(static_cast<float>(lq)) *
+           (expm1f(-d) + (r.w1 != 0.0f ? r.w1 * expf(-d) : 0.0f));
+  }
+  float q = 0.0f;
+  for (int i = 0; i < te.k; ++i) {
+    const float w = teacher_value(te, row, i);
+    if (teacher_index(te, row, i) == idx && w != -INFINITY)
+      q += expf(static_cast<float>(log_q(w, r, bucket, it)));
+  }
+  return (1.0f + r.w1) * expf(static_cast<float>(lp)) - q;
+}
+
+__device__ __forceinline__ DistillRow load_row(const float* stats) {
+  const float4 a = reinterpret_cast<const float4*>(stats)[0];
+  const float4 b = reinterpret_cast<const float4*>(stats)[1];
+  return DistillRow{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+}
+
+// The row's loss and statistics from the sum over its entries.
+__device__ __forceinline__ void finish_row(DistillRow r, float sum, float mass_r, float p_rest,
+                                           bool none, bool bad, bool dup, float temperature,
+                                           float* loss, float* stats) {
+  if (mass_r != 0.0f)
+    sum += p_rest > 0.0f ? divergence_term(mass_r, logf(mass_r) - logf(p_rest)) : INFINITY;
+  else
+    sum += p_rest;
+  float l = temperature * temperature * (sum + r.w1);
+  r.spread = (1.0f + r.w1) - (mass_r != 0.0f && p_rest > 0.0f ? mass_r / p_rest : 0.0f);
+  r.dup = dup ? 1.0f : 0.0f;
+  r.none = none ? 1.0f : 0.0f;
+  if (r.m == -INFINITY && r.logs == r.logs) l = INFINITY;  // the student has no class left
+  if (none) l = 0.0f;
+  if (bad) {
+    l = r.logs = r.spread = __int_as_float(0x7fffffff);
+    r.none = 0.0f;
+  }
+  *loss = l;
+  if (stats) {
+    reinterpret_cast<float4*>(stats)[0] = make_float4(r.m, r.logs, r.spread, r.w1);
+    reinterpret_cast<float4*>(stats)[1] = make_float4(r.tmax, r.tlog, r.dup, r.none);
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kDsThreads)
 distill_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld, Teacher te,
@@ -206,25 +256,10 @@ distill_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t l
     const float d = static_cast<float>(log_q(v, r, bucket, it) - lp);
     term = first ? divergence_term(q, d) : q * (d - 1.0f);
   }
-  float sum = block_sum<kDsWarps>(term, fpart);
-  if (mass_r != 0.0f)
-    sum += p_rest > 0.0f ? divergence_term(mass_r, logf(mass_r) - logf(p_rest)) : INFINITY;
-  else
-    sum += p_rest;
-  float l = temperature * temperature * (sum + r.w1);
-  r.spread = (1.0f + r.w1) - (mass_r != 0.0f && p_rest > 0.0f ? mass_r / p_rest : 0.0f);
-  r.dup = any_dup ? 1.0f : 0.0f;
-  r.none = distinct == 0 ? 1.0f : 0.0f;
-  if (r.m == -INFINITY && r.logs == r.logs) l = INFINITY;  // the student has no class left
-  if (distinct == 0) l = 0.0f;
-  if (any_bad) {
-    l = r.logs = r.spread = __int_as_float(0x7fffffff);
-    r.none = 0.0f;
-  }
-  if (tid == 0) {
-    loss[row] = l;
-    if (stats) *reinterpret_cast<DistillRow*>(stats + row * kDsStats) = r;
-  }
+  const float sum = block_sum<kDsWarps>(term, fpart);
+  if (tid == 0)
+    finish_row(r, sum, mass_r, p_rest, distinct == 0, any_bad, any_dup, temperature, loss + row,
+               stats ? stats + row * kDsStats : nullptr);
 }
 
 template <typename T>
@@ -232,13 +267,11 @@ __global__ void __launch_bounds__(kDsThreads)
 distill_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld, Teacher te,
                    float temperature, InvT it, int bucket, const float* __restrict__ stats,
                    const float* __restrict__ g_loss, int64_t g_stride, T* __restrict__ grad) {
-  __shared__ int64_t kidx[kDsMaxKept];
-  __shared__ float kq[kDsMaxKept];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
   const T* x = logits + row * ld;
   T* out = grad + row * c;
-  const DistillRow r = *reinterpret_cast<const DistillRow*>(stats + row * kDsStats);
+  const DistillRow r = load_row(stats + row * kDsStats);
   const float g = g_loss[row * g_stride] * temperature;
   if (r.none != 0.0f || g == 0.0f || (r.m == -INFINITY && r.logs == r.logs)) {
     for (int64_t j = tid; j < c; j += kDsThreads) out[j] = from_f<T>(0.0f);
@@ -249,30 +282,176 @@ distill_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t l
     const float p = expf(scaled(to_f(x[j]) - r.m, it) - r.logs);
     out[j] = from_f<T>(p * f);
   }
-  int64_t idx = -1;
-  float v = 0.0f;
+  __syncthreads();  // orders the writes above before those below
   if (tid < te.k) {
-    idx = teacher_index(te, row, tid);
-    v = teacher_value(te, row, tid);
-    if (v == -INFINITY || idx >= c) idx = -1;
-    kidx[tid] = idx;
-    kq[tid] = idx >= 0 ? expf(static_cast<float>(log_q(v, r, bucket, it))) : 0.0f;
+    const int64_t idx = teacher_index(te, row, tid);
+    const float v = teacher_value(te, row, tid);
+    if (idx >= 0 && idx < c && v != -INFINITY) {
+      const double lp = (static_cast<double>(to_f(x[idx])) - r.m) * it.full -
+                        static_cast<double>(r.logs);
+      out[idx] = from_f<T>(g * kept_gradient(te, row, c, idx, v, lp, r, bucket, it));
+    }
   }
-  __syncthreads();  // also orders the writes above before those below
-  if (idx >= 0) {
+}
+
+// Rows of at most 8 G classes, a group of G lanes per row (class_rows.cuh).
+// The kept classes of a row are bits in shared memory; lane l takes the
+// teacher's entries l, l + G, ...
+template <int G>
+struct NarrowBits {
+  static constexpr int kWords = G < 4 ? 1 : G / 4;  // 8 G bits
+};
+
+template <typename T, int G>
+__global__ void __launch_bounds__(kNarrowThreads)
+distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_t ld, Teacher te,
+                          float temperature, InvT it, int bucket, float* __restrict__ loss,
+                          float* __restrict__ stats) {
+  constexpr int kWords = NarrowBits<G>::kWords;
+  __shared__ uint32_t all_bits[kNarrowThreads / G * kWords];
+  const int lane = threadIdx.x & (G - 1);
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * (kNarrowThreads / G) + threadIdx.x / G;
+  const bool live = at < n;
+  const int64_t row = live ? at : n - 1;  // the last warp's idle groups follow along
+  const T* x = logits + row * ld;
+  uint32_t* bits = all_bits + threadIdx.x / G * kWords;
+  float v[kNarrowElems];
+#pragma unroll
+  for (int i = 0; i < kNarrowElems; ++i)
+    v[i] = lane + G * i < c ? to_f(x[lane + G * i]) : -INFINITY;
+  for (int i = lane; i < kWords; i += G) bits[i] = 0;
+  __syncwarp();
+  // teacher: kept classes, maximum, log sum, sum of probabilities
+  bool bad = false, dup = false;
+  float tmax = -INFINITY, nan = 0.0f;
+  float distinct = 0.0f;
+  for (int e = lane; e < te.k; e += G) {
+    const int64_t idx = teacher_index(te, row, e);
+    const float tv = teacher_value(te, row, e);
+    if (idx < 0 || tv == -INFINITY) continue;
+    if (idx >= c) {
+      bad = true;
+      continue;
+    }
+    const uint32_t bit = 1u << (idx & 31);
+    const bool first = !(atomicOr(bits + (idx >> 5), bit) & bit);
+    dup |= !first;
+    distinct += first ? 1.0f : 0.0f;
+    tmax = fmaxf(tmax, tv);
+    if (tv != tv) nan = tv;
+  }
+  const unsigned mine = group_mask<G>();
+  bad = __ballot_sync(kFullMask, bad) & mine;
+  dup = __ballot_sync(kFullMask, dup) & mine;
+  __syncwarp();
+  distinct = group_sum<G>(distinct);
+  DistillRow r;
+  r.tmax = group_max<G>(tmax);
+  float tsum = 0.0f, tcnt = 0.0f;
+  double mass = 0.0;
+  for (int e = lane; e < te.k; e += G) {
+    const int64_t idx = teacher_index(te, row, e);
+    const float tv = teacher_value(te, row, e);
+    if (idx < 0 || idx >= c || tv == -INFINITY) continue;
+    if (bucket) mass += exp(static_cast<double>(tv));
+    else if (tv == r.tmax) tcnt += 1.0f;
+    else tsum += expf(scaled(tv - r.tmax, it));
+  }
+  r.tlog = log1pf(group_sum<G>(tsum + nan) + (group_sum<G>(tcnt) - 1.0f));
+  // student: the sums over the classes that are not kept and over the kept ones
+  float m = v[0];
+#pragma unroll
+  for (int i = 1; i < kNarrowElems; ++i) m = fmaxf(m, v[i]);
+  m = group_max<G>(m);
+  if (m != m) m = -INFINITY;
+  float s_rest = 0.0f, c_rest = 0.0f, s_kept = 0.0f, c_kept = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kNarrowElems; ++i) {
+    const int j = lane + G * i;
+    const bool kept = (bits[j >> 5] >> (j & 31)) & 1u;
+    const float one = j < c && v[i] == m ? 1.0f : 0.0f;
+    const float e = v[i] == m ? 0.0f : expf(scaled(v[i] - m, it));
+    s_kept += kept ? e : 0.0f;
+    c_kept += kept ? one : 0.0f;
+    s_rest += kept ? 0.0f : e;
+    c_rest += kept ? 0.0f : one;
+  }
+  s_rest = group_sum<G>(s_rest);
+  c_rest = group_sum<G>(c_rest);
+  const float s = s_rest + group_sum<G>(s_kept) + (group_sum<G>(c_kept) + c_rest - 1.0f);
+  r.m = m;
+  r.logs = m == INFINITY ? __int_as_float(0x7fffffff) : log1pf(s);
+  const float p_rest = (s_rest + c_rest) / (1.0f + s);
+  float mass_r = 0.0f;
+  r.w1 = 0.0f;
+  if (bucket) {
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) mass += __shfl_xor_sync(kFullMask, mass, o);
+    // a small difference where the teacher is sure of its kept classes: 64 bits
+    const float raw = static_cast<float>(1.0 - mass);
+    if (raw == raw && raw < 0.0f) r.w1 = -raw;
+    else mass_r = raw;
+    if (distinct == static_cast<float>(c)) {  // no class is left to take the rest
+      r.w1 = -raw;
+      mass_r = 0.0f;
+    }
+  }
+  float sum = 0.0f;
+  for (int e = lane; e < te.k; e += G) {
+    const int64_t idx = teacher_index(te, row, e);
+    const float tv = teacher_value(te, row, e);
+    if (idx < 0 || idx >= c || tv == -INFINITY) continue;
+    bool first = true;
+    if (dup)  // the first of equal entries by its place
+      for (int q = 0; q < e && first; ++q)
+        first = teacher_index(te, row, q) != idx || teacher_value(te, row, q) == -INFINITY;
+    const double lq = log_q(tv, r, bucket, it);
+    const double lp = (static_cast<double>(to_f(x[idx])) - m) * it.full -
+                      static_cast<double>(r.logs);
+    const float q = expf(static_cast<float>(lq));
+    const float d = static_cast<float>(lq - lp);
+    sum += first ? divergence_term(q, d) : q * (d - 1.0f);
+  }
+  sum = group_sum<G>(sum);
+  if (live && lane == 0) finish_row(r, sum, mass_r, p_rest, distinct == 0.0f, bad, dup,
+                                    temperature, loss + row,
+                                    stats ? stats + row * kDsStats : nullptr);
+}
+
+template <typename T, int G>
+__global__ void __launch_bounds__(kNarrowThreads)
+distill_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_t ld, Teacher te,
+                          float temperature, InvT it, int bucket,
+                          const float* __restrict__ stats, const float* __restrict__ g_loss,
+                          int64_t g_stride, T* __restrict__ grad) {
+  const int lane = threadIdx.x & (G - 1);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kNarrowThreads / G) + threadIdx.x / G;
+  const unsigned mine = group_mask<G>();
+  if (row >= n) return;
+  const T* x = logits + row * ld;
+  T* out = grad + row * c;
+  float v[kNarrowElems];
+#pragma unroll
+  for (int i = 0; i < kNarrowElems; ++i)
+    v[i] = lane + G * i < c ? to_f(x[lane + G * i]) : -INFINITY;
+  const DistillRow r = load_row(stats + row * kDsStats);
+  const float g = g_loss[row * g_stride] * temperature;
+  const bool zero = r.none != 0.0f || g == 0.0f || (r.m == -INFINITY && r.logs == r.logs);
+  const float f = g * r.spread;
+#pragma unroll
+  for (int i = 0; i < kNarrowElems; ++i)
+    if (lane + G * i < c)
+      out[lane + G * i] =
+          from_f<T>(zero ? 0.0f : f * expf(scaled(v[i] - r.m, it) - r.logs));
+  if (zero) return;
+  __syncwarp(mine);  // orders the writes above before those below
+  for (int e = lane; e < te.k; e += G) {
+    const int64_t idx = teacher_index(te, row, e);
+    const float tv = teacher_value(te, row, e);
+    if (idx < 0 || idx >= c || tv == -INFINITY) continue;
     const double lp = (static_cast<double>(to_f(x[idx])) - r.m) * it.full -
                       static_cast<double>(r.logs);
-    float w;
-    if (r.dup != 0.0f) {
-      float q = 0.0f;
-      for (int i = 0; i < te.k; ++i)
-        if (kidx[i] == idx) q += kq[i];
-      w = (1.0f + r.w1) * expf(static_cast<float>(lp)) - q;
-    } else {
-      const float d = static_cast<float>(log_q(v, r, bucket, it) - lp);
-      w = kq[tid] * (expm1f(-d) + (r.w1 != 0.0f ? r.w1 * expf(-d) : 0.0f));
-    }
-    out[idx] = from_f<T>(g * w);
+    out[idx] = from_f<T>(g * kept_gradient(te, row, c, idx, tv, lp, r, bucket, it));
   }
 }
 
@@ -326,8 +505,16 @@ int cign_distill_fwd(int64_t n, int64_t c, int32_t x_type, const void* logits, i
                "distill_fwd: NULL argument");
   CIGN_REQUIRE(aligned16(stats), CIGN_ERR_ALIGNMENT, "distill_fwd: stats must be 16-byte aligned");
   const Teacher te{values, index, ld_values, ld_index, k, value_type, index_type};
-  const size_t smem = static_cast<size_t>((c + 31) / 32) * 4;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (c <= kNarrowMax) {
+    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c, G,
+        distill_narrow_fwd_kernel<T, G><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
+            n, static_cast<int>(c), static_cast<const T*>(logits), ld, te, temperature,
+            inverse(temperature), tail, loss, stats)));
+    CIGN_CHECK_LAUNCH("distill_narrow_fwd_kernel");
+    return CIGN_OK;
+  }
+  const size_t smem = static_cast<size_t>((c + 31) / 32) * 4;
   CIGN_TYPE_DISPATCH(x_type, T, {
     if (smem > 32768)
       CIGN_CHECK_CUDA(cudaFuncSetAttribute(distill_fwd_kernel<T>,
@@ -356,6 +543,15 @@ int cign_distill_bwd(int64_t n, int64_t c, int32_t x_type, const void* logits, i
   CIGN_REQUIRE(aligned16(stats), CIGN_ERR_ALIGNMENT, "distill_bwd: stats must be 16-byte aligned");
   const Teacher te{values, index, ld_values, ld_index, k, value_type, index_type};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (c <= kNarrowMax) {
+    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c, G,
+        distill_narrow_bwd_kernel<T, G><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
+            n, static_cast<int>(c), static_cast<const T*>(logits), ld, te, temperature,
+            inverse(temperature), tail, stats, grad_loss, grad_loss_stride,
+            static_cast<T*>(grad_logits))));
+    CIGN_CHECK_LAUNCH("distill_narrow_bwd_kernel");
+    return CIGN_OK;
+  }
   CIGN_TYPE_DISPATCH(x_type, T,
       distill_bwd_kernel<T><<<static_cast<unsigned>(n), kDsThreads, 0, s>>>(
           n, c, static_cast<const T*>(logits), ld, te, temperature, inverse(temperature), tail,

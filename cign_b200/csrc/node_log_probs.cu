@@ -99,6 +99,76 @@ log_probs_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t
   }
 }
 
+// Rows of at most 8 G classes, a group of G lanes per row (class_rows.cuh).
+template <typename T, int G>
+__global__ void __launch_bounds__(kNarrowThreads)
+log_probs_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_t ld,
+                            const int64_t* __restrict__ labels, int top_k, LogProbOut out) {
+  const int lane = threadIdx.x & (G - 1);
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * (kNarrowThreads / G) + threadIdx.x / G;
+  const bool live = at < n;
+  const int64_t row = live ? at : n - 1;  // the last warp's idle groups follow along
+  const T* x = logits + row * ld;
+  const int64_t y = out.log_prob ? labels[row] : -1;
+  float v[kNarrowElems];
+#pragma unroll
+  for (int i = 0; i < kNarrowElems; ++i)
+    v[i] = lane + G * i < c ? to_f(x[lane + G * i]) : -INFINITY;
+  const float xy = y >= 0 && y < c ? to_f(x[y]) : 0.0f;
+  float m = v[0];
+#pragma unroll
+  for (int i = 1; i < kNarrowElems; ++i) m = fmaxf(m, v[i]);
+  m = group_max<G>(m);
+  if (m != m) m = -INFINITY;
+  float s = 0.0f, cnt = 0.0f, t = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kNarrowElems; ++i) {
+    if (v[i] == m) {
+      cnt += 1.0f;
+    } else {
+      const float d = v[i] - m;
+      const float e = expf(d);
+      s += e;
+      t = fmaf(e, fmaxf(d, -1e30f), t);  // d = -inf: e = 0
+    }
+  }
+  RowStat a;
+  a.m = m;
+  a.s = group_sum<G>(s) + (group_sum<G>(cnt) - 1.0f);
+  a.t = group_sum<G>(t);
+  const float logs = stat_log(a);
+  if (live && lane == 0) {
+    if (out.stats) *reinterpret_cast<float2*>(out.stats + 2 * row) = make_float2(m, logs);
+    if (out.entropy) out.entropy[row] = stat_nothing(a) ? 0.0f : logs - a.t / (1.0f + a.s);
+    if (out.log_prob) {
+      float lp = 0.0f;
+      if (y >= c) lp = __int_as_float(0x7fffffff);
+      else if (y >= 0) lp = log_prob_of(xy, m, logs);
+      out.log_prob[row] = lp;
+    }
+  }
+  uint64_t last = ~0ull;
+  for (int k = 0; k < top_k; ++k) {
+    uint64_t key = 0;
+#pragma unroll
+    for (int i = 0; i < kNarrowElems; ++i) {
+      const int j = lane + G * i;
+      const uint64_t q = class_key(v[i], static_cast<uint32_t>(j));
+      if (j < c && q < last && q > key) key = q;
+    }
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) {
+      const uint64_t q = __shfl_xor_sync(kFullMask, key, o);
+      if (q > key) key = q;
+    }
+    last = key;
+    if (live && lane == k % G) {
+      out.top_index[row * top_k + k] = key_index(key);
+      out.top_log_probs[row * top_k + k] = log_prob_of(key_value(key), m, logs);
+    }
+  }
+}
+
 struct LogProbGrads {
   const float* log_prob;  // element r at r * stride; NULL = no such gradient
   int64_t log_prob_stride;
@@ -154,6 +224,65 @@ log_probs_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t
   }
 }
 
+template <typename T, int G>
+__global__ void __launch_bounds__(kNarrowThreads)
+log_probs_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_t ld,
+                            const int64_t* __restrict__ labels, const float* __restrict__ stats,
+                            const float* __restrict__ entropy, int top_k,
+                            const int64_t* __restrict__ top_index, LogProbGrads g,
+                            T* __restrict__ grad) {
+  const int lane = threadIdx.x & (G - 1);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kNarrowThreads / G) + threadIdx.x / G;
+  if (row >= n) return;
+  const T* x = logits + row * ld;
+  T* out = grad + row * c;
+  const float nan = __int_as_float(0x7fffffff);
+  const int64_t y = (g.log_prob && labels) ? labels[row] : -1;
+  const float gl = y >= 0 ? (y < c ? g.log_prob[row * g.log_prob_stride] : nan) : 0.0f;
+  const float gh = g.entropy ? g.entropy[row * g.entropy_stride] : 0.0f;
+  float G_all = gl;
+  bool any = !(gl == 0.0f) || !(gh == 0.0f);
+  if (g.top)
+    for (int i = 0; i < top_k; ++i) {
+      const float v = g.top[row * top_k + i];
+      G_all += v;
+      any |= !(v == 0.0f);
+    }
+  const float2 st = *reinterpret_cast<const float2*>(stats + 2 * row);
+  // no gradient reaches the row, or it has no distribution
+  if (!any || (st.x == -INFINITY && st.y == st.y)) {
+#pragma unroll
+    for (int i = 0; i < kNarrowElems; ++i)
+      if (lane + G * i < c) out[lane + G * i] = from_f<T>(0.0f);
+    return;
+  }
+  const float H = g.entropy ? entropy[row] : 0.0f;
+  float v[kNarrowElems];
+#pragma unroll
+  for (int i = 0; i < kNarrowElems; ++i)
+    if (lane + G * i < c) v[i] = to_f(x[lane + G * i]);
+#pragma unroll
+  for (int i = 0; i < kNarrowElems; ++i) {
+    const int j = lane + G * i;
+    if (j < c) {
+      const float lp = (v[i] - st.x) - st.y;
+      const float p = expf(lp);
+      const float spread = gh * p * (fmaxf(lp, -1e30f) + H);  // lp = -inf: p = 0
+      float a = 0.0f;
+      bool special = j == y;
+      if (special) a = gl;
+      if (g.top)
+        for (int q = 0; q < top_k; ++q)
+          if (top_index[row * top_k + q] == j) {
+            a += g.top[row * top_k + q];
+            special = true;
+          }
+      const float r = special ? (a - G_all) - G_all * expm1f(lp) : -p * G_all;
+      out[j] = from_f<T>(r - spread);
+    }
+  }
+}
+
 int lp_check(int64_t n, int64_t c, int32_t x_type, int64_t ld, int32_t top_k, const char* name) {
   CIGN_REQUIRE(n >= 0 && c > 0, CIGN_ERR_INVALID_ARGUMENT, "%s: bad sizes", name);
   CIGN_REQUIRE(known_type(x_type), CIGN_ERR_INVALID_ARGUMENT, "%s: unknown element type", name);
@@ -186,6 +315,13 @@ int cign_node_log_probs_fwd(int64_t n, int64_t c, int32_t x_type, const void* lo
                CIGN_ERR_NULL_POINTER, "node_log_probs_fwd: NULL argument");
   const LogProbOut out{log_prob, entropy, stats, top_log_probs, top_index};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (c <= kNarrowMax) {
+    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c, G,
+        log_probs_narrow_fwd_kernel<T, G><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
+            n, static_cast<int>(c), static_cast<const T*>(logits), ld, labels, top_k, out)));
+    CIGN_CHECK_LAUNCH("log_probs_narrow_fwd_kernel");
+    return CIGN_OK;
+  }
   CIGN_TYPE_DISPATCH(x_type, T,
       log_probs_fwd_kernel<T><<<static_cast<unsigned>(n), kLpThreads, 0, s>>>(
           n, c, static_cast<const T*>(logits), ld, labels, top_k, out));
@@ -208,6 +344,14 @@ int cign_node_log_probs_bwd(int64_t n, int64_t c, int32_t x_type, const void* lo
   const LogProbGrads g{grad_log_prob, grad_log_prob_stride, grad_entropy, grad_entropy_stride,
                        top_k > 0 ? grad_top : nullptr};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (c <= kNarrowMax) {
+    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c, G,
+        log_probs_narrow_bwd_kernel<T, G><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
+            n, static_cast<int>(c), static_cast<const T*>(logits), ld, labels, stats, entropy,
+            top_k, top_index, g, static_cast<T*>(grad_logits))));
+    CIGN_CHECK_LAUNCH("log_probs_narrow_bwd_kernel");
+    return CIGN_OK;
+  }
   CIGN_TYPE_DISPATCH(x_type, T,
       log_probs_bwd_kernel<T><<<static_cast<unsigned>(n), kLpThreads, 0, s>>>(
           n, c, static_cast<const T*>(logits), ld, labels, stats, entropy, top_k, top_index, g,
