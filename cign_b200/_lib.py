@@ -12,6 +12,7 @@ from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t
 from pathlib import Path
 
 import torch
+from torch.autograd.function import once_differentiable
 
 LIB_PATH = Path(__file__).resolve().parent / "libcign_sm100.so"
 
@@ -280,6 +281,34 @@ def stream_on(device) -> c_void_p:
 def workspace(nbytes: int, device) -> torch.Tensor:
     """Caller-owned scratch (16-byte aligned by the caching allocator)."""
     return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+
+
+def launch(name: str, t: torch.Tensor, *args) -> None:
+    """Call the entry point `name` with `args` and, last, the current stream of
+    t's device; raises on an error status.  Pointers are plain ints (None =
+    NULL).  One call instead of load_library/DeviceGuard/stream_of/check, for
+    ops whose smallest calls take less time than those."""
+    fn = getattr(_LIB or load_library(), name)
+    idx = t.get_device()
+    stream = torch._C._cuda_getCurrentRawStream(idx)
+    if torch._C._cuda_getDevice() == idx:
+        rc = fn(*args, stream)
+    else:
+        with DeviceGuard(t.device):
+            rc = fn(*args, stream)
+    if rc != CIGN_OK:
+        check(rc, name)
+
+
+def once(backward):
+    """The backward of an autograd node whose gradient has no derivative: asking
+    for one raises, as torch's once_differentiable makes it; its bookkeeping is
+    skipped where no graph of the gradient is recorded."""
+    refusing = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (refusing if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return staticmethod(run)
 
 
 class DeviceGuard:

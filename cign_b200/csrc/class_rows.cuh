@@ -14,7 +14,8 @@ namespace cign {
 __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <typename T> __device__ __forceinline__ T from_f(float v);  // to nearest, ties to even
+template <typename T>
+__device__ __forceinline__ T from_f(float v);  // to nearest, ties to even
 template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
@@ -31,6 +32,35 @@ inline size_t type_size(int32_t t) { return t == CIGN_F32 ? 4 : 2; }
     else if ((TYPE) == CIGN_BF16) { using T = __nv_bfloat16; __VA_ARGS__; } \
     else { using T = __half; __VA_ARGS__; }                           \
   } while (0)
+
+// V neighbouring elements as one load or store: 16 bytes, or one element.
+template <typename T, int V>
+struct Pack {
+  static_assert(V == 1 || V * sizeof(T) == 16, "one element or 16 bytes");
+  T e[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
+  Pack<T, V> r;
+  if constexpr (V == 1) {
+    r.e[0] = *p;
+  } else {
+    *reinterpret_cast<uint4*>(&r) = *reinterpret_cast<const uint4*>(p);
+  }
+  return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) {
+  if constexpr (V == 1) *p = v.e[0];
+  else *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&v);
+}
+// Element i of a parameter vector of run-time type, `none` without one.
+__device__ __forceinline__ float load_param(const void* p, int32_t type, int64_t i, float none) {
+  if (p == nullptr) return none;
+  if (type == CIGN_F32) return static_cast<const float*>(p)[i];
+  if (type == CIGN_BF16) return to_f(static_cast<const __nv_bfloat16*>(p)[i]);
+  return to_f(static_cast<const __half*>(p)[i]);
+}
 
 // ---------------------------------------------------------------- block sums
 // Sum of v over the block, in lane order then warp order (fixed, so runs

@@ -8,110 +8,444 @@
 //   grad_w = sum_rows g xh,  grad_b = sum_rows g
 // Statistics, products and sums are float32 whatever the element type; y and
 // the gradients are rounded once.
+//
+// Both passes are bound by memory: a row is read once into registers, the
+// statistics are formed there (the variance from differences, so a far mean
+// costs no digits), and the result is written.  A thread holds the same
+// columns of every row that it meets, so weight, bias and the two sums of the
+// backward stay in registers over all rows of a persistent block, which writes
+// one partial sum of the parameter gradients at its end; a second kernel adds
+// the partial sums in block order.  x and g are thus read once for all three
+// gradients, and nothing is added atomically.
 #include "class_rows.cuh"
 
 namespace cign {
 namespace {
 
-constexpr int kLnThreads = 256;
-constexpr int kLnWarps = kLnThreads / 32;
-constexpr int kLnRowsPerChunk = 64;  // rows of one partial sum of the parameter gradients
+constexpr int kLnGroupThreads = 256;  // block of the kernels with several rows per block
+constexpr int kLnBlockThreads = 512;  // of a block that holds one row; the widest rows take twice that
+constexpr int kLnMaxBlocks = 1184;    // partial sums of the parameter gradients (148 SMs x 8)
+constexpr int kLnWideThreads = 256;
+constexpr int kLnWideWarps = kLnWideThreads / 32;
 
-template <typename T, typename P>
-__global__ void __launch_bounds__(kLnThreads)
-layer_norm_fwd_kernel(int64_t n, int64_t d, const T* __restrict__ x, int64_t ldx,
-                      const P* __restrict__ w, const P* __restrict__ b, float eps,
-                      T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
-  __shared__ float part[kLnWarps];
-  const float inv_d = 1.0f / static_cast<float>(d);
-  for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
-    const T* xr = x + row * ldx;
+// Sum over the lanes of a row: a group of G lanes (a power of two up to 32),
+// or with BLOCK the whole block through shared memory.  `slot` alternates
+// between two sets of partial sums, so that one barrier per sum is enough:
+// a set is written again only after the barrier of the next sum.
+template <int BLOCK>
+__device__ __forceinline__ float row_sum(float v, int G, float* part, int& slot) {
+  if constexpr (BLOCK == 0) {
+    for (int o = G >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+    return v;
+  } else {
+    v = warp_sum(v);
+    float* p = part + slot * 32;
+    slot ^= 1;
+    if ((threadIdx.x & 31) == 0) p[threadIdx.x >> 5] = v;
+    __syncthreads();
     float s = 0.0f;
-    for (int64_t j = threadIdx.x; j < d; j += kLnThreads) s += to_f(xr[j]);
-    const float mu = block_sum<kLnWarps>(s, part) * inv_d;
-    float v = 0.0f;
-    for (int64_t j = threadIdx.x; j < d; j += kLnThreads) {
-      const float a = to_f(xr[j]) - mu;
-      v = fmaf(a, a, v);
+    const int warps = blockDim.x >> 5;
+    for (int w = 0; w < warps; ++w) s += p[w];
+    return s;
+  }
+}
+
+// Two sums at once, one barrier.
+template <int BLOCK>
+__device__ __forceinline__ void row_sum2(float& a, float& b, int G, float2* part, int& slot) {
+  if constexpr (BLOCK == 0) {
+    for (int o = G >> 1; o > 0; o >>= 1) {
+      a += __shfl_xor_sync(kFullMask, a, o);
+      b += __shfl_xor_sync(kFullMask, b, o);
     }
-    const float rs = rsqrtf(block_sum<kLnWarps>(v, part) * inv_d + eps);
-    if (threadIdx.x == 0 && mean != nullptr) {
+  } else {
+    a = warp_sum(a);
+    b = warp_sum(b);
+    float2* p = part + slot * 32;
+    slot ^= 1;
+    if ((threadIdx.x & 31) == 0) p[threadIdx.x >> 5] = make_float2(a, b);
+    __syncthreads();
+    a = b = 0.0f;
+    const int warps = blockDim.x >> 5;
+    for (int w = 0; w < warps; ++w) {
+      a += p[w].x;
+      b += p[w].y;
+    }
+  }
+}
+
+struct LnRows {
+  int64_t n, d;
+  int nvec;  // d / V
+  int G;     // lanes of a row (rows share a block); the block holds one row with BLOCK
+};
+
+template <typename T, int V, int NV, int BLOCK>
+__global__ void __launch_bounds__(BLOCK ? BLOCK * kLnBlockThreads : kLnGroupThreads)
+layer_norm_fwd_kernel(LnRows p, const T* __restrict__ x, int64_t ldx, const void* __restrict__ w,
+                      const void* __restrict__ b, int32_t param_type, float eps,
+                      T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
+  __shared__ float part[64];
+  int slot = 0;
+  const int lane = BLOCK ? threadIdx.x : threadIdx.x & (p.G - 1);
+  const int lanes = BLOCK ? blockDim.x : p.G;
+  const int per_block = BLOCK ? 1 : kLnGroupThreads / p.G;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block +
+                        (BLOCK ? 0 : threadIdx.x / p.G);
+  float wv[NV][V], bv[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int c = lane + lanes * i;
+      wv[i][e] = c < p.nvec ? load_param(w, param_type, c * V + e, 1.0f) : 0.0f;
+      bv[i][e] = c < p.nvec ? load_param(b, param_type, c * V + e, 0.0f) : 0.0f;
+    }
+  const float inv_d = 1.0f / static_cast<float>(p.d);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
+  // every group of a warp takes part in the sums until the last of them is done
+  for (int64_t at = first; at - (BLOCK ? 0 : threadIdx.x / p.G) < p.n; at += step) {
+    const bool live = at < p.n;
+    const int64_t row = live ? at : p.n - 1;
+    const T* xr = x + row * ldx;
+    float xv[NV][V];
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = lane + lanes * i;
+      Pack<T, V> q;
+      if (c < p.nvec) q = load_pack<T, V>(xr + static_cast<int64_t>(c) * V);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        xv[i][e] = c < p.nvec ? to_f(q.e[e]) : 0.0f;
+        s += xv[i][e];
+      }
+    }
+    const float mu = row_sum<BLOCK>(s, p.G, part, slot) * inv_d;
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        xv[i][e] -= mu;
+        if (lane + lanes * i < p.nvec) v = fmaf(xv[i][e], xv[i][e], v);
+      }
+    const float rs = rsqrtf(row_sum<BLOCK>(v, p.G, part, slot) * inv_d + eps);
+    if (live && lane == 0 && mean != nullptr) {
       mean[row] = mu;
       rstd[row] = rs;
     }
-    for (int64_t j = threadIdx.x; j < d; j += kLnThreads) {
-      const float xh = (to_f(xr[j]) - mu) * rs;
-      y[row * d + j] = from_f<T>(fmaf(xh, w ? to_f(w[j]) : 1.0f, b ? to_f(b[j]) : 0.0f));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = lane + lanes * i;
+      Pack<T, V> q;
+#pragma unroll
+      for (int e = 0; e < V; ++e) q.e[e] = from_f<T>(fmaf(xv[i][e] * rs, wv[i][e], bv[i][e]));
+      if (live && c < p.nvec) store_pack<T, V>(y + row * p.d + static_cast<int64_t>(c) * V, q);
     }
   }
 }
 
-template <typename T, typename P>
-__global__ void __launch_bounds__(kLnThreads)
-layer_norm_bwd_x_kernel(int64_t n, int64_t d, const T* __restrict__ gy, int64_t ldg,
-                        const T* __restrict__ x, int64_t ldx, const P* __restrict__ w,
-                        const float* __restrict__ mean, const float* __restrict__ rstd,
-                        T* __restrict__ gx) {
-  __shared__ float part[kLnWarps];
-  const float inv_d = 1.0f / static_cast<float>(d);
-  for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
+// partial: [gridDim.x, 2, d] sums of g xh and g over the block's rows, or NULL.
+template <typename T, int V, int NV, int BLOCK>
+__global__ void __launch_bounds__(BLOCK ? BLOCK * kLnBlockThreads : kLnGroupThreads)
+layer_norm_bwd_kernel(LnRows p, const T* __restrict__ gy, int64_t ldg, const T* __restrict__ x,
+                      int64_t ldx, const void* __restrict__ w, int32_t param_type,
+                      const float* __restrict__ mean, const float* __restrict__ rstd,
+                      T* __restrict__ gx, float* __restrict__ partial) {
+  __shared__ float2 part[64];
+  extern __shared__ float columns[];  // BLOCK == 0: [warps, G * NV * V]
+  int slot = 0;
+  const int lane = BLOCK ? threadIdx.x : threadIdx.x & (p.G - 1);
+  const int lanes = BLOCK ? blockDim.x : p.G;
+  const int per_block = BLOCK ? 1 : kLnGroupThreads / p.G;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block +
+                        (BLOCK ? 0 : threadIdx.x / p.G);
+  float wv[NV][V], aw[NV][V], ab[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int c = lane + lanes * i;
+      wv[i][e] = c < p.nvec ? load_param(w, param_type, c * V + e, 1.0f) : 0.0f;
+      aw[i][e] = ab[i][e] = 0.0f;
+    }
+  const float inv_d = 1.0f / static_cast<float>(p.d);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
+  for (int64_t at = first; at - (BLOCK ? 0 : threadIdx.x / p.G) < p.n; at += step) {
+    const bool live = at < p.n;
+    const int64_t row = live ? at : p.n - 1;
     const T* xr = x + row * ldx;
     const T* gr = gy + row * ldg;
+    Pack<T, V> xq[NV], gq[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = lane + lanes * i;
+      if (live && c < p.nvec) {
+        xq[i] = load_pack<T, V>(xr + static_cast<int64_t>(c) * V);
+        gq[i] = load_pack<T, V>(gr + static_cast<int64_t>(c) * V);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) xq[i].e[e] = gq[i].e[e] = from_f<T>(0.0f);
+      }
+    }
     const float mu = mean[row], rs = rstd[row];
     float s1 = 0.0f, s2 = 0.0f;
-    for (int64_t j = threadIdx.x; j < d; j += kLnThreads) {
-      const float u = to_f(gr[j]) * (w ? to_f(w[j]) : 1.0f);
-      s1 += u;
-      s2 = fmaf(u, (to_f(xr[j]) - mu) * rs, s2);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float g = to_f(gq[i].e[e]);
+        const float xh = (to_f(xq[i].e[e]) - mu) * rs;
+        const float u = g * wv[i][e];
+        s1 += u;
+        s2 = fmaf(u, xh, s2);
+        if (live) {
+          aw[i][e] = fmaf(g, xh, aw[i][e]);
+          ab[i][e] += g;
+        }
+      }
+    if (gx != nullptr) {
+      row_sum2<BLOCK>(s1, s2, p.G, part, slot);
+      s1 *= inv_d;
+      s2 *= inv_d;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = lane + lanes * i;
+        Pack<T, V> q;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float xh = (to_f(xq[i].e[e]) - mu) * rs;
+          q.e[e] = from_f<T>(rs * (to_f(gq[i].e[e]) * wv[i][e] - s1 - xh * s2));
+        }
+        if (live && c < p.nvec) store_pack<T, V>(gx + row * p.d + static_cast<int64_t>(c) * V, q);
+      }
     }
-    s1 = block_sum<kLnWarps>(s1, part) * inv_d;
-    s2 = block_sum<kLnWarps>(s2, part) * inv_d;
-    for (int64_t j = threadIdx.x; j < d; j += kLnThreads) {
-      const float u = to_f(gr[j]) * (w ? to_f(w[j]) : 1.0f);
-      const float xh = (to_f(xr[j]) - mu) * rs;
-      gx[row * d + j] = from_f<T>(rs * (u - s1 - xh * s2));
+  }
+  if (partial == nullptr) return;
+  float* pw = partial + static_cast<int64_t>(blockIdx.x) * 2 * p.d;
+  if constexpr (BLOCK != 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = lane + lanes * i;
+      if (c < p.nvec)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          pw[c * V + e] = aw[i][e];
+          pw[p.d + c * V + e] = ab[i][e];
+        }
+    }
+  } else {
+    // the groups of a warp by shuffles, then the warps in order
+    const int cols = p.G * NV * V;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          float v = which == 0 ? aw[i][e] : ab[i][e];
+          for (int o = 16; o >= p.G; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+          if ((threadIdx.x & 31) < p.G)
+            columns[(threadIdx.x >> 5) * cols + (lane + p.G * i) * V + e] = v;
+        }
+      __syncthreads();
+      for (int j = threadIdx.x; j < p.d; j += kLnGroupThreads) {
+        float v = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kLnGroupThreads / 32; ++k) v += columns[k * cols + j];
+        pw[which * p.d + j] = v;
+      }
     }
   }
 }
 
-// Partial sums over one chunk of rows, rows in order; one thread per column.
+// out[j] = sum over blocks of partial[block, which, j]: a block of 16 warps
+// covers 32 columns, warp w adds its share of the blocks in order, then the
+// warps are added in order.
+constexpr int kLnSumWarps = 16;
+template <typename P>
+__global__ void __launch_bounds__(kLnSumWarps * 32)
+layer_norm_param_sum_kernel(int blocks, int64_t d, const float* __restrict__ partial,
+                            P* __restrict__ gw, P* __restrict__ gb) {
+  __shared__ float part[kLnSumWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  P* out = blockIdx.y == 0 ? gw : gb;
+  if (out == nullptr) return;
+  const int64_t j = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  const int share = (blocks + kLnSumWarps - 1) / kLnSumWarps;
+  const int b0 = warp * share, b1 = b0 + share < blocks ? b0 + share : blocks;
+  float s = 0.0f;
+  if (j < d && b0 < b1) s = ordered_sum<1>(partial + blockIdx.y * d + j, 2 * d, b0, b1);
+  part[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && j < d) {
+    float t = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kLnSumWarps; ++k) t += part[k][lane];
+    out[j] = from_f<P>(t);
+  }
+}
+
+// Rows that do not fit the registers of one block: a block per row, which
+// reads the row again for each of its sums (from L2).
 template <typename T>
-__global__ void __launch_bounds__(kLnThreads)
-layer_norm_bwd_param_kernel(int64_t n, int64_t d, const T* __restrict__ gy, int64_t ldg,
-                            const T* __restrict__ x, int64_t ldx, const float* __restrict__ mean,
-                            const float* __restrict__ rstd, float* __restrict__ pw,
-                            float* __restrict__ pb) {
-  const int64_t j = static_cast<int64_t>(blockIdx.y) * kLnThreads + threadIdx.x;
+__global__ void __launch_bounds__(kLnWideThreads)
+layer_norm_wide_fwd_kernel(int64_t n, int64_t d, const T* __restrict__ x, int64_t ldx,
+                           const void* __restrict__ w, const void* __restrict__ b,
+                           int32_t param_type, float eps, T* __restrict__ y,
+                           float* __restrict__ mean, float* __restrict__ rstd) {
+  __shared__ float part[kLnWideWarps];
+  const float inv_d = 1.0f / static_cast<float>(d);
+  const int64_t row = blockIdx.x;
+  const T* xr = x + row * ldx;
+  float s = 0.0f;
+  for (int64_t j = threadIdx.x; j < d; j += kLnWideThreads) s += to_f(xr[j]);
+  const float mu = block_sum<kLnWideWarps>(s, part) * inv_d;
+  float v = 0.0f;
+  for (int64_t j = threadIdx.x; j < d; j += kLnWideThreads) {
+    const float a = to_f(xr[j]) - mu;
+    v = fmaf(a, a, v);
+  }
+  const float rs = rsqrtf(block_sum<kLnWideWarps>(v, part) * inv_d + eps);
+  if (threadIdx.x == 0 && mean != nullptr) {
+    mean[row] = mu;
+    rstd[row] = rs;
+  }
+  for (int64_t j = threadIdx.x; j < d; j += kLnWideThreads) {
+    const float xh = (to_f(xr[j]) - mu) * rs;
+    y[row * d + j] = from_f<T>(fmaf(xh, load_param(w, param_type, j, 1.0f),
+                                    load_param(b, param_type, j, 0.0f)));
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLnWideThreads)
+layer_norm_wide_bwd_kernel(int64_t n, int64_t d, const T* __restrict__ gy, int64_t ldg,
+                           const T* __restrict__ x, int64_t ldx, const void* __restrict__ w,
+                           int32_t param_type, const float* __restrict__ mean,
+                           const float* __restrict__ rstd, T* __restrict__ gx) {
+  __shared__ float part[kLnWideWarps];
+  const float inv_d = 1.0f / static_cast<float>(d);
+  const int64_t row = blockIdx.x;
+  const T* xr = x + row * ldx;
+  const T* gr = gy + row * ldg;
+  const float mu = mean[row], rs = rstd[row];
+  float s1 = 0.0f, s2 = 0.0f;
+  for (int64_t j = threadIdx.x; j < d; j += kLnWideThreads) {
+    const float u = to_f(gr[j]) * load_param(w, param_type, j, 1.0f);
+    s1 += u;
+    s2 = fmaf(u, (to_f(xr[j]) - mu) * rs, s2);
+  }
+  s1 = block_sum<kLnWideWarps>(s1, part) * inv_d;
+  s2 = block_sum<kLnWideWarps>(s2, part) * inv_d;
+  for (int64_t j = threadIdx.x; j < d; j += kLnWideThreads) {
+    const float u = to_f(gr[j]) * load_param(w, param_type, j, 1.0f);
+    const float xh = (to_f(xr[j]) - mu) * rs;
+    gx[row * d + j] = from_f<T>(rs * (u - s1 - xh * s2));
+  }
+}
+
+// Partial sums of the parameter gradients over a chunk of rows, rows in order.
+template <typename T>
+__global__ void __launch_bounds__(kLnWideThreads)
+layer_norm_wide_param_kernel(int64_t n, int64_t d, int64_t chunk, const T* __restrict__ gy,
+                             int64_t ldg, const T* __restrict__ x, int64_t ldx,
+                             const float* __restrict__ mean, const float* __restrict__ rstd,
+                             float* __restrict__ partial) {
+  const int64_t j = static_cast<int64_t>(blockIdx.y) * kLnWideThreads + threadIdx.x;
   if (j >= d) return;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kLnRowsPerChunk;
-  const int64_t r1 = r0 + kLnRowsPerChunk < n ? r0 + kLnRowsPerChunk : n;
+  const int64_t r0 = blockIdx.x * chunk;
+  const int64_t r1 = r0 + chunk < n ? r0 + chunk : n;
   float aw = 0.0f, ab = 0.0f;
   for (int64_t r = r0; r < r1; ++r) {
     const float g = to_f(gy[r * ldg + j]);
     aw = fmaf(g, (to_f(x[r * ldx + j]) - mean[r]) * rstd[r], aw);
     ab += g;
   }
-  pw[static_cast<int64_t>(blockIdx.x) * d + j] = aw;
-  pb[static_cast<int64_t>(blockIdx.x) * d + j] = ab;
+  float* pw = partial + static_cast<int64_t>(blockIdx.x) * 2 * d;
+  pw[j] = aw;
+  pw[d + j] = ab;
 }
 
-template <typename P>
-__global__ void __launch_bounds__(kLnThreads)
-layer_norm_param_sum_kernel(int64_t chunks, int64_t d, const float* __restrict__ pw,
-                            const float* __restrict__ pb, P* __restrict__ gw,
-                            P* __restrict__ gb) {
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * kLnThreads + threadIdx.x;
-  if (j >= d) return;
-  float aw = 0.0f, ab = 0.0f;
-  for (int64_t c = 0; c < chunks; ++c) {
-    aw += pw[c * d + j];
-    ab += pb[c * d + j];
+// How a row of nvec loads is spread: lanes of a group, or threads of a block,
+// and loads per thread.
+struct LnShape {
+  bool fits = false, block = false;
+  int lanes = 0, nv = 0;
+};
+LnShape ln_shape(int64_t nvec, int max_nv_group, int max_nv_block) {
+  LnShape s;
+  for (int g = 4; g <= 32; g *= 2)
+    if (nvec <= static_cast<int64_t>(g) * max_nv_group) {
+      s.fits = true;
+      s.lanes = g;
+      s.nv = static_cast<int>((nvec + g - 1) / g);
+      return s;
+    }
+  for (int nv = 1; nv <= max_nv_block; nv *= 2) {
+    const int64_t t = ((nvec + nv - 1) / nv + 31) / 32 * 32;
+    if (t <= kLnBlockThreads || (nv == max_nv_block && t <= 2 * kLnBlockThreads)) {
+      s.fits = s.block = true;
+      s.lanes = static_cast<int>(t);
+      s.nv = nv;
+      return s;
+    }
   }
-  if (gw) gw[j] = from_f<P>(aw);
-  if (gb) gb[j] = from_f<P>(ab);
+  return s;
+}
+// Loads of 16 bytes where every row of every matrix starts on 16 bytes and
+// the width is a whole number of them; else of one element.
+template <typename T>
+LnShape ln_shape_of(int64_t d, bool wide_loads, int* vec) {
+  constexpr int V = 16 / sizeof(T);
+  *vec = wide_loads ? V : 1;
+  return wide_loads ? ln_shape(d / V, 16 / V, 16 / V) : ln_shape(d, 16, 16);
 }
 
-int64_t ln_chunks(int64_t n) { return (n + kLnRowsPerChunk - 1) / kLnRowsPerChunk; }
+#define CIGN_LN_NV(V_, NV_, BLOCK_, ...)                                \
+  { constexpr int V = V_, NV = NV_, BLOCK = BLOCK_; __VA_ARGS__; }
+// CALL with V, NV (loads per thread, rounded up) and BLOCK (0: rows share a
+// block; 1, 2: a row per block of at most that many times kLnBlockThreads).
+#define CIGN_LN_DISPATCH(T, vec, shape, ...)                                             \
+  do {                                                                                   \
+    constexpr int kV = 16 / sizeof(T), kMost = 16 / kV;                                  \
+    const int nv_ = (shape).nv;                                                          \
+    if ((vec) > 1 && !(shape).block) {                                                   \
+      if (nv_ <= 1) CIGN_LN_NV(kV, 1, 0, __VA_ARGS__)                                    \
+      else if (nv_ <= 2) CIGN_LN_NV(kV, 2, 0, __VA_ARGS__)                               \
+      else if (nv_ <= 3) CIGN_LN_NV(kV, (kMost < 3 ? kMost : 3), 0, __VA_ARGS__)         \
+      else CIGN_LN_NV(kV, kMost, 0, __VA_ARGS__)                                         \
+    } else if ((vec) > 1) {                                                              \
+      if (nv_ <= 1) CIGN_LN_NV(kV, 1, 1, __VA_ARGS__)                                    \
+      else if (nv_ <= 2 && (shape).lanes <= kLnBlockThreads)                             \
+        CIGN_LN_NV(kV, 2, 1, __VA_ARGS__)                                                \
+      else if ((shape).lanes <= kLnBlockThreads) CIGN_LN_NV(kV, kMost, 1, __VA_ARGS__)   \
+      else CIGN_LN_NV(kV, kMost, 2, __VA_ARGS__)                                         \
+    } else if (!(shape).block) {                                                         \
+      if (nv_ <= 2) CIGN_LN_NV(1, 2, 0, __VA_ARGS__)                                     \
+      else if (nv_ <= 4) CIGN_LN_NV(1, 4, 0, __VA_ARGS__)                                \
+      else if (nv_ <= 8) CIGN_LN_NV(1, 8, 0, __VA_ARGS__)                                \
+      else if (nv_ <= 12) CIGN_LN_NV(1, 12, 0, __VA_ARGS__)                              \
+      else CIGN_LN_NV(1, 16, 0, __VA_ARGS__)                                             \
+    } else {                                                                             \
+      if (nv_ <= 2) CIGN_LN_NV(1, 2, 1, __VA_ARGS__)                                     \
+      else if (nv_ <= 4) CIGN_LN_NV(1, 4, 1, __VA_ARGS__)                                \
+      else if (nv_ <= 8) CIGN_LN_NV(1, 8, 1, __VA_ARGS__)                                \
+      else if ((shape).lanes <= kLnBlockThreads) CIGN_LN_NV(1, 16, 1, __VA_ARGS__)       \
+      else CIGN_LN_NV(1, 16, 2, __VA_ARGS__)                                             \
+    }                                                                                    \
+  } while (0)
+
+bool rows_aligned16(const void* p, int64_t ld, size_t size) {
+  return p == nullptr || (aligned16(p) && (ld * size) % 16 == 0);
+}
+
+int64_t ln_wide_chunk(int64_t n) {
+  const int64_t c = (n + kLnMaxBlocks - 1) / kLnMaxBlocks;
+  return c < 16 ? 16 : c;
+}
 
 int ln_check(int64_t n, int64_t d, int32_t x_type, int32_t param_type, const char* name) {
   CIGN_REQUIRE(n >= 0 && d > 0, CIGN_ERR_INVALID_ARGUMENT, "%s: bad sizes", name);
@@ -119,6 +453,83 @@ int ln_check(int64_t n, int64_t d, int32_t x_type, int32_t param_type, const cha
                "%s: unknown element type", name);
   CIGN_REQUIRE(n < (1ll << 31) && d < (1ll << 24), CIGN_ERR_UNSUPPORTED,
                "%s: at most 2^31 - 1 rows of at most 2^24 - 1 columns", name);
+  return CIGN_OK;
+}
+
+template <typename T>
+int ln_fwd(int64_t n, int64_t d, const T* x, int64_t ldx, const void* w, const void* b,
+           int32_t param_type, float eps, T* y, float* mean, float* rstd, cudaStream_t s) {
+  int vec;
+  const bool wide_loads = d % (16 / sizeof(T)) == 0 && rows_aligned16(x, ldx, sizeof(T)) &&
+                          aligned16(y);
+  const LnShape shape = ln_shape_of<T>(d, wide_loads, &vec);
+  if (!shape.fits) {
+    layer_norm_wide_fwd_kernel<T><<<static_cast<unsigned>(n), kLnWideThreads, 0, s>>>(
+        n, d, x, ldx, w, b, param_type, eps, y, mean, rstd);
+    CIGN_CHECK_LAUNCH("layer_norm_wide_fwd_kernel");
+    return CIGN_OK;
+  }
+  const LnRows p{n, d, static_cast<int>(d / vec), shape.block ? 32 : shape.lanes};
+  const int threads = shape.block ? shape.lanes : kLnGroupThreads;
+  const int64_t blocks = shape.block ? n : (n + threads / shape.lanes - 1) / (threads / shape.lanes);
+  const int64_t resident = static_cast<int64_t>(sm_count()) * (2048 / threads);
+  const unsigned grid = static_cast<unsigned>(blocks < resident ? blocks : resident);
+  CIGN_LN_DISPATCH(T, vec, shape,
+      (layer_norm_fwd_kernel<T, V, NV, BLOCK><<<grid, threads, 0, s>>>(
+          p, x, ldx, w, b, param_type, eps, y, mean, rstd)));
+  CIGN_CHECK_LAUNCH("layer_norm_fwd_kernel");
+  return CIGN_OK;
+}
+
+template <typename T>
+int ln_bwd(int64_t n, int64_t d, const T* gy, int64_t ldg, const T* x, int64_t ldx, const void* w,
+           int32_t param_type, const float* mean, const float* rstd, T* gx, void* gw, void* gb,
+           float* partial, cudaStream_t s) {
+  int vec;
+  const bool wide_loads = d % (16 / sizeof(T)) == 0 && rows_aligned16(x, ldx, sizeof(T)) &&
+                          rows_aligned16(gy, ldg, sizeof(T)) && aligned16(gx);
+  const LnShape shape = ln_shape_of<T>(d, wide_loads, &vec);
+  const bool params = gw != nullptr || gb != nullptr;
+  int sums = 0;
+  if (!shape.fits) {
+    if (gx) {
+      layer_norm_wide_bwd_kernel<T><<<static_cast<unsigned>(n), kLnWideThreads, 0, s>>>(
+          n, d, gy, ldg, x, ldx, w, param_type, mean, rstd, gx);
+      CIGN_CHECK_LAUNCH("layer_norm_wide_bwd_kernel");
+    }
+    if (params) {
+      const int64_t chunk = ln_wide_chunk(n);
+      sums = static_cast<int>((n + chunk - 1) / chunk);
+      const unsigned cols = static_cast<unsigned>((d + kLnWideThreads - 1) / kLnWideThreads);
+      CIGN_REQUIRE(cols < 65536, CIGN_ERR_UNSUPPORTED, "layer_norm_bwd: too many columns");
+      layer_norm_wide_param_kernel<T><<<dim3(sums, cols), kLnWideThreads, 0, s>>>(
+          n, d, chunk, gy, ldg, x, ldx, mean, rstd, partial);
+      CIGN_CHECK_LAUNCH("layer_norm_wide_param_kernel");
+    }
+  } else if (gx || params) {
+    const LnRows p{n, d, static_cast<int>(d / vec), shape.block ? 32 : shape.lanes};
+    const int threads = shape.block ? shape.lanes : kLnGroupThreads;
+    const int64_t blocks =
+        shape.block ? n : (n + threads / shape.lanes - 1) / (threads / shape.lanes);
+    int64_t resident = static_cast<int64_t>(sm_count()) *
+                       (shape.block ? (1024 / threads > 1 ? 1024 / threads : 1) : 3);
+    if (resident > kLnMaxBlocks) resident = kLnMaxBlocks;
+    sums = static_cast<int>(blocks < resident ? blocks : resident);
+    CIGN_LN_DISPATCH(T, vec, shape, {
+      const size_t smem =
+          BLOCK != 0 ? 0 : static_cast<size_t>(kLnGroupThreads / 32) * p.G * NV * V * sizeof(float);
+      layer_norm_bwd_kernel<T, V, NV, BLOCK><<<sums, threads, smem, s>>>(
+          p, gy, ldg, x, ldx, w, param_type, mean, rstd, gx, params ? partial : nullptr);
+    });
+    CIGN_CHECK_LAUNCH("layer_norm_bwd_kernel");
+  }
+  if (params) {
+    const dim3 grid(static_cast<unsigned>((d + 31) / 32), 2);
+    CIGN_TYPE_DISPATCH(param_type, P,
+        (layer_norm_param_sum_kernel<P><<<grid, kLnSumWarps * 32, 0, s>>>(
+            sums, d, partial, static_cast<P*>(gw), static_cast<P*>(gb))));
+    CIGN_CHECK_LAUNCH("layer_norm_param_sum_kernel");
+  }
   return CIGN_OK;
 }
 
@@ -140,17 +551,14 @@ int cign_layer_norm_fwd(int64_t n, int64_t d, int32_t x_type, int32_t param_type
   CIGN_REQUIRE(x && y && (mean == nullptr) == (rstd == nullptr), CIGN_ERR_NULL_POINTER,
                "layer_norm_fwd: NULL argument");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  CIGN_TYPE_DISPATCH(x_type, T, CIGN_TYPE_DISPATCH(param_type, P,
-      layer_norm_fwd_kernel<T, P><<<static_cast<unsigned>(n), kLnThreads, 0, s>>>(
-          n, d, static_cast<const T*>(x), ldx, static_cast<const P*>(w),
-          static_cast<const P*>(b), eps, static_cast<T*>(y), mean, rstd)));
-  CIGN_CHECK_LAUNCH("layer_norm_fwd_kernel");
-  return CIGN_OK;
+  CIGN_TYPE_DISPATCH(x_type, T,
+      return ln_fwd<T>(n, d, static_cast<const T*>(x), ldx, w, b, param_type, eps,
+                       static_cast<T*>(y), mean, rstd, s));
 }
 
 size_t cign_layer_norm_bwd_workspace_bytes(int64_t n, int64_t d) {
   if (n <= 0 || d <= 0) return 0;
-  return 2 * static_cast<size_t>(ln_chunks(n)) * d * sizeof(float);
+  return 2 * static_cast<size_t>(n < kLnMaxBlocks ? n : kLnMaxBlocks) * d * sizeof(float);
 }
 
 int cign_layer_norm_bwd(int64_t n, int64_t d, int32_t x_type, int32_t param_type, const void* gy,
@@ -169,38 +577,17 @@ int cign_layer_norm_bwd(int64_t n, int64_t d, int32_t x_type, int32_t param_type
     return CIGN_OK;
   }
   CIGN_REQUIRE(gy && x && mean && rstd, CIGN_ERR_NULL_POINTER, "layer_norm_bwd: NULL argument");
-  const bool params = gw != nullptr || gb != nullptr;
-  if (params) {
+  if (gw != nullptr || gb != nullptr) {
     const size_t need = cign_layer_norm_bwd_workspace_bytes(n, d);
     CIGN_REQUIRE(ws != nullptr && ws_bytes >= need, CIGN_ERR_INVALID_ARGUMENT,
                  "layer_norm_bwd: workspace too small (%zu < %zu bytes)", ws_bytes, need);
     CIGN_REQUIRE(aligned16(ws), CIGN_ERR_ALIGNMENT,
                  "layer_norm_bwd: ws must be 16-byte aligned");
   }
-  if (gx) {
-    CIGN_TYPE_DISPATCH(x_type, T, CIGN_TYPE_DISPATCH(param_type, P,
-        layer_norm_bwd_x_kernel<T, P><<<static_cast<unsigned>(n), kLnThreads, 0, s>>>(
-            n, d, static_cast<const T*>(gy), ldg, static_cast<const T*>(x), ldx,
-            static_cast<const P*>(w), mean, rstd, static_cast<T*>(gx))));
-    CIGN_CHECK_LAUNCH("layer_norm_bwd_x_kernel");
-  }
-  if (params) {
-    const int64_t chunks = ln_chunks(n);
-    float* pw = static_cast<float*>(ws);
-    float* pb = pw + chunks * d;
-    const unsigned cols = static_cast<unsigned>((d + kLnThreads - 1) / kLnThreads);
-    CIGN_REQUIRE(cols < 65536, CIGN_ERR_UNSUPPORTED, "layer_norm_bwd: too many columns");
-    CIGN_TYPE_DISPATCH(x_type, T,
-        layer_norm_bwd_param_kernel<T><<<dim3(static_cast<unsigned>(chunks), cols), kLnThreads, 0,
-                                          s>>>(n, d, static_cast<const T*>(gy), ldg,
-                                               static_cast<const T*>(x), ldx, mean, rstd, pw, pb));
-    CIGN_CHECK_LAUNCH("layer_norm_bwd_param_kernel");
-    CIGN_TYPE_DISPATCH(param_type, P,
-        layer_norm_param_sum_kernel<P><<<cols, kLnThreads, 0, s>>>(
-            chunks, d, pw, pb, static_cast<P*>(gw), static_cast<P*>(gb)));
-    CIGN_CHECK_LAUNCH("layer_norm_param_sum_kernel");
-  }
-  return CIGN_OK;
+  CIGN_TYPE_DISPATCH(x_type, T,
+      return ln_bwd<T>(n, d, static_cast<const T*>(gy), ldg, static_cast<const T*>(x), ldx, w,
+                       param_type, mean, rstd, static_cast<T*>(gx), gw, gb,
+                       static_cast<float*>(ws), s));
 }
 
 }  // extern "C"

@@ -5,7 +5,6 @@ them, with the gradient of the student's logits (cign_distill_fwd/_bwd).
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -16,21 +15,18 @@ _INDEX_CODES = {torch.int32: 0, torch.int64: 1}
 
 
 def _teacher_args(values, ld_v, index, ld_i):
-    return (values.size(1), _lib.TYPE_CODES[values.dtype], _lib.ptr(values), ld_v,
-            _INDEX_CODES[index.dtype], _lib.ptr(index), ld_i)
+    return (values.size(1), _lib.TYPE_CODES[values.dtype], values.data_ptr(), ld_v,
+            _INDEX_CODES[index.dtype], index.data_ptr(), ld_i)
 
 
 def _forward(logits, ld, values, ld_v, index, ld_i, temperature, tail, need_stats):
-    lib = _lib.load_library()
     n, c = logits.shape
     dev = logits.device
     loss = torch.empty((n,), dtype=torch.float32, device=dev)
     stats = torch.empty((n, 8), dtype=torch.float32, device=dev) if need_stats else None
-    with _lib.DeviceGuard(dev):
-        rc = lib.cign_distill_fwd(n, c, _lib.TYPE_CODES[logits.dtype], _lib.ptr(logits), ld,
-                                  *_teacher_args(values, ld_v, index, ld_i), temperature, tail,
-                                  _lib.ptr(loss), _lib.ptr(stats), _lib.stream_of(logits))
-    _lib.check(rc, "cign_distill_fwd")
+    _lib.launch("cign_distill_fwd", logits, n, c, _lib.TYPE_CODES[logits.dtype], logits.data_ptr(),
+                ld, *_teacher_args(values, ld_v, index, ld_i), temperature, tail, loss.data_ptr(),
+                None if stats is None else stats.data_ptr())
     return loss, stats
 
 
@@ -45,20 +41,15 @@ class _DistillFn(torch.autograd.Function):
         ctx.args = ld, ld_v, ld_i, temperature, tail
         return loss
 
-    @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, g_loss):
-        lib = _lib.load_library()
         logits, values, index, stats = ctx.saved_tensors
         ld, ld_v, ld_i, temperature, tail = ctx.args
         n, c = logits.shape
-        grad = torch.empty((n, c), dtype=logits.dtype, device=logits.device)
-        with _lib.DeviceGuard(logits.device):
-            rc = lib.cign_distill_bwd(n, c, _lib.TYPE_CODES[logits.dtype], _lib.ptr(logits), ld,
-                                      *_teacher_args(values, ld_v, index, ld_i), temperature, tail,
-                                      _lib.ptr(stats), _lib.ptr(g_loss), g_loss.stride(0),
-                                      _lib.ptr(grad), _lib.stream_of(logits))
-        _lib.check(rc, "cign_distill_bwd")
+        grad = logits.new_empty((n, c))
+        _lib.launch("cign_distill_bwd", logits, n, c, _lib.TYPE_CODES[logits.dtype],
+                    logits.data_ptr(), ld, *_teacher_args(values, ld_v, index, ld_i), temperature,
+                    tail, stats.data_ptr(), g_loss.data_ptr(), g_loss.stride(0), grad.data_ptr())
         return grad, None, None, None, None
 
 

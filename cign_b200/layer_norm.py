@@ -14,62 +14,58 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
 
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _forward(x, ldx, weight, bias, eps, need_stats):
-    lib = _lib.load_library()
     n, d = x.shape
-    y = torch.empty((n, d), dtype=x.dtype, device=x.device)
-    mean = rstd = None
-    if need_stats:
-        mean, rstd = torch.empty((2, n), dtype=torch.float32, device=x.device).unbind(0)
-    param = weight if weight is not None else bias
-    with _lib.DeviceGuard(x.device):
-        rc = lib.cign_layer_norm_fwd(n, d, _lib.TYPE_CODES[x.dtype],
-                                     _lib.TYPE_CODES[x.dtype if param is None else param.dtype],
-                                     _lib.ptr(x), ldx, _lib.ptr(weight), _lib.ptr(bias), eps,
-                                     _lib.ptr(y), _lib.ptr(mean), _lib.ptr(rstd),
-                                     _lib.stream_of(x))
-    _lib.check(rc, "cign_layer_norm_fwd")
-    return y, mean, rstd
+    y = x.new_empty((n, d))
+    param = x if weight is None and bias is None else (bias if weight is None else weight)
+    stats = mean = rstd = None
+    if need_stats:  # mean [n], then rstd [n]
+        stats = torch.empty((2 * n,), dtype=torch.float32, device=x.device)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * n
+    _lib.launch("cign_layer_norm_fwd", x, n, d, _lib.TYPE_CODES[x.dtype],
+                _lib.TYPE_CODES[param.dtype], x.data_ptr(), ldx, _ptr(weight), _ptr(bias), eps,
+                y.data_ptr(), mean, rstd)
+    return y, stats
 
 
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         rows, ldx = _lib.rows_of(x)
-        y, mean, rstd = _forward(rows, ldx, weight, bias, eps, True)
-        ctx.save_for_backward(rows, weight, mean, rstd)
+        y, stats = _forward(rows, ldx, weight, bias, eps, True)
+        ctx.save_for_backward(rows, weight, stats)
         ctx.ldx = ldx
         ctx.bias_dtype = None if bias is None else bias.dtype
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, gy):
-        lib = _lib.load_library()
-        x, weight, mean, rstd = ctx.saved_tensors
+        x, weight, stats = ctx.saved_tensors
         n, d = x.shape
-        dev = x.device
         gy, ldg = _lib.rows_of(gy)
         want_x, want_w, want_b, _ = ctx.needs_input_grad
-        gx = torch.empty((n, d), dtype=x.dtype, device=dev) if want_x else None
-        gw = torch.empty((d,), dtype=weight.dtype, device=dev) if want_w else None
-        gb = torch.empty((d,), dtype=ctx.bias_dtype, device=dev) if want_b else None
-        param = x.dtype if weight is None and ctx.bias_dtype is None else (
-            ctx.bias_dtype if weight is None else weight.dtype)
-        ws = _lib.workspace(lib.cign_layer_norm_bwd_workspace_bytes(n, d) if want_w or want_b
-                            else 0, dev)
-        with _lib.DeviceGuard(dev):
-            rc = lib.cign_layer_norm_bwd(n, d, _lib.TYPE_CODES[x.dtype], _lib.TYPE_CODES[param],
-                                         _lib.ptr(gy), ldg, _lib.ptr(x), ctx.ldx,
-                                         _lib.ptr(weight), _lib.ptr(mean), _lib.ptr(rstd),
-                                         _lib.ptr(gx), _lib.ptr(gw), _lib.ptr(gb), _lib.ptr(ws),
-                                         ws.numel(), _lib.stream_of(x))
-        _lib.check(rc, "cign_layer_norm_bwd")
+        param = ctx.bias_dtype or (x if weight is None else weight).dtype
+        gx = x.new_empty((n, d)) if want_x else None
+        gw = weight.new_empty((d,)) if want_w else None
+        gb = torch.empty((d,), dtype=ctx.bias_dtype, device=x.device) if want_b else None
+        ws, ws_bytes = None, 0
+        if want_w or want_b:
+            ws_bytes = _lib.load_library().cign_layer_norm_bwd_workspace_bytes(n, d)
+            ws = _lib.workspace(ws_bytes, x.device)
+        mean = stats.data_ptr()
+        _lib.launch("cign_layer_norm_bwd", x, n, d, _lib.TYPE_CODES[x.dtype],
+                    _lib.TYPE_CODES[param], gy.data_ptr(), ldg, x.data_ptr(), ctx.ldx,
+                    _ptr(weight), mean, mean + 4 * n, _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws),
+                    ws_bytes)
         return gx, gw, gb, None
 
 

@@ -12,7 +12,6 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -26,8 +25,11 @@ class NodeLogProbs(NamedTuple):
     top_index: Optional[torch.Tensor]      # [N, top_k] int64
 
 
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _forward(logits, ld, labels, top_k, need_stats):
-    lib = _lib.load_library()
     n, c = logits.shape
     dev = logits.device
     log_prob = None if labels is None else torch.empty((n,), dtype=torch.float32, device=dev)
@@ -37,12 +39,9 @@ def _forward(logits, ld, labels, top_k, need_stats):
     if top_k:
         top = torch.empty((n, top_k), dtype=torch.float32, device=dev)
         index = torch.empty((n, top_k), dtype=torch.int64, device=dev)
-    with _lib.DeviceGuard(dev):
-        rc = lib.cign_node_log_probs_fwd(n, c, _lib.TYPE_CODES[logits.dtype], _lib.ptr(logits), ld,
-                                         _lib.ptr(labels), top_k, _lib.ptr(log_prob),
-                                         _lib.ptr(entropy), _lib.ptr(stats), _lib.ptr(top),
-                                         _lib.ptr(index), _lib.stream_of(logits))
-    _lib.check(rc, "cign_node_log_probs_fwd")
+    _lib.launch("cign_node_log_probs_fwd", logits, n, c, _lib.TYPE_CODES[logits.dtype],
+                logits.data_ptr(), ld, _ptr(labels), top_k, _ptr(log_prob), entropy.data_ptr(),
+                _ptr(stats), _ptr(top), _ptr(index))
     return log_prob, entropy, top, index, stats
 
 
@@ -59,24 +58,19 @@ class _NodeLogProbsFn(torch.autograd.Function):
             ctx.mark_non_differentiable(index)
         return log_prob, entropy, top, index
 
-    @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, g_log_prob, g_entropy, g_top, _):
         if g_log_prob is None and g_entropy is None and g_top is None:
             return None, None, None
-        lib = _lib.load_library()
         logits, labels, stats, entropy, index = ctx.saved_tensors
         n, c = logits.shape
-        grad = torch.empty((n, c), dtype=logits.dtype, device=logits.device)
+        grad = logits.new_empty((n, c))
         g_top = None if g_top is None else g_top.contiguous()
-        with _lib.DeviceGuard(logits.device):
-            rc = lib.cign_node_log_probs_bwd(
-                n, c, _lib.TYPE_CODES[logits.dtype], _lib.ptr(logits), ctx.ld, _lib.ptr(labels),
-                _lib.ptr(stats), _lib.ptr(entropy), ctx.top_k, _lib.ptr(index),
-                _lib.ptr(g_log_prob), 0 if g_log_prob is None else g_log_prob.stride(0),
-                _lib.ptr(g_entropy), 0 if g_entropy is None else g_entropy.stride(0),
-                _lib.ptr(g_top), _lib.ptr(grad), _lib.stream_of(logits))
-        _lib.check(rc, "cign_node_log_probs_bwd")
+        _lib.launch("cign_node_log_probs_bwd", logits, n, c, _lib.TYPE_CODES[logits.dtype],
+                    logits.data_ptr(), ctx.ld, _ptr(labels), stats.data_ptr(), entropy.data_ptr(),
+                    ctx.top_k, _ptr(index), _ptr(g_log_prob),
+                    0 if g_log_prob is None else g_log_prob.stride(0), _ptr(g_entropy),
+                    0 if g_entropy is None else g_entropy.stride(0), _ptr(g_top), grad.data_ptr())
         return grad, None, None
 
 
