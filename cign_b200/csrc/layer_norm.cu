@@ -17,6 +17,8 @@
 // one partial sum of the parameter gradients at its end; a second kernel adds
 // the partial sums in block order.  x and g are thus read once for all three
 // gradients, and nothing is added atomically.
+#include <atomic>
+
 #include "class_rows.cuh"
 
 namespace cign {
@@ -24,7 +26,7 @@ namespace {
 
 constexpr int kLnGroupThreads = 256;  // block of the kernels with several rows per block
 constexpr int kLnBlockThreads = 512;  // of a block that holds one row; the widest rows take twice that
-constexpr int kLnMaxBlocks = 1184;    // partial sums of the parameter gradients (148 SMs x 8)
+constexpr int kLnMaxBlocks = 1776;    // partial sums of the parameter gradients (148 SMs x 12)
 constexpr int kLnWideThreads = 256;
 constexpr int kLnWideWarps = kLnWideThreads / 32;
 
@@ -80,6 +82,21 @@ struct LnRows {
   int G;     // lanes of a row (rows share a block); the block holds one row with BLOCK
 };
 
+// This thread's columns of row `at`, or of the last row; columns behind the
+// last are loaded from it (the caller drops them).  No load depends on a
+// branch, so all are in flight together, and the callers ask for a row while
+// they work on the one before.
+template <typename T, int V, int NV>
+__device__ __forceinline__ void load_row(Pack<T, V> (&q)[NV], const T* base, int64_t ld,
+                                         int64_t at, const LnRows& p, int lane, int lanes) {
+  const T* r = base + (at < p.n ? at : p.n - 1) * ld;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = lane + lanes * i;
+    q[i] = load_pack<T, V>(r + static_cast<int64_t>(c < p.nvec ? c : p.nvec - 1) * V);
+  }
+}
+
 template <typename T, int V, int NV, int BLOCK>
 __global__ void __launch_bounds__(BLOCK ? BLOCK * kLnBlockThreads : kLnGroupThreads)
 layer_norm_fwd_kernel(LnRows p, const T* __restrict__ x, int64_t ldx, const void* __restrict__ w,
@@ -104,23 +121,22 @@ layer_norm_fwd_kernel(LnRows p, const T* __restrict__ x, int64_t ldx, const void
   const float inv_d = 1.0f / static_cast<float>(p.d);
   const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
   // every group of a warp takes part in the sums until the last of them is done
-  for (int64_t at = first; at - (BLOCK ? 0 : threadIdx.x / p.G) < p.n; at += step) {
+  const int64_t off = BLOCK ? 0 : threadIdx.x / p.G;
+  Pack<T, V> next[NV];
+  load_row<T, V, NV>(next, x, ldx, first, p, lane, lanes);
+  for (int64_t at = first; at - off < p.n; at += step) {
     const bool live = at < p.n;
     const int64_t row = live ? at : p.n - 1;
-    const T* xr = x + row * ldx;
     float xv[NV][V];
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = lane + lanes * i;
-      Pack<T, V> q;
-      if (c < p.nvec) q = load_pack<T, V>(xr + static_cast<int64_t>(c) * V);
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        xv[i][e] = c < p.nvec ? to_f(q.e[e]) : 0.0f;
+        xv[i][e] = lane + lanes * i < p.nvec ? to_f(next[i].e[e]) : 0.0f;
         s += xv[i][e];
       }
-    }
+    load_row<T, V, NV>(next, x, ldx, at + step, p, lane, lanes);
     const float mu = row_sum<BLOCK>(s, p.G, part, slot) * inv_d;
     float v = 0.0f;
 #pragma unroll
@@ -172,23 +188,25 @@ layer_norm_bwd_kernel(LnRows p, const T* __restrict__ gy, int64_t ldg, const T* 
     }
   const float inv_d = 1.0f / static_cast<float>(p.d);
   const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
-  for (int64_t at = first; at - (BLOCK ? 0 : threadIdx.x / p.G) < p.n; at += step) {
+  const int64_t off = BLOCK ? 0 : threadIdx.x / p.G;
+  Pack<T, V> xn[NV], gn[NV];
+  load_row<T, V, NV>(xn, x, ldx, first, p, lane, lanes);
+  load_row<T, V, NV>(gn, gy, ldg, first, p, lane, lanes);
+  for (int64_t at = first; at - off < p.n; at += step) {
     const bool live = at < p.n;
     const int64_t row = live ? at : p.n - 1;
-    const T* xr = x + row * ldx;
-    const T* gr = gy + row * ldg;
     Pack<T, V> xq[NV], gq[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = lane + lanes * i;
-      if (live && c < p.nvec) {
-        xq[i] = load_pack<T, V>(xr + static_cast<int64_t>(c) * V);
-        gq[i] = load_pack<T, V>(gr + static_cast<int64_t>(c) * V);
-      } else {
+      const bool in = live && lane + lanes * i < p.nvec;
 #pragma unroll
-        for (int e = 0; e < V; ++e) xq[i].e[e] = gq[i].e[e] = from_f<T>(0.0f);
+      for (int e = 0; e < V; ++e) {
+        xq[i].e[e] = in ? xn[i].e[e] : from_f<T>(0.0f);
+        gq[i].e[e] = in ? gn[i].e[e] : from_f<T>(0.0f);
       }
     }
+    load_row<T, V, NV>(xn, x, ldx, at + step, p, lane, lanes);
+    load_row<T, V, NV>(gn, gy, ldg, at + step, p, lane, lanes);
     const float mu = mean[row], rs = rstd[row];
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
@@ -384,13 +402,19 @@ LnShape ln_shape(int64_t nvec, int max_nv_group, int max_nv_block) {
       s.nv = static_cast<int>((nvec + g - 1) / g);
       return s;
     }
-  for (int nv = 1; nv <= max_nv_block; nv *= 2) {
+  // the work of a row: its loads, the idle ones among them, and what every
+  // thread of the row pays once (its share of the sum and the barrier), which
+  // takes about as long as one load's elements
+  int64_t best = 0;
+  for (int nv = max_nv_block; nv >= 1; nv = nv > 4 ? nv - 4 : nv - 1) {
     const int64_t t = ((nvec + nv - 1) / nv + 31) / 32 * 32;
-    if (t <= kLnBlockThreads || (nv == max_nv_block && t <= 2 * kLnBlockThreads)) {
+    if (t > (nv == max_nv_block ? 2 : 1) * kLnBlockThreads) continue;
+    const int64_t cost = t * (nv + (max_nv_block > 4 ? 4 : 1));
+    if (!s.fits || cost < best) {
+      best = cost;
       s.fits = s.block = true;
       s.lanes = static_cast<int>(t);
       s.nv = nv;
-      return s;
     }
   }
   return s;
@@ -421,6 +445,8 @@ LnShape ln_shape_of(int64_t d, bool wide_loads, int* vec) {
       if (nv_ <= 1) CIGN_LN_NV(kV, 1, 1, __VA_ARGS__)                                    \
       else if (nv_ <= 2 && (shape).lanes <= kLnBlockThreads)                             \
         CIGN_LN_NV(kV, 2, 1, __VA_ARGS__)                                                \
+      else if (nv_ <= 3 && (shape).lanes <= kLnBlockThreads)                             \
+        CIGN_LN_NV(kV, (kMost < 3 ? kMost : 3), 1, __VA_ARGS__)                          \
       else if ((shape).lanes <= kLnBlockThreads) CIGN_LN_NV(kV, kMost, 1, __VA_ARGS__)   \
       else CIGN_LN_NV(kV, kMost, 2, __VA_ARGS__)                                         \
     } else if (!(shape).block) {                                                         \
@@ -433,10 +459,27 @@ LnShape ln_shape_of(int64_t d, bool wide_loads, int* vec) {
       if (nv_ <= 2) CIGN_LN_NV(1, 2, 1, __VA_ARGS__)                                     \
       else if (nv_ <= 4) CIGN_LN_NV(1, 4, 1, __VA_ARGS__)                                \
       else if (nv_ <= 8) CIGN_LN_NV(1, 8, 1, __VA_ARGS__)                                \
+      else if (nv_ <= 12) CIGN_LN_NV(1, 12, 1, __VA_ARGS__)                              \
       else if ((shape).lanes <= kLnBlockThreads) CIGN_LN_NV(1, 16, 1, __VA_ARGS__)       \
       else CIGN_LN_NV(1, 16, 2, __VA_ARGS__)                                             \
     }                                                                                    \
   } while (0)
+
+// Blocks of `kernel` that the device holds at once: the grid of a persistent
+// kernel.  Asked once per kernel and block size.
+template <auto kernel>
+int64_t resident_blocks(int threads, size_t smem) {
+  static std::atomic<int> known[2 * kLnBlockThreads / 32 + 1];
+  std::atomic<int>& k = known[threads / 32];
+  int per_sm = k.load(std::memory_order_relaxed);
+  if (per_sm == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem) !=
+            cudaSuccess || per_sm < 1)
+      per_sm = 1;
+    k.store(per_sm, std::memory_order_relaxed);
+  }
+  return static_cast<int64_t>(per_sm) * sm_count();
+}
 
 bool rows_aligned16(const void* p, int64_t ld, size_t size) {
   return p == nullptr || (aligned16(p) && (ld * size) % 16 == 0);
@@ -472,11 +515,12 @@ int ln_fwd(int64_t n, int64_t d, const T* x, int64_t ldx, const void* w, const v
   const LnRows p{n, d, static_cast<int>(d / vec), shape.block ? 32 : shape.lanes};
   const int threads = shape.block ? shape.lanes : kLnGroupThreads;
   const int64_t blocks = shape.block ? n : (n + threads / shape.lanes - 1) / (threads / shape.lanes);
-  const int64_t resident = static_cast<int64_t>(sm_count()) * (2048 / threads);
-  const unsigned grid = static_cast<unsigned>(blocks < resident ? blocks : resident);
-  CIGN_LN_DISPATCH(T, vec, shape,
-      (layer_norm_fwd_kernel<T, V, NV, BLOCK><<<grid, threads, 0, s>>>(
-          p, x, ldx, w, b, param_type, eps, y, mean, rstd)));
+  CIGN_LN_DISPATCH(T, vec, shape, {
+    constexpr auto kernel = layer_norm_fwd_kernel<T, V, NV, BLOCK>;
+    const int64_t resident = resident_blocks<kernel>(threads, 0);
+    kernel<<<static_cast<unsigned>(blocks < resident ? blocks : resident), threads, 0, s>>>(
+        p, x, ldx, w, b, param_type, eps, y, mean, rstd);
+  });
   CIGN_CHECK_LAUNCH("layer_norm_fwd_kernel");
   return CIGN_OK;
 }
@@ -511,15 +555,16 @@ int ln_bwd(int64_t n, int64_t d, const T* gy, int64_t ldg, const T* x, int64_t l
     const int threads = shape.block ? shape.lanes : kLnGroupThreads;
     const int64_t blocks =
         shape.block ? n : (n + threads / shape.lanes - 1) / (threads / shape.lanes);
-    int64_t resident = static_cast<int64_t>(sm_count()) *
-                       (shape.block ? (1024 / threads > 1 ? 1024 / threads : 1) : 3);
-    if (resident > kLnMaxBlocks) resident = kLnMaxBlocks;
-    sums = static_cast<int>(blocks < resident ? blocks : resident);
     CIGN_LN_DISPATCH(T, vec, shape, {
-      const size_t smem =
-          BLOCK != 0 ? 0 : static_cast<size_t>(kLnGroupThreads / 32) * p.G * NV * V * sizeof(float);
-      layer_norm_bwd_kernel<T, V, NV, BLOCK><<<sums, threads, smem, s>>>(
-          p, gy, ldg, x, ldx, w, param_type, mean, rstd, gx, params ? partial : nullptr);
+      constexpr auto kernel = layer_norm_bwd_kernel<T, V, NV, BLOCK>;
+      const size_t smem = BLOCK != 0 ? 0 : static_cast<size_t>(kLnGroupThreads / 32) * p.G * NV *
+                                               V * sizeof(float);
+      int64_t grid = resident_blocks<kernel>(threads, smem);
+      if (grid > kLnMaxBlocks) grid = kLnMaxBlocks;
+      if (grid > blocks) grid = blocks;
+      sums = static_cast<int>(grid);
+      kernel<<<sums, threads, smem, s>>>(p, gy, ldg, x, ldx, w, param_type, mean, rstd, gx,
+                                         params ? partial : nullptr);
     });
     CIGN_CHECK_LAUNCH("layer_norm_bwd_kernel");
   }
