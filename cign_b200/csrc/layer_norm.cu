@@ -46,8 +46,10 @@ __device__ __forceinline__ float row_sum(float v, int G, float* part, int& slot)
     if ((threadIdx.x & 31) == 0) p[threadIdx.x >> 5] = v;
     __syncthreads();
     float s = 0.0f;
-    const int warps = blockDim.x >> 5;
-    for (int w = 0; w < warps; ++w) s += p[w];
+    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); w += 4) {  // the rest of p is 0
+      const float4 q = *reinterpret_cast<const float4*>(p + w);
+      s += (q.x + q.y) + (q.z + q.w);
+    }
     return s;
   }
 }
@@ -68,10 +70,10 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, int G, float2* part
     if ((threadIdx.x & 31) == 0) p[threadIdx.x >> 5] = make_float2(a, b);
     __syncthreads();
     a = b = 0.0f;
-    const int warps = blockDim.x >> 5;
-    for (int w = 0; w < warps; ++w) {
-      a += p[w].x;
-      b += p[w].y;
+    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); w += 2) {
+      const float4 q = *reinterpret_cast<const float4*>(p + w);
+      a += q.x + q.z;
+      b += q.y + q.w;
     }
   }
 }
@@ -102,7 +104,9 @@ __global__ void __launch_bounds__(BLOCK ? BLOCK * kLnBlockThreads : kLnGroupThre
 layer_norm_fwd_kernel(LnRows p, const T* __restrict__ x, int64_t ldx, const void* __restrict__ w,
                       const void* __restrict__ b, int32_t param_type, float eps,
                       T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
-  __shared__ float part[64];
+  __shared__ __align__(16) float part[64];
+  if (BLOCK != 0 && threadIdx.x < 32) part[threadIdx.x] = part[32 + threadIdx.x] = 0.0f;
+  if (BLOCK != 0) __syncthreads();
   int slot = 0;
   const int lane = BLOCK ? threadIdx.x : threadIdx.x & (p.G - 1);
   const int lanes = BLOCK ? blockDim.x : p.G;
@@ -130,22 +134,28 @@ layer_norm_fwd_kernel(LnRows p, const T* __restrict__ x, int64_t ldx, const void
     float xv[NV][V];
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      float a = 0.0f;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        xv[i][e] = lane + lanes * i < p.nvec ? to_f(next[i].e[e]) : 0.0f;
-        s += xv[i][e];
+        xv[i][e] = to_f(next[i].e[e]);
+        a += xv[i][e];
       }
+      s += lane + lanes * i < p.nvec ? a : 0.0f;
+    }
     load_row<T, V, NV>(next, x, ldx, at + step, p, lane, lanes);
     const float mu = row_sum<BLOCK>(s, p.G, part, slot) * inv_d;
     float v = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      float a = 0.0f;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         xv[i][e] -= mu;
-        if (lane + lanes * i < p.nvec) v = fmaf(xv[i][e], xv[i][e], v);
+        a = fmaf(xv[i][e], xv[i][e], a);
       }
+      v += lane + lanes * i < p.nvec ? a : 0.0f;
+    }
     const float rs = rsqrtf(row_sum<BLOCK>(v, p.G, part, slot) * inv_d + eps);
     if (live && lane == 0 && mean != nullptr) {
       mean[row] = mu;
@@ -169,7 +179,10 @@ layer_norm_bwd_kernel(LnRows p, const T* __restrict__ gy, int64_t ldg, const T* 
                       int64_t ldx, const void* __restrict__ w, int32_t param_type,
                       const float* __restrict__ mean, const float* __restrict__ rstd,
                       T* __restrict__ gx, float* __restrict__ partial) {
-  __shared__ float2 part[64];
+  __shared__ __align__(16) float2 part[64];
+  if (BLOCK != 0 && threadIdx.x < 32)
+    part[threadIdx.x] = part[32 + threadIdx.x] = make_float2(0.0f, 0.0f);
+  if (BLOCK != 0) __syncthreads();
   extern __shared__ float columns[];  // BLOCK == 0: [warps, G * NV * V]
   int slot = 0;
   const int lane = BLOCK ? threadIdx.x : threadIdx.x & (p.G - 1);
@@ -192,50 +205,48 @@ layer_norm_bwd_kernel(LnRows p, const T* __restrict__ gy, int64_t ldg, const T* 
   Pack<T, V> xn[NV], gn[NV];
   load_row<T, V, NV>(xn, x, ldx, first, p, lane, lanes);
   load_row<T, V, NV>(gn, gy, ldg, first, p, lane, lanes);
+  float mu_next = mean[first < p.n ? first : p.n - 1];
+  float rs_next = rstd[first < p.n ? first : p.n - 1];
   for (int64_t at = first; at - off < p.n; at += step) {
     const bool live = at < p.n;
     const int64_t row = live ? at : p.n - 1;
-    Pack<T, V> xq[NV], gq[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const bool in = live && lane + lanes * i < p.nvec;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        xq[i].e[e] = in ? xn[i].e[e] : from_f<T>(0.0f);
-        gq[i].e[e] = in ? gn[i].e[e] : from_f<T>(0.0f);
-      }
-    }
-    load_row<T, V, NV>(xn, x, ldx, at + step, p, lane, lanes);
-    load_row<T, V, NV>(gn, gy, ldg, at + step, p, lane, lanes);
-    const float mu = mean[row], rs = rstd[row];
+    const float mu = mu_next, rs = rs_next;
+    // with e = x - mean and h = g rstd: u = g w, u xh = rstd u e, g xh = h e and
+    // grad_x = h w - rstd <u> - e rstd^3 <u e>.  Columns behind the last have
+    // w = 0 and their sums are dropped.
+    float ev[NV][V], hv[NV][V];
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float g = to_f(gq[i].e[e]);
-        const float xh = (to_f(xq[i].e[e]) - mu) * rs;
+        const float g = to_f(gn[i].e[e]);
+        ev[i][e] = to_f(xn[i].e[e]) - mu;
+        hv[i][e] = g * rs;
         const float u = g * wv[i][e];
         s1 += u;
-        s2 = fmaf(u, xh, s2);
-        if (live) {
-          aw[i][e] = fmaf(g, xh, aw[i][e]);
+        s2 = fmaf(u, ev[i][e], s2);
+        if (BLOCK != 0 || live) {
+          aw[i][e] = fmaf(hv[i][e], ev[i][e], aw[i][e]);
           ab[i][e] += g;
         }
       }
+    const int64_t then = at + step < p.n ? at + step : p.n - 1;
+    load_row<T, V, NV>(xn, x, ldx, then, p, lane, lanes);
+    load_row<T, V, NV>(gn, gy, ldg, then, p, lane, lanes);
+    mu_next = mean[then];
+    rs_next = rstd[then];
     if (gx != nullptr) {
       row_sum2<BLOCK>(s1, s2, p.G, part, slot);
-      s1 *= inv_d;
-      s2 *= inv_d;
+      s1 *= -rs * inv_d;
+      s2 *= -rs * rs * rs * inv_d;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = lane + lanes * i;
         Pack<T, V> q;
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float xh = (to_f(xq[i].e[e]) - mu) * rs;
-          q.e[e] = from_f<T>(rs * (to_f(gq[i].e[e]) * wv[i][e] - s1 - xh * s2));
-        }
+        for (int e = 0; e < V; ++e)
+          q.e[e] = from_f<T>(fmaf(ev[i][e], s2, fmaf(hv[i][e], wv[i][e], s1)));
         if (live && c < p.nvec) store_pack<T, V>(gx + row * p.d + static_cast<int64_t>(c) * V, q);
       }
     }
