@@ -30,15 +30,30 @@ constexpr int kLnMaxBlocks = 1776;    // partial sums of the parameter gradients
 constexpr int kLnWideThreads = 256;
 constexpr int kLnWideWarps = kLnWideThreads / 32;
 
-// Sum over the lanes of a row: a group of G lanes (a power of two up to 32),
-// or with BLOCK the whole block through shared memory.  `slot` alternates
-// between two sets of partial sums, so that one barrier per sum is enough:
-// a set is written again only after the barrier of the next sum.
-template <int BLOCK>
-__device__ __forceinline__ float row_sum(float v, int G, float* part, int& slot) {
+// How a row lies in a block.  LANES lanes hold it, load i of lane l covering
+// columns (l + LANES i) V ...; LANES == 0: the block's threads, known at launch.
+// BLOCK != 0: the block holds one row (of at most BLOCK * kLnBlockThreads
+// threads); else a group of LANES <= 32 lanes does, and the block
+// kLnGroupThreads / LANES rows.  With LANES known, the addresses of a lane's
+// loads differ by constants, which halves the instructions of the kernels that
+// load single elements.
+template <int LANES, int BLOCK>
+struct LnLanes {
+  __device__ __forceinline__ static int count() { return LANES ? LANES : blockDim.x; }
+  __device__ __forceinline__ static int lane() {
+    return BLOCK ? threadIdx.x : threadIdx.x & (LANES - 1);
+  }
+  __device__ __forceinline__ static int group() { return BLOCK ? 0 : threadIdx.x / (LANES | !LANES); }
+  static constexpr int kRows = BLOCK ? 1 : kLnGroupThreads / (LANES | !LANES);
+};
+
+// Sums over the lanes of a row.  `slot` alternates between two sets of partial
+// sums in shared memory, so that one barrier per sum is enough: a set is
+// written again only after the barrier of the next sum.
+template <int LANES, int BLOCK>
+__device__ __forceinline__ float row_sum(float v, float* part, int& slot) {
   if constexpr (BLOCK == 0) {
-    for (int o = G >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
-    return v;
+    return group_sum<LANES>(v);
   } else {
     v = warp_sum(v);
     float* p = part + slot * 32;
@@ -46,22 +61,20 @@ __device__ __forceinline__ float row_sum(float v, int G, float* part, int& slot)
     if ((threadIdx.x & 31) == 0) p[threadIdx.x >> 5] = v;
     __syncthreads();
     float s = 0.0f;
-    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); w += 4) {  // the rest of p is 0
+#pragma unroll (LANES ? 8 : 1)
+    for (int w = 0; w < LnLanes<LANES, BLOCK>::count() / 32; w += 4) {  // the rest of p is 0
       const float4 q = *reinterpret_cast<const float4*>(p + w);
       s += (q.x + q.y) + (q.z + q.w);
     }
     return s;
   }
 }
-
 // Two sums at once, one barrier.
-template <int BLOCK>
-__device__ __forceinline__ void row_sum2(float& a, float& b, int G, float2* part, int& slot) {
+template <int LANES, int BLOCK>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float2* part, int& slot) {
   if constexpr (BLOCK == 0) {
-    for (int o = G >> 1; o > 0; o >>= 1) {
-      a += __shfl_xor_sync(kFullMask, a, o);
-      b += __shfl_xor_sync(kFullMask, b, o);
-    }
+    a = group_sum<LANES>(a);
+    b = group_sum<LANES>(b);
   } else {
     a = warp_sum(a);
     b = warp_sum(b);
@@ -70,7 +83,8 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, int G, float2* part
     if ((threadIdx.x & 31) == 0) p[threadIdx.x >> 5] = make_float2(a, b);
     __syncthreads();
     a = b = 0.0f;
-    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); w += 2) {
+#pragma unroll (LANES ? 16 : 1)
+    for (int w = 0; w < LnLanes<LANES, BLOCK>::count() / 32; w += 2) {
       const float4 q = *reinterpret_cast<const float4*>(p + w);
       a += q.x + q.z;
       b += q.y + q.w;
@@ -78,59 +92,55 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, int G, float2* part
   }
 }
 
-struct LnRows {
-  int64_t n, d;
-  int nvec;  // d / V
-  int G;     // lanes of a row (rows share a block); the block holds one row with BLOCK
-};
-
-// This thread's columns of row `at`, or of the last row; columns behind the
-// last are loaded from it (the caller drops them).  No load depends on a
+// This lane's loads of the row at r (the lane's first).  `loads`: how many of
+// them lie in the row; all but the last SLACK do.  No load depends on a
 // branch, so all are in flight together, and the callers ask for a row while
 // they work on the one before.
-template <typename T, int V, int NV>
-__device__ __forceinline__ void load_row(Pack<T, V> (&q)[NV], const T* base, int64_t ld,
-                                         int64_t at, const LnRows& p, int lane, int lanes) {
-  const T* r = base + (at < p.n ? at : p.n - 1) * ld;
+template <typename T, int V, int NV, int SLACK>
+__device__ __forceinline__ void load_row(Pack<T, V> (&q)[NV], const T* r, int loads, int lanes) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = lane + lanes * i;
-    q[i] = load_pack<T, V>(r + static_cast<int64_t>(c < p.nvec ? c : p.nvec - 1) * V);
-  }
+  for (int i = 0; i < NV; ++i)
+    q[i] = load_pack<T, V>(r + (i < NV - SLACK ? i : (i < loads ? i : loads - 1)) * lanes * V);
 }
 
-template <typename T, int V, int NV, int BLOCK>
-__global__ void __launch_bounds__(BLOCK ? BLOCK * kLnBlockThreads : kLnGroupThreads)
-layer_norm_fwd_kernel(LnRows p, const T* __restrict__ x, int64_t ldx, const void* __restrict__ w,
-                      const void* __restrict__ b, int32_t param_type, float eps,
-                      T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
+// At most 80 registers: left alone, the compiler gives the 16-element bf16 row
+// 98 and fewer blocks are resident (131072 x 1024: 110 us, 96 us with 80; 64
+// spill, 111 us).
+template <typename T, int V, int NV, int SLACK, int LANES, int BLOCK>
+__global__ void __maxnreg__(BLOCK == 2 ? 64 : 80)
+layer_norm_fwd_kernel(int64_t n, int d, const T* __restrict__ x, int64_t ldx,
+                      const void* __restrict__ w, const void* __restrict__ b, int32_t param_type,
+                      float eps, T* __restrict__ y, float* __restrict__ mean,
+                      float* __restrict__ rstd) {
+  using L = LnLanes<LANES, BLOCK>;
   __shared__ __align__(16) float part[64];
   if (BLOCK != 0 && threadIdx.x < 32) part[threadIdx.x] = part[32 + threadIdx.x] = 0.0f;
   if (BLOCK != 0) __syncthreads();
   int slot = 0;
-  const int lane = BLOCK ? threadIdx.x : threadIdx.x & (p.G - 1);
-  const int lanes = BLOCK ? blockDim.x : p.G;
-  const int per_block = BLOCK ? 1 : kLnGroupThreads / p.G;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block +
-                        (BLOCK ? 0 : threadIdx.x / p.G);
+  const int lane = L::lane(), lanes = L::count();
+  const int nvec = d / V;
+  // a lane of a row narrower than the lanes has no load of its own; it repeats the last one
+  const int own = nvec > lane ? (nvec - lane + lanes - 1) / lanes : 0;
+  const int at_lane = own > 0 ? lane : nvec - 1, loads = own > 0 ? own : 1;
   float wv[NV][V], bv[NV][V];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int c = lane + lanes * i;
-      wv[i][e] = c < p.nvec ? load_param(w, param_type, c * V + e, 1.0f) : 0.0f;
-      bv[i][e] = c < p.nvec ? load_param(b, param_type, c * V + e, 0.0f) : 0.0f;
+      const int f = (lane + lanes * i) * V + e;
+      wv[i][e] = i < own ? load_param(w, param_type, f, 1.0f) : 0.0f;
+      bv[i][e] = i < own ? load_param(b, param_type, f, 0.0f) : 0.0f;
     }
-  const float inv_d = 1.0f / static_cast<float>(p.d);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
-  // every group of a warp takes part in the sums until the last of them is done
-  const int64_t off = BLOCK ? 0 : threadIdx.x / p.G;
+  const float inv_d = 1.0f / static_cast<float>(d);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * L::kRows;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * L::kRows + L::group();
+  const T* xp = x + (row < n ? row : n - 1) * ldx + at_lane * V;
+  T* yp = y + row * d + lane * V;
   Pack<T, V> next[NV];
-  load_row<T, V, NV>(next, x, ldx, first, p, lane, lanes);
-  for (int64_t at = first; at - off < p.n; at += step) {
-    const bool live = at < p.n;
-    const int64_t row = live ? at : p.n - 1;
+  load_row<T, V, NV, SLACK>(next, xp, loads, lanes);
+  // every group of a block goes on until the last of them is done, as all lanes take part in the sums
+  for (; row - L::group() < n; row += step, yp += step * d) {
+    const bool live = BLOCK != 0 || row < n;
     float xv[NV][V];
     float s = 0.0f;
 #pragma unroll
@@ -141,10 +151,11 @@ layer_norm_fwd_kernel(LnRows p, const T* __restrict__ x, int64_t ldx, const void
         xv[i][e] = to_f(next[i].e[e]);
         a += xv[i][e];
       }
-      s += lane + lanes * i < p.nvec ? a : 0.0f;
+      s += i < NV - SLACK || i < own ? a : 0.0f;
     }
-    load_row<T, V, NV>(next, x, ldx, at + step, p, lane, lanes);
-    const float mu = row_sum<BLOCK>(s, p.G, part, slot) * inv_d;
+    if (row + step < n) xp += step * ldx;
+    load_row<T, V, NV, SLACK>(next, xp, loads, lanes);
+    const float mu = row_sum<LANES, BLOCK>(s, part, slot) * inv_d;
     float v = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -154,66 +165,67 @@ layer_norm_fwd_kernel(LnRows p, const T* __restrict__ x, int64_t ldx, const void
         xv[i][e] -= mu;
         a = fmaf(xv[i][e], xv[i][e], a);
       }
-      v += lane + lanes * i < p.nvec ? a : 0.0f;
+      v += i < NV - SLACK || i < own ? a : 0.0f;
     }
-    const float rs = rsqrtf(row_sum<BLOCK>(v, p.G, part, slot) * inv_d + eps);
+    const float rs = rsqrtf(row_sum<LANES, BLOCK>(v, part, slot) * inv_d + eps);
     if (live && lane == 0 && mean != nullptr) {
       mean[row] = mu;
       rstd[row] = rs;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = lane + lanes * i;
       Pack<T, V> q;
 #pragma unroll
       for (int e = 0; e < V; ++e) q.e[e] = from_f<T>(fmaf(xv[i][e] * rs, wv[i][e], bv[i][e]));
-      if (live && c < p.nvec) store_pack<T, V>(y + row * p.d + static_cast<int64_t>(c) * V, q);
+      if (live && (i < NV - SLACK || i < own)) store_pack<T, V>(yp + i * lanes * V, q);
     }
   }
 }
 
 // partial: [gridDim.x, 2, d] sums of g xh and g over the block's rows, or NULL.
-template <typename T, int V, int NV, int BLOCK>
+template <typename T, int V, int NV, int SLACK, int LANES, int BLOCK>
 __global__ void __launch_bounds__(BLOCK ? BLOCK * kLnBlockThreads : kLnGroupThreads)
-layer_norm_bwd_kernel(LnRows p, const T* __restrict__ gy, int64_t ldg, const T* __restrict__ x,
-                      int64_t ldx, const void* __restrict__ w, int32_t param_type,
-                      const float* __restrict__ mean, const float* __restrict__ rstd,
-                      T* __restrict__ gx, float* __restrict__ partial) {
+layer_norm_bwd_kernel(int64_t n, int d, const T* __restrict__ gy, int64_t ldg,
+                      const T* __restrict__ x, int64_t ldx, const void* __restrict__ w,
+                      int32_t param_type, const float* __restrict__ mean,
+                      const float* __restrict__ rstd, T* __restrict__ gx,
+                      float* __restrict__ partial) {
+  using L = LnLanes<LANES, BLOCK>;
   __shared__ __align__(16) float2 part[64];
   if (BLOCK != 0 && threadIdx.x < 32)
     part[threadIdx.x] = part[32 + threadIdx.x] = make_float2(0.0f, 0.0f);
   if (BLOCK != 0) __syncthreads();
-  extern __shared__ float columns[];  // BLOCK == 0: [warps, G * NV * V]
+  extern __shared__ float columns[];  // BLOCK == 0: [rows of the block, LANES * NV * V]
   int slot = 0;
-  const int lane = BLOCK ? threadIdx.x : threadIdx.x & (p.G - 1);
-  const int lanes = BLOCK ? blockDim.x : p.G;
-  const int per_block = BLOCK ? 1 : kLnGroupThreads / p.G;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block +
-                        (BLOCK ? 0 : threadIdx.x / p.G);
+  const int lane = L::lane(), lanes = L::count();
+  const int nvec = d / V;
+  const int own = nvec > lane ? (nvec - lane + lanes - 1) / lanes : 0;
+  const int at_lane = own > 0 ? lane : nvec - 1, loads = own > 0 ? own : 1;
   float wv[NV][V], aw[NV][V], ab[NV][V];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int c = lane + lanes * i;
-      wv[i][e] = c < p.nvec ? load_param(w, param_type, c * V + e, 1.0f) : 0.0f;
+      wv[i][e] = i < own ? load_param(w, param_type, (lane + lanes * i) * V + e, 1.0f) : 0.0f;
       aw[i][e] = ab[i][e] = 0.0f;
     }
-  const float inv_d = 1.0f / static_cast<float>(p.d);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
-  const int64_t off = BLOCK ? 0 : threadIdx.x / p.G;
+  const float inv_d = 1.0f / static_cast<float>(d);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * L::kRows;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * L::kRows + L::group();
+  int64_t loaded = row < n ? row : n - 1;
+  const T* xp = x + loaded * ldx + at_lane * V;
+  const T* gp = gy + loaded * ldg + at_lane * V;
+  T* op = gx + row * d + lane * V;
   Pack<T, V> xn[NV], gn[NV];
-  load_row<T, V, NV>(xn, x, ldx, first, p, lane, lanes);
-  load_row<T, V, NV>(gn, gy, ldg, first, p, lane, lanes);
-  float mu_next = mean[first < p.n ? first : p.n - 1];
-  float rs_next = rstd[first < p.n ? first : p.n - 1];
-  for (int64_t at = first; at - off < p.n; at += step) {
-    const bool live = at < p.n;
-    const int64_t row = live ? at : p.n - 1;
+  load_row<T, V, NV, SLACK>(xn, xp, loads, lanes);
+  load_row<T, V, NV, SLACK>(gn, gp, loads, lanes);
+  float mu_next = mean[loaded], rs_next = rstd[loaded];
+  for (; row - L::group() < n; row += step, op += step * d) {
+    const bool live = BLOCK != 0 || row < n;
     const float mu = mu_next, rs = rs_next;
     // with e = x - mean and h = g rstd: u = g w, u xh = rstd u e, g xh = h e and
-    // grad_x = h w - rstd <u> - e rstd^3 <u e>.  Columns behind the last have
-    // w = 0 and their sums are dropped.
+    // grad_x = h w - rstd <u> - e rstd^3 <u e>.  Loads behind the last repeat it:
+    // they have w = 0 and their sums are dropped.
     float ev[NV][V], hv[NV][V];
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
@@ -226,65 +238,65 @@ layer_norm_bwd_kernel(LnRows p, const T* __restrict__ gy, int64_t ldg, const T* 
         const float u = g * wv[i][e];
         s1 += u;
         s2 = fmaf(u, ev[i][e], s2);
-        if (BLOCK != 0 || live) {
+        if (live) {
           aw[i][e] = fmaf(hv[i][e], ev[i][e], aw[i][e]);
           ab[i][e] += g;
         }
       }
-    const int64_t then = at + step < p.n ? at + step : p.n - 1;
-    load_row<T, V, NV>(xn, x, ldx, then, p, lane, lanes);
-    load_row<T, V, NV>(gn, gy, ldg, then, p, lane, lanes);
-    mu_next = mean[then];
-    rs_next = rstd[then];
+    if (row + step < n) {
+      xp += step * ldx;
+      gp += step * ldg;
+      loaded = row + step;
+    }
+    load_row<T, V, NV, SLACK>(xn, xp, loads, lanes);
+    load_row<T, V, NV, SLACK>(gn, gp, loads, lanes);
+    mu_next = mean[loaded];
+    rs_next = rstd[loaded];
     if (gx != nullptr) {
-      row_sum2<BLOCK>(s1, s2, p.G, part, slot);
+      row_sum2<LANES, BLOCK>(s1, s2, part, slot);
       s1 *= -rs * inv_d;
       s2 *= -rs * rs * rs * inv_d;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = lane + lanes * i;
         Pack<T, V> q;
 #pragma unroll
         for (int e = 0; e < V; ++e)
           q.e[e] = from_f<T>(fmaf(ev[i][e], s2, fmaf(hv[i][e], wv[i][e], s1)));
-        if (live && c < p.nvec) store_pack<T, V>(gx + row * p.d + static_cast<int64_t>(c) * V, q);
+        if (live && (i < NV - SLACK || i < own)) store_pack<T, V>(op + i * lanes * V, q);
       }
     }
   }
   if (partial == nullptr) return;
-  float* pw = partial + static_cast<int64_t>(blockIdx.x) * 2 * p.d;
+  float* pw = partial + static_cast<int64_t>(blockIdx.x) * 2 * d;
   if constexpr (BLOCK != 0) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = lane + lanes * i;
-      if (c < p.nvec)
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          pw[c * V + e] = aw[i][e];
-          pw[p.d + c * V + e] = ab[i][e];
+      for (int e = 0; e < V; ++e) {
+        const int f = (lane + lanes * i) * V + e;
+        if (i < own) {
+          pw[f] = aw[i][e];
+          pw[d + f] = ab[i][e];
         }
-    }
+      }
   } else {
-    // the groups of a warp by shuffles, then the warps in order
-    const int cols = p.G * NV * V;
+    // the rows' groups in order
+    constexpr int kCols = LANES * NV * V;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          float v = which == 0 ? aw[i][e] : ab[i][e];
-          for (int o = 16; o >= p.G; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
-          if ((threadIdx.x & 31) < p.G)
-            columns[(threadIdx.x >> 5) * cols + (lane + p.G * i) * V + e] = v;
-        }
+        for (int e = 0; e < V; ++e)
+          columns[L::group() * kCols + (lane + LANES * i) * V + e] =
+              which == 0 ? aw[i][e] : ab[i][e];
       __syncthreads();
-      for (int j = threadIdx.x; j < p.d; j += kLnGroupThreads) {
+      for (int j = threadIdx.x; j < d; j += kLnGroupThreads) {
         float v = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kLnGroupThreads / 32; ++k) v += columns[k * cols + j];
-        pw[which * p.d + j] = v;
+#pragma unroll 8
+        for (int k = 0; k < L::kRows; ++k) v += columns[k * kCols + j];
+        pw[which * d + j] = v;
       }
     }
   }
@@ -398,16 +410,17 @@ layer_norm_wide_param_kernel(int64_t n, int64_t d, int64_t chunk, const T* __res
   pw[d + j] = ab;
 }
 
-// How a row of nvec loads is spread: lanes of a group, or threads of a block,
-// and loads per thread.
+// How a row of nvec loads is spread: over a group of lanes (4 to 32) or the
+// threads of a block, and how many loads a thread makes, at most 16 elements.
 struct LnShape {
   bool fits = false, block = false;
   int lanes = 0, nv = 0;
 };
-LnShape ln_shape(int64_t nvec, int max_nv_group, int max_nv_block) {
+// Loads of 16 bytes.
+LnShape ln_shape(int64_t nvec, int max_nv) {
   LnShape s;
   for (int g = 4; g <= 32; g *= 2)
-    if (nvec <= static_cast<int64_t>(g) * max_nv_group) {
+    if (nvec <= static_cast<int64_t>(g) * max_nv) {
       s.fits = true;
       s.lanes = g;
       s.nv = static_cast<int>((nvec + g - 1) / g);
@@ -417,63 +430,104 @@ LnShape ln_shape(int64_t nvec, int max_nv_group, int max_nv_block) {
   // thread of the row pays once (its share of the sum and the barrier), which
   // takes about as long as one load's elements
   int64_t best = 0;
-  for (int nv = max_nv_block; nv >= 1; nv = nv > 4 ? nv - 4 : nv - 1) {
+  for (int nv = max_nv; nv >= 1; --nv) {
     const int64_t t = ((nvec + nv - 1) / nv + 31) / 32 * 32;
-    if (t > (nv == max_nv_block ? 2 : 1) * kLnBlockThreads) continue;
-    const int64_t cost = t * (nv + (max_nv_block > 4 ? 4 : 1));
+    if (t > (nv == max_nv ? 2 : 1) * kLnBlockThreads) continue;
+    const int64_t full = (nvec + t - 1) / t;  // at most nv; t is whole warps
+    const int64_t cost = t * (full + 1);
     if (!s.fits || cost < best) {
       best = cost;
       s.fits = s.block = true;
       s.lanes = static_cast<int>(t);
-      s.nv = nv;
+      s.nv = static_cast<int>(full);
     }
   }
   return s;
 }
-// Loads of 16 bytes where every row of every matrix starts on 16 bytes and
-// the width is a whole number of them; else of one element.
-template <typename T>
-LnShape ln_shape_of(int64_t d, bool wide_loads, int* vec) {
-  constexpr int V = 16 / sizeof(T);
-  *vec = wide_loads ? V : 1;
-  return wide_loads ? ln_shape(d / V, 16 / V, 16 / V) : ln_shape(d, 16, 16);
+// Loads of one element: the fewest lanes that hold the row.
+LnShape ln_shape_elements(int64_t d) {
+  LnShape s;
+  for (int g = 8; g <= 2 * kLnBlockThreads; g *= 2)
+    if (d <= static_cast<int64_t>(g) * (g < 32 ? 4 : 16)) {
+      s.fits = true;
+      s.block = g > 32;
+      s.lanes = g;
+      s.nv = static_cast<int>((d + g - 1) / g);
+      return s;
+    }
+  return s;
 }
 
-#define CIGN_LN_NV(V_, NV_, BLOCK_, ...)                                \
-  { constexpr int V = V_, NV = NV_, BLOCK = BLOCK_; __VA_ARGS__; }
-// CALL with V, NV (loads per thread, rounded up) and BLOCK (0: rows share a
-// block; 1, 2: a row per block of at most that many times kLnBlockThreads).
-#define CIGN_LN_DISPATCH(T, vec, shape, ...)                                             \
+struct LnPlan {
+  bool wide;  // loads of 16 bytes: every row of every matrix starts on 16 bytes
+  LnShape shape;
+  int threads;
+  int64_t blocks;  // that the rows need
+};
+
+template <typename T>
+LnPlan ln_plan(int64_t n, int64_t d, const void* const* ptrs, const int64_t* lds, int count) {
+  constexpr int V = 16 / sizeof(T);
+  LnPlan p;
+  p.wide = d % V == 0;
+  for (int i = 0; i < count; ++i)
+    if (ptrs[i] != nullptr && (!aligned16(ptrs[i]) || (lds[i] * sizeof(T)) % 16 != 0))
+      p.wide = false;
+  p.shape = p.wide ? ln_shape(d / V, 16 / V) : ln_shape_elements(d);
+  p.threads = p.shape.block ? p.shape.lanes : kLnGroupThreads;
+  const int rows = p.shape.block || !p.shape.fits ? 1 : p.threads / p.shape.lanes;
+  p.blocks = (n + rows - 1) / rows;
+  return p;
+}
+
+#define CIGN_LN_CASE(V_, NV_, SLACK_, LANES_, BLOCK_, ...)                               \
+  {                                                                                      \
+    constexpr int V = V_, NV = NV_, SLACK = SLACK_, LANES = LANES_, BLOCK = BLOCK_;      \
+    __VA_ARGS__;                                                                         \
+  }
+#define CIGN_LN_GROUP(LANES_, ...)                                                       \
+  {                                                                                      \
+    if (nv_ <= 1) CIGN_LN_CASE(kV, 1, 1, LANES_, 0, __VA_ARGS__)                         \
+    else if (nv_ <= 2) CIGN_LN_CASE(kV, 2, 1, LANES_, 0, __VA_ARGS__)                    \
+    else if (nv_ <= 3) CIGN_LN_CASE(kV, (kMost < 3 ? kMost : 3), 1, LANES_, 0, __VA_ARGS__) \
+    else CIGN_LN_CASE(kV, kMost, 1, LANES_, 0, __VA_ARGS__)                              \
+  }
+#define CIGN_LN_ELEMENTS(LANES_, BLOCK_, ...)                                            \
+  {                                                                                      \
+    if (nv_ <= 12) CIGN_LN_CASE(1, 12, 4, LANES_, BLOCK_, __VA_ARGS__)                   \
+    else CIGN_LN_CASE(1, 16, 4, LANES_, BLOCK_, __VA_ARGS__)                             \
+  }
+// CALL with V, NV (loads per thread, rounded up), SLACK (how many of them may
+// lie behind the row), LANES and BLOCK bound to the plan's.
+#define CIGN_LN_DISPATCH(T, plan, ...)                                                   \
   do {                                                                                   \
     constexpr int kV = 16 / sizeof(T), kMost = 16 / kV;                                  \
-    const int nv_ = (shape).nv;                                                          \
-    if ((vec) > 1 && !(shape).block) {                                                   \
-      if (nv_ <= 1) CIGN_LN_NV(kV, 1, 0, __VA_ARGS__)                                    \
-      else if (nv_ <= 2) CIGN_LN_NV(kV, 2, 0, __VA_ARGS__)                               \
-      else if (nv_ <= 3) CIGN_LN_NV(kV, (kMost < 3 ? kMost : 3), 0, __VA_ARGS__)         \
-      else CIGN_LN_NV(kV, kMost, 0, __VA_ARGS__)                                         \
-    } else if ((vec) > 1) {                                                              \
-      if (nv_ <= 1) CIGN_LN_NV(kV, 1, 1, __VA_ARGS__)                                    \
-      else if (nv_ <= 2 && (shape).lanes <= kLnBlockThreads)                             \
-        CIGN_LN_NV(kV, 2, 1, __VA_ARGS__)                                                \
-      else if (nv_ <= 3 && (shape).lanes <= kLnBlockThreads)                             \
-        CIGN_LN_NV(kV, (kMost < 3 ? kMost : 3), 1, __VA_ARGS__)                          \
-      else if ((shape).lanes <= kLnBlockThreads) CIGN_LN_NV(kV, kMost, 1, __VA_ARGS__)   \
-      else CIGN_LN_NV(kV, kMost, 2, __VA_ARGS__)                                         \
-    } else if (!(shape).block) {                                                         \
-      if (nv_ <= 2) CIGN_LN_NV(1, 2, 0, __VA_ARGS__)                                     \
-      else if (nv_ <= 4) CIGN_LN_NV(1, 4, 0, __VA_ARGS__)                                \
-      else if (nv_ <= 8) CIGN_LN_NV(1, 8, 0, __VA_ARGS__)                                \
-      else if (nv_ <= 12) CIGN_LN_NV(1, 12, 0, __VA_ARGS__)                              \
-      else CIGN_LN_NV(1, 16, 0, __VA_ARGS__)                                             \
-    } else {                                                                             \
-      if (nv_ <= 2) CIGN_LN_NV(1, 2, 1, __VA_ARGS__)                                     \
-      else if (nv_ <= 4) CIGN_LN_NV(1, 4, 1, __VA_ARGS__)                                \
-      else if (nv_ <= 8) CIGN_LN_NV(1, 8, 1, __VA_ARGS__)                                \
-      else if (nv_ <= 12) CIGN_LN_NV(1, 12, 1, __VA_ARGS__)                              \
-      else if ((shape).lanes <= kLnBlockThreads) CIGN_LN_NV(1, 16, 1, __VA_ARGS__)       \
-      else CIGN_LN_NV(1, 16, 2, __VA_ARGS__)                                             \
+    const int nv_ = (plan).shape.nv, lanes_ = (plan).shape.lanes;                        \
+    if ((plan).wide && !(plan).shape.block) {                                            \
+      if (lanes_ == 4) CIGN_LN_GROUP(4, __VA_ARGS__)                                     \
+      else if (lanes_ == 8) CIGN_LN_GROUP(8, __VA_ARGS__)                                \
+      else if (lanes_ == 16) CIGN_LN_GROUP(16, __VA_ARGS__)                              \
+      else CIGN_LN_GROUP(32, __VA_ARGS__)                                                \
+    } else if ((plan).wide) {                                                            \
+      if (lanes_ > kLnBlockThreads) CIGN_LN_CASE(kV, kMost, 1, 0, 2, __VA_ARGS__)        \
+      else if (nv_ <= 1) CIGN_LN_CASE(kV, 1, 1, 0, 1, __VA_ARGS__)                       \
+      else if (nv_ <= 2) CIGN_LN_CASE(kV, 2, 1, 0, 1, __VA_ARGS__)                       \
+      else if (nv_ <= 3) CIGN_LN_CASE(kV, (kMost < 3 ? kMost : 3), 1, 0, 1, __VA_ARGS__) \
+      else CIGN_LN_CASE(kV, kMost, 1, 0, 1, __VA_ARGS__)                                 \
+    } else if (lanes_ <= 8) CIGN_LN_CASE(1, 4, 4, 8, 0, __VA_ARGS__)                     \
+    else if (lanes_ <= 16) CIGN_LN_CASE(1, 4, 4, 16, 0, __VA_ARGS__)                     \
+    else if (lanes_ <= 32) {                                                             \
+      if (nv_ <= 4) CIGN_LN_CASE(1, 4, 4, 32, 0, __VA_ARGS__)                            \
+      else if (nv_ <= 6) CIGN_LN_CASE(1, 6, 2, 32, 0, __VA_ARGS__)                       \
+      else if (nv_ <= 8) CIGN_LN_CASE(1, 8, 2, 32, 0, __VA_ARGS__)                       \
+      else if (nv_ <= 10) CIGN_LN_CASE(1, 10, 2, 32, 0, __VA_ARGS__)                     \
+      else CIGN_LN_ELEMENTS(32, 0, __VA_ARGS__)                                          \
     }                                                                                    \
+    else if (lanes_ <= 64) CIGN_LN_ELEMENTS(64, 1, __VA_ARGS__)                          \
+    else if (lanes_ <= 128) CIGN_LN_ELEMENTS(128, 1, __VA_ARGS__)                        \
+    else if (lanes_ <= 256) CIGN_LN_ELEMENTS(256, 1, __VA_ARGS__)                        \
+    else if (lanes_ <= 512) CIGN_LN_ELEMENTS(512, 1, __VA_ARGS__)                        \
+    else CIGN_LN_CASE(1, 16, 8, 1024, 2, __VA_ARGS__)                                    \
   } while (0)
 
 // Blocks of `kernel` that the device holds at once: the grid of a persistent
@@ -490,10 +544,6 @@ int64_t resident_blocks(int threads, size_t smem) {
     k.store(per_sm, std::memory_order_relaxed);
   }
   return static_cast<int64_t>(per_sm) * sm_count();
-}
-
-bool rows_aligned16(const void* p, int64_t ld, size_t size) {
-  return p == nullptr || (aligned16(p) && (ld * size) % 16 == 0);
 }
 
 int64_t ln_wide_chunk(int64_t n) {
@@ -513,24 +563,20 @@ int ln_check(int64_t n, int64_t d, int32_t x_type, int32_t param_type, const cha
 template <typename T>
 int ln_fwd(int64_t n, int64_t d, const T* x, int64_t ldx, const void* w, const void* b,
            int32_t param_type, float eps, T* y, float* mean, float* rstd, cudaStream_t s) {
-  int vec;
-  const bool wide_loads = d % (16 / sizeof(T)) == 0 && rows_aligned16(x, ldx, sizeof(T)) &&
-                          aligned16(y);
-  const LnShape shape = ln_shape_of<T>(d, wide_loads, &vec);
-  if (!shape.fits) {
+  const void* ptrs[] = {x, y};
+  const int64_t lds[] = {ldx, d};
+  const LnPlan plan = ln_plan<T>(n, d, ptrs, lds, 2);
+  if (!plan.shape.fits) {
     layer_norm_wide_fwd_kernel<T><<<static_cast<unsigned>(n), kLnWideThreads, 0, s>>>(
         n, d, x, ldx, w, b, param_type, eps, y, mean, rstd);
     CIGN_CHECK_LAUNCH("layer_norm_wide_fwd_kernel");
     return CIGN_OK;
   }
-  const LnRows p{n, d, static_cast<int>(d / vec), shape.block ? 32 : shape.lanes};
-  const int threads = shape.block ? shape.lanes : kLnGroupThreads;
-  const int64_t blocks = shape.block ? n : (n + threads / shape.lanes - 1) / (threads / shape.lanes);
-  CIGN_LN_DISPATCH(T, vec, shape, {
-    constexpr auto kernel = layer_norm_fwd_kernel<T, V, NV, BLOCK>;
-    const int64_t resident = resident_blocks<kernel>(threads, 0);
-    kernel<<<static_cast<unsigned>(blocks < resident ? blocks : resident), threads, 0, s>>>(
-        p, x, ldx, w, b, param_type, eps, y, mean, rstd);
+  CIGN_LN_DISPATCH(T, plan, {
+    constexpr auto kernel = layer_norm_fwd_kernel<T, V, NV, SLACK, LANES, BLOCK>;
+    const int64_t resident = resident_blocks<kernel>(plan.threads, 0);
+    kernel<<<static_cast<unsigned>(plan.blocks < resident ? plan.blocks : resident), plan.threads,
+             0, s>>>(n, static_cast<int>(d), x, ldx, w, b, param_type, eps, y, mean, rstd);
   });
   CIGN_CHECK_LAUNCH("layer_norm_fwd_kernel");
   return CIGN_OK;
@@ -540,13 +586,12 @@ template <typename T>
 int ln_bwd(int64_t n, int64_t d, const T* gy, int64_t ldg, const T* x, int64_t ldx, const void* w,
            int32_t param_type, const float* mean, const float* rstd, T* gx, void* gw, void* gb,
            float* partial, cudaStream_t s) {
-  int vec;
-  const bool wide_loads = d % (16 / sizeof(T)) == 0 && rows_aligned16(x, ldx, sizeof(T)) &&
-                          rows_aligned16(gy, ldg, sizeof(T)) && aligned16(gx);
-  const LnShape shape = ln_shape_of<T>(d, wide_loads, &vec);
+  const void* ptrs[] = {x, gy, gx};
+  const int64_t lds[] = {ldx, ldg, d};
+  const LnPlan plan = ln_plan<T>(n, d, ptrs, lds, 3);
   const bool params = gw != nullptr || gb != nullptr;
   int sums = 0;
-  if (!shape.fits) {
+  if (!plan.shape.fits) {
     if (gx) {
       layer_norm_wide_bwd_kernel<T><<<static_cast<unsigned>(n), kLnWideThreads, 0, s>>>(
           n, d, gy, ldg, x, ldx, w, param_type, mean, rstd, gx);
@@ -562,20 +607,15 @@ int ln_bwd(int64_t n, int64_t d, const T* gy, int64_t ldg, const T* x, int64_t l
       CIGN_CHECK_LAUNCH("layer_norm_wide_param_kernel");
     }
   } else if (gx || params) {
-    const LnRows p{n, d, static_cast<int>(d / vec), shape.block ? 32 : shape.lanes};
-    const int threads = shape.block ? shape.lanes : kLnGroupThreads;
-    const int64_t blocks =
-        shape.block ? n : (n + threads / shape.lanes - 1) / (threads / shape.lanes);
-    CIGN_LN_DISPATCH(T, vec, shape, {
-      constexpr auto kernel = layer_norm_bwd_kernel<T, V, NV, BLOCK>;
-      const size_t smem = BLOCK != 0 ? 0 : static_cast<size_t>(kLnGroupThreads / 32) * p.G * NV *
-                                               V * sizeof(float);
-      int64_t grid = resident_blocks<kernel>(threads, smem);
-      if (grid > kLnMaxBlocks) grid = kLnMaxBlocks;
-      if (grid > blocks) grid = blocks;
-      sums = static_cast<int>(grid);
-      kernel<<<sums, threads, smem, s>>>(p, gy, ldg, x, ldx, w, param_type, mean, rstd, gx,
-                                         params ? partial : nullptr);
+    CIGN_LN_DISPATCH(T, plan, {
+      constexpr auto kernel = layer_norm_bwd_kernel<T, V, NV, SLACK, LANES, BLOCK>;
+      const size_t smem = BLOCK != 0 ? 0 : kLnGroupThreads * NV * V * sizeof(float);
+      int64_t resident = resident_blocks<kernel>(plan.threads, smem);
+      if (resident > kLnMaxBlocks) resident = kLnMaxBlocks;
+      sums = static_cast<int>(plan.blocks < resident ? plan.blocks : resident);
+      kernel<<<sums, plan.threads, smem, s>>>(n, static_cast<int>(d), gy, ldg, x, ldx, w,
+                                              param_type, mean, rstd, gx,
+                                              params ? partial : nullptr);
     });
     CIGN_CHECK_LAUNCH("layer_norm_bwd_kernel");
   }

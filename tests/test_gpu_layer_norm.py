@@ -91,6 +91,37 @@ def test_many_rows(cuda, n, d):
     run_case(cuda, n, d, torch.bfloat16, torch.bfloat16)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,d", [(1, 3), (2, 3), (17, 3), (40, 1), (33, 9), (5000, 13), (40007, 31), (9001, 301),
+                                 (3000, 1027), (1501, 2049), (2111, 4111), (700, 8175)])
+def test_odd_widths_over_many_rows(cuda, n, d, dtype):
+    """Rows that start anywhere within 16 bytes, more than the device holds at once.  Equal rows need not come
+    out bit for bit equal: where a row starts decides how its sum is grouped, and each grouping is within the
+    allowed error of the exact row."""
+    run_case(cuda, n, d, dtype, torch.float32)
+    x = torch.randn(1, d, device=cuda).to(dtype).repeat(n, 1)
+    r = reference(x[:1], None, None, torch.ones_like(x[:1]), EPS)
+    check(layer_norm(x), r["y"].expand(n, d), r["ty"].expand(n, d), f"equal rows n={n} d={d} {dtype}")
+
+
+def test_neighbours_and_ends_are_not_read_into_a_row(cuda):
+    """NaN around the matrix and in every second row leaves the other rows as they are."""
+    for dtype in DTYPES:
+        for n, d in ((9, 5), (300, 37), (40, 1033), (20, 4099)):
+            buf = torch.full((n * d + 32,), float("nan"), dtype=dtype, device=cuda)
+            x = buf[16:16 + n * d].view(n, d)
+            x.copy_(torch.randn(n, d, device=cuda))
+            clean = layer_norm(x)
+            assert torch.isfinite(clean).all()
+            x[::2] = float("nan")
+            y = layer_norm(x)
+            assert torch.equal(y[1::2], clean[1::2]) and torch.isnan(y[::2]).all()
+            xr = x.clone().requires_grad_()
+            gy = torch.randn(n, d, device=cuda).to(dtype)
+            (gx,) = torch.autograd.grad(layer_norm(xr), xr, gy)
+            assert torch.isfinite(gx[1::2]).all()
+
+
 @pytest.mark.parametrize("d", [64, 777, 2560, 20000])
 def test_far_mean(cuda, d):
     """A mean a thousand times the spread: the variance is formed from differences."""
