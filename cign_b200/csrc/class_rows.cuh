@@ -77,6 +77,25 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
   return s;
 }
 
+// e^d, d <= 0, by the hardware's 2^x; below 2^-126 zero.  For 16-bit logits the
+// argument d log2 e is rounded to float32, which leaves a relative error of
+// about |d| 2^-23: the terms of a softmax sum weigh e^d, and a gradient is
+// rounded to 16 bits.  For float32 logits what the rounding drops is put back
+// (an error of 2^-21 at every d), so that the small probabilities beside a sure
+// class keep their digits.
+template <typename T>
+__device__ __forceinline__ float exp_neg(float d) {
+  constexpr float kLog2e = 1.44269504f, kLog2eRest = 1.9259629e-8f, kLn2 = 0.693147181f;
+  const float t = d * kLog2e;
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  if constexpr (sizeof(T) == 4) {
+    const float rest = fmaf(d, kLog2eRest, fmaf(d, kLog2e, -t));
+    e = t > -126.0f ? fmaf(e, rest * kLn2, e) : e;  // not where e is 0 or d infinite
+  }
+  return e;
+}
+
 // ---------------------------------------------------------------- softmax
 // Running statistics of the values seen so far, relative to their maximum m:
 //   s = sum e^(x - m) - 1   (without the maximum's own e^0)
@@ -132,14 +151,13 @@ __device__ __forceinline__ RowStat stat_shfl_xor(const RowStat& a, int o) {
 }
 
 // ---------------------------------------------------------------- narrow rows
-// Rows of at most 8 G classes are held by a group of G lanes (a power of two,
-// G <= 32), class lane + G i in register i: the loads and stores of a group
+// Rows of at most E G classes are held by a group of G lanes (a power of two,
+// G <= 32), class lane + G i in register i < E: the loads and stores of a group
 // cover G neighbouring elements at a time, a row is read once, and the 32 / G
-// rows of a warp are neighbours.  8 loads in flight per lane are what covers
-// the memory latency at full occupancy.
-constexpr int kNarrowElems = 8;
+// rows of a warp are neighbours.  E is 6 or 8: 6 and more loads in flight per
+// lane cover the memory latency, and no more than a quarter of them is idle.
 constexpr int kNarrowThreads = 256;
-constexpr int64_t kNarrowMax = 32 * kNarrowElems;
+constexpr int64_t kNarrowMax = 32 * 8;
 
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
@@ -164,15 +182,24 @@ inline unsigned narrow_grid(int64_t n, int G) {
   return static_cast<unsigned>((n + kNarrowThreads / G - 1) / (kNarrowThreads / G));
 }
 
-// CALL with `G` bound to the lanes of a row of c <= kNarrowMax classes.
-#define CIGN_GROUP_DISPATCH(c, G, ...)                               \
-  do {                                                                \
-    if ((c) <= 8) { constexpr int G = 1; __VA_ARGS__; }               \
-    else if ((c) <= 16) { constexpr int G = 2; __VA_ARGS__; }         \
-    else if ((c) <= 32) { constexpr int G = 4; __VA_ARGS__; }         \
-    else if ((c) <= 64) { constexpr int G = 8; __VA_ARGS__; }         \
-    else if ((c) <= 128) { constexpr int G = 16; __VA_ARGS__; }       \
-    else { constexpr int G = 32; __VA_ARGS__; }                       \
+#define CIGN_GROUP_CASE(G_, E_, ...) \
+  { constexpr int G = G_, E = E_; __VA_ARGS__; }
+// CALL with `G` and `E` bound to the lanes and registers of a row of
+// c <= kNarrowMax classes.
+#define CIGN_GROUP_DISPATCH(c, ...)                            \
+  do {                                                          \
+    if ((c) <= 6) CIGN_GROUP_CASE(1, 6, __VA_ARGS__)            \
+    else if ((c) <= 8) CIGN_GROUP_CASE(1, 8, __VA_ARGS__)       \
+    else if ((c) <= 12) CIGN_GROUP_CASE(2, 6, __VA_ARGS__)      \
+    else if ((c) <= 16) CIGN_GROUP_CASE(2, 8, __VA_ARGS__)      \
+    else if ((c) <= 24) CIGN_GROUP_CASE(4, 6, __VA_ARGS__)      \
+    else if ((c) <= 32) CIGN_GROUP_CASE(4, 8, __VA_ARGS__)      \
+    else if ((c) <= 48) CIGN_GROUP_CASE(8, 6, __VA_ARGS__)      \
+    else if ((c) <= 64) CIGN_GROUP_CASE(8, 8, __VA_ARGS__)      \
+    else if ((c) <= 96) CIGN_GROUP_CASE(16, 6, __VA_ARGS__)     \
+    else if ((c) <= 128) CIGN_GROUP_CASE(16, 8, __VA_ARGS__)    \
+    else if ((c) <= 192) CIGN_GROUP_CASE(32, 6, __VA_ARGS__)    \
+    else CIGN_GROUP_CASE(32, 8, __VA_ARGS__)                    \
   } while (0)
 
 // ---------------------------------------------------------------- ordering

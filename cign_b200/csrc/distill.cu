@@ -294,15 +294,15 @@ distill_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t l
   }
 }
 
-// Rows of at most 8 G classes, a group of G lanes per row (class_rows.cuh).
+// Rows of at most E G classes, a group of G lanes per row (class_rows.cuh).
 // The kept classes of a row are bits in shared memory; lane l takes the
 // teacher's entries l, l + G, ...
 template <int G>
 struct NarrowBits {
-  static constexpr int kWords = G < 4 ? 1 : G / 4;  // 8 G bits
+  static constexpr int kWords = G < 4 ? 1 : G / 4;  // 8 G bits, E <= 8
 };
 
-template <typename T, int G>
+template <typename T, int G, int E>
 __global__ void __launch_bounds__(kNarrowThreads)
 distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_t ld, Teacher te,
                           float temperature, InvT it, int bucket, float* __restrict__ loss,
@@ -315,9 +315,9 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
   const int64_t row = live ? at : n - 1;  // the last warp's idle groups follow along
   const T* x = logits + row * ld;
   uint32_t* bits = all_bits + threadIdx.x / G * kWords;
-  float v[kNarrowElems];
+  float v[E];
 #pragma unroll
-  for (int i = 0; i < kNarrowElems; ++i)
+  for (int i = 0; i < E; ++i)
     v[i] = lane + G * i < c ? to_f(x[lane + G * i]) : -INFINITY;
   for (int i = lane; i < kWords; i += G) bits[i] = 0;
   __syncwarp();
@@ -361,12 +361,12 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
   // student: the sums over the classes that are not kept and over the kept ones
   float m = v[0];
 #pragma unroll
-  for (int i = 1; i < kNarrowElems; ++i) m = fmaxf(m, v[i]);
+  for (int i = 1; i < E; ++i) m = fmaxf(m, v[i]);
   m = group_max<G>(m);
   if (m != m) m = -INFINITY;
   float s_rest = 0.0f, c_rest = 0.0f, s_kept = 0.0f, c_kept = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kNarrowElems; ++i) {
+  for (int i = 0; i < E; ++i) {
     const int j = lane + G * i;
     const bool kept = (bits[j >> 5] >> (j & 31)) & 1u;
     const float one = j < c && v[i] == m ? 1.0f : 0.0f;
@@ -418,7 +418,7 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
                                     stats ? stats + row * kDsStats : nullptr);
 }
 
-template <typename T, int G>
+template <typename T, int G, int E>
 __global__ void __launch_bounds__(kNarrowThreads)
 distill_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_t ld, Teacher te,
                           float temperature, InvT it, int bucket,
@@ -430,16 +430,16 @@ distill_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
   if (row >= n) return;
   const T* x = logits + row * ld;
   T* out = grad + row * c;
-  float v[kNarrowElems];
+  float v[E];
 #pragma unroll
-  for (int i = 0; i < kNarrowElems; ++i)
+  for (int i = 0; i < E; ++i)
     v[i] = lane + G * i < c ? to_f(x[lane + G * i]) : -INFINITY;
   const DistillRow r = load_row(stats + row * kDsStats);
   const float g = g_loss[row * g_stride] * temperature;
   const bool zero = r.none != 0.0f || g == 0.0f || (r.m == -INFINITY && r.logs == r.logs);
   const float f = g * r.spread;
 #pragma unroll
-  for (int i = 0; i < kNarrowElems; ++i)
+  for (int i = 0; i < E; ++i)
     if (lane + G * i < c)
       out[lane + G * i] =
           from_f<T>(zero ? 0.0f : f * expf(scaled(v[i] - r.m, it) - r.logs));
@@ -507,8 +507,8 @@ int cign_distill_fwd(int64_t n, int64_t c, int32_t x_type, const void* logits, i
   const Teacher te{values, index, ld_values, ld_index, k, value_type, index_type};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c <= kNarrowMax) {
-    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c, G,
-        distill_narrow_fwd_kernel<T, G><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
+    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c,
+        distill_narrow_fwd_kernel<T, G, E><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
             n, static_cast<int>(c), static_cast<const T*>(logits), ld, te, temperature,
             inverse(temperature), tail, loss, stats)));
     CIGN_CHECK_LAUNCH("distill_narrow_fwd_kernel");
@@ -544,8 +544,8 @@ int cign_distill_bwd(int64_t n, int64_t c, int32_t x_type, const void* logits, i
   const Teacher te{values, index, ld_values, ld_index, k, value_type, index_type};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c <= kNarrowMax) {
-    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c, G,
-        distill_narrow_bwd_kernel<T, G><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
+    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c,
+        distill_narrow_bwd_kernel<T, G, E><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
             n, static_cast<int>(c), static_cast<const T*>(logits), ld, te, temperature,
             inverse(temperature), tail, stats, grad_loss, grad_loss_stride,
             static_cast<T*>(grad_logits))));

@@ -99,8 +99,8 @@ log_probs_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t
   }
 }
 
-// Rows of at most 8 G classes, a group of G lanes per row (class_rows.cuh).
-template <typename T, int G>
+// Rows of at most E G classes, a group of G lanes per row (class_rows.cuh).
+template <typename T, int G, int E>
 __global__ void __launch_bounds__(kNarrowThreads)
 log_probs_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_t ld,
                             const int64_t* __restrict__ labels, int top_k, LogProbOut out) {
@@ -109,28 +109,24 @@ log_probs_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int6
   const bool live = at < n;
   const int64_t row = live ? at : n - 1;  // the last warp's idle groups follow along
   const T* x = logits + row * ld;
-  const int64_t y = out.log_prob ? labels[row] : -1;
-  float v[kNarrowElems];
+  float v[E];
 #pragma unroll
-  for (int i = 0; i < kNarrowElems; ++i)
-    v[i] = lane + G * i < c ? to_f(x[lane + G * i]) : -INFINITY;
-  const float xy = y >= 0 && y < c ? to_f(x[y]) : 0.0f;
+  for (int i = 0; i < E; ++i) v[i] = lane + G * i < c ? to_f(x[lane + G * i]) : -INFINITY;
+  const int64_t y = out.log_prob ? labels[row] : -1;
   float m = v[0];
 #pragma unroll
-  for (int i = 1; i < kNarrowElems; ++i) m = fmaxf(m, v[i]);
+  for (int i = 1; i < E; ++i) m = fmaxf(m, v[i]);
   m = group_max<G>(m);
   if (m != m) m = -INFINITY;
   float s = 0.0f, cnt = 0.0f, t = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kNarrowElems; ++i) {
-    if (v[i] == m) {
-      cnt += 1.0f;
-    } else {
-      const float d = v[i] - m;
-      const float e = expf(d);
-      s += e;
-      t = fmaf(e, fmaxf(d, -1e30f), t);  // d = -inf: e = 0
-    }
+  for (int i = 0; i < E; ++i) {
+    const bool top = v[i] == m;  // its e^0 is counted, not added
+    const float d = v[i] - m;
+    const float e = exp_neg<T>(d);
+    cnt += top ? 1.0f : 0.0f;
+    s += top ? 0.0f : e;
+    t = fmaf(e, fmaxf(d, -1e30f), t);  // d = -inf: e = 0; d = NaN (m = -inf): dropped below
   }
   RowStat a;
   a.m = m;
@@ -143,7 +139,7 @@ log_probs_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int6
     if (out.log_prob) {
       float lp = 0.0f;
       if (y >= c) lp = __int_as_float(0x7fffffff);
-      else if (y >= 0) lp = log_prob_of(xy, m, logs);
+      else if (y >= 0) lp = log_prob_of(to_f(x[y]), m, logs);
       out.log_prob[row] = lp;
     }
   }
@@ -151,7 +147,7 @@ log_probs_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int6
   for (int k = 0; k < top_k; ++k) {
     uint64_t key = 0;
 #pragma unroll
-    for (int i = 0; i < kNarrowElems; ++i) {
+    for (int i = 0; i < E; ++i) {
       const int j = lane + G * i;
       const uint64_t q = class_key(v[i], static_cast<uint32_t>(j));
       if (j < c && q < last && q > key) key = q;
@@ -224,7 +220,46 @@ log_probs_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t
   }
 }
 
-template <typename T, int G>
+// What reaches a row: the sum G of the gradients of its log probabilities, the
+// entropy's, and whether there is any at all.
+struct RowGrads {
+  int64_t y;
+  float gl, gh, all, H;
+  bool any;
+};
+__device__ __forceinline__ RowGrads row_grads(const LogProbGrads& g, const int64_t* labels,
+                                              const float* entropy, int top_k, int64_t row,
+                                              int64_t c) {
+  RowGrads r;
+  // no load waits for another
+  const float gl = g.log_prob ? g.log_prob[row * g.log_prob_stride] : 0.0f;
+  r.y = g.log_prob ? labels[row] : -1;
+  r.gl = r.y >= 0 ? (r.y < c ? gl : __int_as_float(0x7fffffff)) : 0.0f;
+  r.gh = g.entropy ? g.entropy[row * g.entropy_stride] : 0.0f;
+  r.H = g.entropy ? entropy[row] : 0.0f;
+  r.all = r.gl;
+  r.any = !(r.gl == 0.0f) || !(r.gh == 0.0f);
+  if (g.top)
+    for (int i = 0; i < top_k; ++i) {
+      const float v = g.top[row * top_k + i];
+      r.all += v;
+      r.any |= !(v == 0.0f);
+    }
+  return r;
+}
+// The gradient of a class that is the label or one of the best: a - p G - spread.
+__device__ __forceinline__ float special_grad(const LogProbGrads& g, const RowGrads& r,
+                                              const int64_t* top_index, int top_k, int64_t row,
+                                              int64_t j, float lp) {
+  float a = j == r.y ? r.gl : 0.0f;
+  if (g.top)
+    for (int i = 0; i < top_k; ++i)
+      if (top_index[row * top_k + i] == j) a += g.top[row * top_k + i];
+  const float spread = r.gh * expf(lp) * (fmaxf(lp, -1e30f) + r.H);
+  return (a - r.all) - r.all * expm1f(lp) - spread;
+}
+
+template <typename T, int G, int E>
 __global__ void __launch_bounds__(kNarrowThreads)
 log_probs_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_t ld,
                             const int64_t* __restrict__ labels, const float* __restrict__ stats,
@@ -236,51 +271,40 @@ log_probs_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int6
   if (row >= n) return;
   const T* x = logits + row * ld;
   T* out = grad + row * c;
-  const float nan = __int_as_float(0x7fffffff);
-  const int64_t y = (g.log_prob && labels) ? labels[row] : -1;
-  const float gl = y >= 0 ? (y < c ? g.log_prob[row * g.log_prob_stride] : nan) : 0.0f;
-  const float gh = g.entropy ? g.entropy[row * g.entropy_stride] : 0.0f;
-  float G_all = gl;
-  bool any = !(gl == 0.0f) || !(gh == 0.0f);
-  if (g.top)
-    for (int i = 0; i < top_k; ++i) {
-      const float v = g.top[row * top_k + i];
-      G_all += v;
-      any |= !(v == 0.0f);
-    }
-  const float2 st = *reinterpret_cast<const float2*>(stats + 2 * row);
-  // no gradient reaches the row, or it has no distribution
-  if (!any || (st.x == -INFINITY && st.y == st.y)) {
+  // the logits are asked for before it is known whether any gradient reaches
+  // the row: waiting for that costs more than the reads it would save
+  float v[E];
 #pragma unroll
-    for (int i = 0; i < kNarrowElems; ++i)
+  for (int i = 0; i < E; ++i) v[i] = lane + G * i < c ? to_f(x[lane + G * i]) : 0.0f;
+  const float2 st = *reinterpret_cast<const float2*>(stats + 2 * row);
+  const RowGrads r = row_grads(g, labels, entropy, top_k, row, c);
+  // no gradient reaches the row, or it has no distribution
+  if (!r.any || (st.x == -INFINITY && st.y == st.y)) {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
       if (lane + G * i < c) out[lane + G * i] = from_f<T>(0.0f);
     return;
   }
-  const float H = g.entropy ? entropy[row] : 0.0f;
-  float v[kNarrowElems];
+  // -p G - gh p (lp + H) = p (A + B lp)
+  const float A = -(r.all + r.gh * r.H), B = -r.gh;
 #pragma unroll
-  for (int i = 0; i < kNarrowElems; ++i)
-    if (lane + G * i < c) v[i] = to_f(x[lane + G * i]);
-#pragma unroll
-  for (int i = 0; i < kNarrowElems; ++i) {
-    const int j = lane + G * i;
-    if (j < c) {
-      const float lp = (v[i] - st.x) - st.y;
-      const float p = expf(lp);
-      const float spread = gh * p * (fmaxf(lp, -1e30f) + H);  // lp = -inf: p = 0
-      float a = 0.0f;
-      bool special = j == y;
-      if (special) a = gl;
-      if (g.top)
-        for (int q = 0; q < top_k; ++q)
-          if (top_index[row * top_k + q] == j) {
-            a += g.top[row * top_k + q];
-            special = true;
-          }
-      const float r = special ? (a - G_all) - G_all * expm1f(lp) : -p * G_all;
-      out[j] = from_f<T>(r - spread);
-    }
+  for (int i = 0; i < E; ++i) {
+    const float lp = (v[i] - st.x) - st.y;
+    const float p = exp_neg<T>(lp);
+    if (lane + G * i < c)
+      out[lane + G * i] = from_f<T>(p * fmaf(B, fmaxf(lp, -1e30f), A));  // lp = -inf: p = 0
   }
+  // the label and the best classes, by the lanes that wrote them above
+  if (r.y >= 0 && r.y < c && (r.y & (G - 1)) == lane)
+    out[r.y] = from_f<T>(special_grad(g, r, top_index, top_k, row, r.y,
+                                      (to_f(x[r.y]) - st.x) - st.y));
+  if (g.top)
+    for (int i = 0; i < top_k; ++i) {
+      const int64_t j = top_index[row * top_k + i];
+      if ((j & (G - 1)) == lane)
+        out[j] = from_f<T>(special_grad(g, r, top_index, top_k, row, j,
+                                        (to_f(x[j]) - st.x) - st.y));
+    }
 }
 
 int lp_check(int64_t n, int64_t c, int32_t x_type, int64_t ld, int32_t top_k, const char* name) {
@@ -316,8 +340,8 @@ int cign_node_log_probs_fwd(int64_t n, int64_t c, int32_t x_type, const void* lo
   const LogProbOut out{log_prob, entropy, stats, top_log_probs, top_index};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c <= kNarrowMax) {
-    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c, G,
-        log_probs_narrow_fwd_kernel<T, G><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
+    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c,
+        log_probs_narrow_fwd_kernel<T, G, E><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
             n, static_cast<int>(c), static_cast<const T*>(logits), ld, labels, top_k, out)));
     CIGN_CHECK_LAUNCH("log_probs_narrow_fwd_kernel");
     return CIGN_OK;
@@ -345,8 +369,8 @@ int cign_node_log_probs_bwd(int64_t n, int64_t c, int32_t x_type, const void* lo
                        top_k > 0 ? grad_top : nullptr};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c <= kNarrowMax) {
-    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c, G,
-        log_probs_narrow_bwd_kernel<T, G><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
+    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c,
+        log_probs_narrow_bwd_kernel<T, G, E><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
             n, static_cast<int>(c), static_cast<const T*>(logits), ld, labels, stats, entropy,
             top_k, top_index, g, static_cast<T*>(grad_logits))));
     CIGN_CHECK_LAUNCH("log_probs_narrow_bwd_kernel");
