@@ -77,23 +77,79 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
   return s;
 }
 
-// e^d, d <= 0, by the hardware's 2^x; below 2^-126 zero.  For 16-bit logits the
-// argument d log2 e is rounded to float32, which leaves a relative error of
-// about |d| 2^-23: the terms of a softmax sum weigh e^d, and a gradient is
-// rounded to 16 bits.  For float32 logits what the rounding drops is put back
-// (an error of 2^-21 at every d), so that the small probabilities beside a sure
-// class keep their digits.
-template <typename T>
-__device__ __forceinline__ float exp_neg(float d) {
-  constexpr float kLog2e = 1.44269504f, kLog2eRest = 1.9259629e-8f, kLn2 = 0.693147181f;
-  const float t = d * kLog2e;
+// Two float32 values of one lane, worked on by one instruction each (sm_100's
+// f32x2 arithmetic): the row kernels are bound by the instructions they issue.
+struct F2 {
+  float x, y;
+};
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("{\n .reg .b64 p, q, r;\n mov.b64 p, {%2, %3};\n mov.b64 q, {%4, %5};\n"
+      " add.rn.f32x2 r, p, q;\n mov.b64 {%0, %1}, r;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("{\n .reg .b64 p, q, r;\n mov.b64 p, {%2, %3};\n mov.b64 q, {%4, %5};\n"
+      " mul.rn.f32x2 r, p, q;\n mov.b64 {%0, %1}, r;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("{\n .reg .b64 p, q, r, s;\n mov.b64 p, {%2, %3};\n mov.b64 q, {%4, %5};\n"
+      " mov.b64 s, {%6, %7};\n fma.rn.f32x2 r, p, q, s;\n mov.b64 {%0, %1}, r;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ F2 both(float v) { return F2{v, v}; }
+// The larger of two values, NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float exp2_hw(float t) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return e;
+}
+
+// e^(d / T) of two values d <= 0 by the hardware's 2^x, `scale` = log2(e) / T;
+// below 2^-126 zero.  d must be finite (callers raise it to kExpFloor).  For
+// 16-bit logits the argument d scale is rounded to float32, which leaves a
+// relative error of about |d| 2^-23: the terms of a softmax sum weigh e^d, and
+// a gradient is rounded to 16 bits.  For float32 logits what the rounding
+// drops is put back, so that the small probabilities beside a sure class keep
+// their digits.
+constexpr float kExpFloor = -1e4f;
+constexpr float kLog2e = 1.44269504f;
+template <typename T>
+__device__ __forceinline__ F2 exp_neg2(F2 d, float scale) {
+  const F2 t = mul2(d, both(scale));
+  F2 e{exp2_hw(t.x), exp2_hw(t.y)};
   if constexpr (sizeof(T) == 4) {
-    const float rest = fmaf(d, kLog2eRest, fmaf(d, kLog2e, -t));
-    e = t > -126.0f ? fmaf(e, rest * kLn2, e) : e;  // not where e is 0 or d infinite
+    const F2 rest = fma2(d, both(scale), F2{-t.x, -t.y});
+    e = fma2(mul2(e, both(0.693147181f)), rest, e);
   }
   return e;
+}
+
+// 1 - e^x for x <= 0, with its digits where x is near 0 (the series to x^8 is
+// exact to float32 for x > -1/2); p = e^x is given.
+__device__ __forceinline__ float one_minus_exp(float x, float p) {
+  float h = fmaf(x, 1.0f / 8.0f, 1.0f);
+  h = fmaf(h * x, 1.0f / 7.0f, 1.0f);
+  h = fmaf(h * x, 1.0f / 6.0f, 1.0f);
+  h = fmaf(h * x, 1.0f / 5.0f, 1.0f);
+  h = fmaf(h * x, 1.0f / 4.0f, 1.0f);
+  h = fmaf(h * x, 1.0f / 3.0f, 1.0f);
+  h = fmaf(h * x, 1.0f / 2.0f, 1.0f);
+  return x > -0.5f ? -h * x : 1.0f - p;
 }
 
 // ---------------------------------------------------------------- softmax
@@ -151,13 +207,15 @@ __device__ __forceinline__ RowStat stat_shfl_xor(const RowStat& a, int o) {
 }
 
 // ---------------------------------------------------------------- narrow rows
-// Rows of at most E G classes are held by a group of G lanes (a power of two,
-// G <= 32), class lane + G i in register i < E: the loads and stores of a group
-// cover G neighbouring elements at a time, a row is read once, and the 32 / G
-// rows of a warp are neighbours.  E is 6 or 8: 6 and more loads in flight per
-// lane cover the memory latency, and no more than a quarter of them is idle.
+// Rows of at most E G classes are held by a group of G lanes (a power of two),
+// class lane + G i in register i < E: a row is read once, and the 32 / G rows
+// of a warp are neighbours.  A row costs a warp E of its steps, the sums over
+// the group and one logarithm, so a kernel that reads rows is cheapest with few
+// lanes and many classes per lane (2.45M x 47 float32: 132 us with 4 lanes, 177
+// with 8, 159 with 2, whose loads are too scattered); one that writes rows has
+// no sums and wants whole sectors (205 us with 8 lanes, 244 with 4, 291 with 16).
 constexpr int kNarrowThreads = 256;
-constexpr int64_t kNarrowMax = 32 * 8;
+constexpr int64_t kNarrowMax = 256;
 
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
@@ -185,14 +243,24 @@ inline unsigned narrow_grid(int64_t n, int G) {
 #define CIGN_GROUP_CASE(G_, E_, ...) \
   { constexpr int G = G_, E = E_; __VA_ARGS__; }
 // CALL with `G` and `E` bound to the lanes and registers of a row of
-// c <= kNarrowMax classes.
+// c <= kNarrowMax classes, in a kernel that reads rows and in one that writes
+// them.
 #define CIGN_GROUP_DISPATCH(c, ...)                            \
   do {                                                          \
-    if ((c) <= 6) CIGN_GROUP_CASE(1, 6, __VA_ARGS__)            \
-    else if ((c) <= 8) CIGN_GROUP_CASE(1, 8, __VA_ARGS__)       \
-    else if ((c) <= 12) CIGN_GROUP_CASE(2, 6, __VA_ARGS__)      \
+    if ((c) <= 8) CIGN_GROUP_CASE(1, 8, __VA_ARGS__)            \
+    else if ((c) <= 16) CIGN_GROUP_CASE(1, 16, __VA_ARGS__)     \
+    else if ((c) <= 32) CIGN_GROUP_CASE(2, 16, __VA_ARGS__)     \
+    else if ((c) <= 48) CIGN_GROUP_CASE(4, 12, __VA_ARGS__)     \
+    else if ((c) <= 64) CIGN_GROUP_CASE(4, 16, __VA_ARGS__)     \
+    else if ((c) <= 96) CIGN_GROUP_CASE(8, 12, __VA_ARGS__)     \
+    else if ((c) <= 128) CIGN_GROUP_CASE(8, 16, __VA_ARGS__)    \
+    else if ((c) <= 192) CIGN_GROUP_CASE(16, 12, __VA_ARGS__)   \
+    else CIGN_GROUP_CASE(16, 16, __VA_ARGS__)                   \
+  } while (0)
+#define CIGN_GROUP_DISPATCH_WRITE(c, ...)                      \
+  do {                                                          \
+    if ((c) <= 8) CIGN_GROUP_CASE(1, 8, __VA_ARGS__)            \
     else if ((c) <= 16) CIGN_GROUP_CASE(2, 8, __VA_ARGS__)      \
-    else if ((c) <= 24) CIGN_GROUP_CASE(4, 6, __VA_ARGS__)      \
     else if ((c) <= 32) CIGN_GROUP_CASE(4, 8, __VA_ARGS__)      \
     else if ((c) <= 48) CIGN_GROUP_CASE(8, 6, __VA_ARGS__)      \
     else if ((c) <= 64) CIGN_GROUP_CASE(8, 8, __VA_ARGS__)      \
@@ -206,17 +274,18 @@ inline unsigned narrow_grid(int64_t n, int G) {
 // Classes are ordered by value, larger first (NaN before everything, as
 // torch.sort orders it), and by index, smaller first: larger keys come first.
 // -0 and +0 are equal.  0 is below every key.
+__device__ __forceinline__ uint32_t value_key(float v) {
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  if (v != v) return 0xffffffffu;
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
 __device__ __forceinline__ uint64_t class_key(float v, uint32_t index) {
-  uint32_t u = __float_as_uint(v + 0.0f);
-  u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  if (v != v) u = 0xffffffffu;
-  return (static_cast<uint64_t>(u) << 32) | static_cast<uint32_t>(~index);
+  return (static_cast<uint64_t>(value_key(v)) << 32) | static_cast<uint32_t>(~index);
 }
 __device__ __forceinline__ uint32_t key_index(uint64_t key) {
   return ~static_cast<uint32_t>(key);
 }
-__device__ __forceinline__ float key_value(uint64_t key) {
-  const uint32_t u = static_cast<uint32_t>(key >> 32);
+__device__ __forceinline__ float key_value(uint32_t u) {
   if (u == 0xffffffffu) return __int_as_float(0x7fffffff);
   return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }

@@ -297,17 +297,12 @@ distill_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t l
 // Rows of at most E G classes, a group of G lanes per row (class_rows.cuh).
 // The kept classes of a row are bits in shared memory; lane l takes the
 // teacher's entries l, l + G, ...
-template <int G>
-struct NarrowBits {
-  static constexpr int kWords = G < 4 ? 1 : G / 4;  // 8 G bits, E <= 8
-};
-
 template <typename T, int G, int E>
 __global__ void __launch_bounds__(kNarrowThreads)
 distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_t ld, Teacher te,
                           float temperature, InvT it, int bucket, float* __restrict__ loss,
                           float* __restrict__ stats) {
-  constexpr int kWords = NarrowBits<G>::kWords;
+  constexpr int kWords = (G * E + 31) / 32;
   __shared__ uint32_t all_bits[kNarrowThreads / G * kWords];
   const int lane = threadIdx.x & (G - 1);
   const int64_t at = static_cast<int64_t>(blockIdx.x) * (kNarrowThreads / G) + threadIdx.x / G;
@@ -544,7 +539,7 @@ int cign_distill_bwd(int64_t n, int64_t c, int32_t x_type, const void* logits, i
   const Teacher te{values, index, ld_values, ld_index, k, value_type, index_type};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c <= kNarrowMax) {
-    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c,
+    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH_WRITE(c,
         distill_narrow_bwd_kernel<T, G, E><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
             n, static_cast<int>(c), static_cast<const T*>(logits), ld, te, temperature,
             inverse(temperature), tail, stats, grad_loss, grad_loss_stride,

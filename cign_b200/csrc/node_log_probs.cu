@@ -94,7 +94,7 @@ log_probs_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t
     last = key;
     if (threadIdx.x == 0) {
       out.top_index[row * top_k + i] = key_index(key);
-      out.top_log_probs[row * top_k + i] = log_prob_of(key_value(key), a.m, logs);
+      out.top_log_probs[row * top_k + i] = log_prob_of(key_value(static_cast<uint32_t>(key >> 32)), a.m, logs);
     }
   }
 }
@@ -109,29 +109,33 @@ log_probs_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int6
   const bool live = at < n;
   const int64_t row = live ? at : n - 1;  // the last warp's idle groups follow along
   const T* x = logits + row * ld;
-  float v[E];
+  const int own = c - lane;  // this lane has every G-th of so many classes
+  F2 v[E / 2];
 #pragma unroll
-  for (int i = 0; i < E; ++i) v[i] = lane + G * i < c ? to_f(x[lane + G * i]) : -INFINITY;
+  for (int i = 0; i < E / 2; ++i) {
+    v[i].x = 2 * i * G < own ? to_f(x[lane + 2 * i * G]) : -INFINITY;
+    v[i].y = (2 * i + 1) * G < own ? to_f(x[lane + (2 * i + 1) * G]) : -INFINITY;
+  }
   const int64_t y = out.log_prob ? labels[row] : -1;
-  float m = v[0];
+  float m = -INFINITY;
 #pragma unroll
-  for (int i = 1; i < E; ++i) m = fmaxf(m, v[i]);
+  for (int i = 0; i < E / 2; ++i) m = fmaxf(m, fmaxf(v[i].x, v[i].y));
   m = group_max<G>(m);
-  if (m != m) m = -INFINITY;
-  float s = 0.0f, cnt = 0.0f, t = 0.0f;
+  F2 s2{0.0f, 0.0f}, cnt2{0.0f, 0.0f}, t2{0.0f, 0.0f};
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const bool top = v[i] == m;  // its e^0 is counted, not added
-    const float d = v[i] - m;
-    const float e = exp_neg<T>(d);
-    cnt += top ? 1.0f : 0.0f;
-    s += top ? 0.0f : e;
-    t = fmaf(e, fmaxf(d, -1e30f), t);  // d = -inf: e = 0; d = NaN (m = -inf): dropped below
+  for (int i = 0; i < E / 2; ++i) {
+    F2 d = add2(v[i], both(-m));  // NaN where all are -inf; t is not used there
+    d = F2{max_nan(d.x, kExpFloor), max_nan(d.y, kExpFloor)};
+    const F2 e = exp_neg2<T>(d, kLog2e);
+    // the maximum's e^0 is counted, not added
+    cnt2 = add2(cnt2, F2{v[i].x == m ? 1.0f : 0.0f, v[i].y == m ? 1.0f : 0.0f});
+    s2 = add2(s2, F2{v[i].x == m ? 0.0f : e.x, v[i].y == m ? 0.0f : e.y});
+    t2 = fma2(e, d, t2);
   }
   RowStat a;
   a.m = m;
-  a.s = group_sum<G>(s) + (group_sum<G>(cnt) - 1.0f);
-  a.t = group_sum<G>(t);
+  a.s = group_sum<G>(s2.x + s2.y) + (group_sum<G>(cnt2.x + cnt2.y) - 1.0f);
+  a.t = group_sum<G>(t2.x + t2.y);
   const float logs = stat_log(a);
   if (live && lane == 0) {
     if (out.stats) *reinterpret_cast<float2*>(out.stats + 2 * row) = make_float2(m, logs);
@@ -143,24 +147,32 @@ log_probs_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int6
       out.log_prob[row] = lp;
     }
   }
-  uint64_t last = ~0ull;
+  if (top_k == 0) return;
+  // the best class of what is left, top_k times; 0 = not there or taken
+  uint32_t key[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    key[i] = i * G < own ? value_key(i % 2 == 0 ? v[i / 2].x : v[i / 2].y) : 0u;
   for (int k = 0; k < top_k; ++k) {
-    uint64_t key = 0;
+    uint32_t best = 0, at_i = 0;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int j = lane + G * i;
-      const uint64_t q = class_key(v[i], static_cast<uint32_t>(j));
-      if (j < c && q < last && q > key) key = q;
-    }
+    for (int i = E - 1; i >= 0; --i)
+      if (key[i] >= best) {
+        best = key[i];
+        at_i = i;
+      }
+    uint32_t most = best;
 #pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) {
-      const uint64_t q = __shfl_xor_sync(kFullMask, key, o);
-      if (q > key) key = q;
-    }
-    last = key;
+    for (int o = G / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(kFullMask, most, o));
+    uint32_t j = best == most ? lane + G * at_i : 0xffffffffu;
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) j = min(j, __shfl_xor_sync(kFullMask, j, o));
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (j == static_cast<uint32_t>(lane + G * i)) key[i] = 0;
     if (live && lane == k % G) {
-      out.top_index[row * top_k + k] = key_index(key);
-      out.top_log_probs[row * top_k + k] = log_prob_of(key_value(key), m, logs);
+      out.top_index[row * top_k + k] = j;
+      out.top_log_probs[row * top_k + k] = log_prob_of(key_value(most), m, logs);
     }
   }
 }
@@ -248,6 +260,7 @@ __device__ __forceinline__ RowGrads row_grads(const LogProbGrads& g, const int64
   return r;
 }
 // The gradient of a class that is the label or one of the best: a - p G - spread.
+template <typename T>
 __device__ __forceinline__ float special_grad(const LogProbGrads& g, const RowGrads& r,
                                               const int64_t* top_index, int top_k, int64_t row,
                                               int64_t j, float lp) {
@@ -255,8 +268,9 @@ __device__ __forceinline__ float special_grad(const LogProbGrads& g, const RowGr
   if (g.top)
     for (int i = 0; i < top_k; ++i)
       if (top_index[row * top_k + i] == j) a += g.top[row * top_k + i];
-  const float spread = r.gh * expf(lp) * (fmaxf(lp, -1e30f) + r.H);
-  return (a - r.all) - r.all * expm1f(lp) - spread;
+  lp = max_nan(lp, kExpFloor);
+  const float p = exp_neg2<T>(both(lp), kLog2e).x;
+  return (a - r.all) + r.all * one_minus_exp(lp, p) - r.gh * p * (lp + r.H);
 }
 
 template <typename T, int G, int E>
@@ -271,39 +285,40 @@ log_probs_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int6
   if (row >= n) return;
   const T* x = logits + row * ld;
   T* out = grad + row * c;
+  const int own = c - lane;
   // the logits are asked for before it is known whether any gradient reaches
   // the row: waiting for that costs more than the reads it would save
-  float v[E];
+  F2 v[E / 2];
 #pragma unroll
-  for (int i = 0; i < E; ++i) v[i] = lane + G * i < c ? to_f(x[lane + G * i]) : 0.0f;
+  for (int i = 0; i < E / 2; ++i) {
+    v[i].x = 2 * i * G < own ? to_f(x[lane + 2 * i * G]) : 0.0f;
+    v[i].y = (2 * i + 1) * G < own ? to_f(x[lane + (2 * i + 1) * G]) : 0.0f;
+  }
   const float2 st = *reinterpret_cast<const float2*>(stats + 2 * row);
   const RowGrads r = row_grads(g, labels, entropy, top_k, row, c);
   // no gradient reaches the row, or it has no distribution
-  if (!r.any || (st.x == -INFINITY && st.y == st.y)) {
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-      if (lane + G * i < c) out[lane + G * i] = from_f<T>(0.0f);
-    return;
-  }
+  const bool none = !r.any || (st.x == -INFINITY && st.y == st.y);
   // -p G - gh p (lp + H) = p (A + B lp)
-  const float A = -(r.all + r.gh * r.H), B = -r.gh;
+  const F2 A = both(-(r.all + r.gh * r.H)), B = both(-r.gh);
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const float lp = (v[i] - st.x) - st.y;
-    const float p = exp_neg<T>(lp);
-    if (lane + G * i < c)
-      out[lane + G * i] = from_f<T>(p * fmaf(B, fmaxf(lp, -1e30f), A));  // lp = -inf: p = 0
+  for (int i = 0; i < E / 2; ++i) {
+    F2 lp = add2(add2(v[i], both(-st.x)), both(-st.y));
+    lp = F2{max_nan(lp.x, kExpFloor), max_nan(lp.y, kExpFloor)};
+    const F2 w = mul2(exp_neg2<T>(lp, kLog2e), fma2(B, lp, A));
+    if (2 * i * G < own) out[lane + 2 * i * G] = from_f<T>(none ? 0.0f : w.x);
+    if ((2 * i + 1) * G < own) out[lane + (2 * i + 1) * G] = from_f<T>(none ? 0.0f : w.y);
   }
+  if (none) return;
   // the label and the best classes, by the lanes that wrote them above
   if (r.y >= 0 && r.y < c && (r.y & (G - 1)) == lane)
-    out[r.y] = from_f<T>(special_grad(g, r, top_index, top_k, row, r.y,
-                                      (to_f(x[r.y]) - st.x) - st.y));
+    out[r.y] = from_f<T>(special_grad<T>(g, r, top_index, top_k, row, r.y,
+                                         (to_f(x[r.y]) - st.x) - st.y));
   if (g.top)
     for (int i = 0; i < top_k; ++i) {
       const int64_t j = top_index[row * top_k + i];
       if ((j & (G - 1)) == lane)
-        out[j] = from_f<T>(special_grad(g, r, top_index, top_k, row, j,
-                                        (to_f(x[j]) - st.x) - st.y));
+        out[j] = from_f<T>(special_grad<T>(g, r, top_index, top_k, row, j,
+                                           (to_f(x[j]) - st.x) - st.y));
     }
 }
 
@@ -369,7 +384,7 @@ int cign_node_log_probs_bwd(int64_t n, int64_t c, int32_t x_type, const void* lo
                        top_k > 0 ? grad_top : nullptr};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c <= kNarrowMax) {
-    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c,
+    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH_WRITE(c,
         log_probs_narrow_bwd_kernel<T, G, E><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
             n, static_cast<int>(c), static_cast<const T*>(logits), ld, labels, stats, entropy,
             top_k, top_index, g, static_cast<T*>(grad_logits))));

@@ -186,12 +186,17 @@ def test_sure_rows_keep_their_digits(cuda):
         x[:, 1] = torch.tensor([25.0, 14.0], device=cuda)
         labels = torch.ones(2, dtype=torch.int64, device=cuda)
         x.requires_grad_()
-        logp, p, lp, H = reference(x, labels)
+        # 1 + e^-25 keeps 16 - 11 digits of the small term in 64 bits, so the oracle takes log1p of the small sum:
+        # s = (c - 1) e^-d, log p = -log1p(s), H = log1p(s) + d s / (1 + s)
+        d = x.detach()[:, 1].double()
+        s = (c - 1) * torch.exp(-d)
+        lp, H = -torch.log1p(s), torch.log1p(s) + d * s / (1 + s)
+        p = (torch.exp(-d) / (1 + s))[:, None].expand(2, c)
         out = node_log_probs(x, labels)
         check(out.log_prob, lp, 64 * U * lp.abs(), "log_prob")
         check(out.entropy, H, 64 * U * H, "entropy")
         (grad,) = torch.autograd.grad(out.log_prob.sum(), x)
-        want = -p
+        want = -p.clone()
         want[:, 1] = -torch.expm1(lp)
         check(grad, want, 64 * U * want.abs(), "grad")
 
