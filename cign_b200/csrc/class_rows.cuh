@@ -290,4 +290,175 @@ __device__ __forceinline__ float key_value(uint32_t u) {
   return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
 
+// ---------------------------------------------------------------- wide rows
+// Rows of more than kNarrowMax classes are streamed by a team of W warps, 16
+// aligned bytes per thread and load.  A row may start anywhere: granule g of
+// V = 16 / sizeof(T) elements covers the row's elements g V - shift ..., and the
+// two granules at its ends are read by elements.
+constexpr int kWideLoads = 4;  // granules of a thread that are in flight together
+
+template <typename T>
+struct RowFrame {
+  static constexpr int V = 16 / sizeof(T);
+  const T* base;  // aligned address of granule 0, at most V - 1 elements before the row
+  int64_t shift;  // the row begins at element `shift` of the frame
+  int64_t end;    // and ends before this one
+  int64_t granules;
+  __device__ __forceinline__ RowFrame(const T* row, int64_t c) {
+    shift = static_cast<int64_t>((reinterpret_cast<uintptr_t>(row) % 16) / sizeof(T));
+    base = row - shift;
+    end = shift + c;
+    granules = (end + V - 1) / V;
+  }
+  // Granule g as it lies in memory, elements outside of the row as `outside`.
+  __device__ __forceinline__ Pack<T, V> load(int64_t g, float outside) const {
+    Pack<T, V> q;
+    if (g * V >= shift && g * V + V <= end) {
+      q = load_pack<T, V>(base + g * V);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int64_t f = g * V + e;
+        q.e[e] = f >= shift && f < end ? base[f] : from_f<T>(outside);
+      }
+    }
+    return q;
+  }
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Pack<T, V>& q, F2 (&v)[V / 2]) {
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) v[i] = F2{to_f(q.e[2 * i]), to_f(q.e[2 * i + 1])};
+}
+template <int N>
+__device__ __forceinline__ float max_of(const F2 (&v)[N]) {
+  float m = max_nan(v[0].x, v[0].y);
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = max_nan(m, max_nan(v[i].x, v[i].y));
+  return m;
+}
+
+template <int W>
+__device__ __forceinline__ void team_sync() {
+  if constexpr (W == 1) __syncwarp();
+  else __syncthreads();
+}
+
+// Running sums of a thread over the values it has seen, relative to m:
+//   s = sum over x < m of e^((x - m) / T),  cnt = how many x equal m,
+//   t = sum of e^((x - m) / T) (x - m)
+// with `scale` = log2(e) / T.  m may be any value that is not below what was
+// seen (a thread that starts with its team's maximum meets larger ones rarely,
+// and both branches below are rare).
+template <typename T, bool ENTROPY>
+struct Stream {
+  float m, cnt;
+  F2 s, t;
+  __device__ __forceinline__ explicit Stream(float start)
+      : m(start), cnt(0.0f), s{0.0f, 0.0f}, t{0.0f, 0.0f} {}
+  // `most` = max_of(v); NaN makes s NaN.
+  template <int N>
+  __device__ __forceinline__ void add(const F2 (&v)[N], float most, float scale) {
+    if (most > m) raise(most, scale);
+    if (most == m) {  // the maximum's e^0 is counted, not added
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const bool px = v[i].x == m, py = v[i].y == m;  // -inf, too
+        F2 d = add2(v[i], both(-m));
+        d = F2{px ? 0.0f : max_nan(d.x, kExpFloor), py ? 0.0f : max_nan(d.y, kExpFloor)};
+        const F2 e = exp_neg2<T>(d, scale);
+        cnt += (px ? 1.0f : 0.0f) + (py ? 1.0f : 0.0f);
+        s = add2(s, F2{px ? 0.0f : e.x, py ? 0.0f : e.y});
+        if (ENTROPY) t = fma2(e, d, t);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        F2 d = add2(v[i], both(-m));
+        d = F2{max_nan(d.x, kExpFloor), max_nan(d.y, kExpFloor)};
+        const F2 e = exp_neg2<T>(d, scale);
+        s = add2(s, e);
+        if (ENTROPY) t = fma2(e, d, t);
+      }
+    }
+  }
+  __device__ __forceinline__ void raise(float to, float scale) {
+    const float d = max_nan(m - to, kExpFloor);
+    const float f = exp_neg2<T>(both(d), scale).x;
+    const float n = (s.x + s.y + cnt) * f;
+    if (ENTROPY) t = F2{fmaf(n, d, f * (t.x + t.y)), 0.0f};
+    s = F2{n, 0.0f};
+    cnt = 0.0f;
+    m = to;
+  }
+};
+
+// The same of a whole team or row.  (m, s, cnt, t) of two disjoint sets join by
+// raising the lower one.
+struct Sums {
+  float m, s, cnt, t;
+};
+template <typename T>
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b, float scale) {
+  const bool ge = a.m >= b.m;
+  const Sums hi = ge ? a : b, lo = ge ? b : a;
+  if (a.m == b.m) return Sums{hi.m, hi.s + lo.s, hi.cnt + lo.cnt, hi.t + lo.t};
+  const float d = max_nan(lo.m - hi.m, kExpFloor);
+  const float f = exp_neg2<T>(both(d), scale).x;
+  const float n = (lo.s + lo.cnt) * f;
+  return Sums{hi.m, hi.s + n, hi.cnt, hi.t + fmaf(n, d, f * lo.t)};
+}
+template <typename T>
+__device__ __forceinline__ Sums join_warp(Sums a, float scale) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    a = join<T>(a, Sums{__shfl_xor_sync(kFullMask, a.m, o), __shfl_xor_sync(kFullMask, a.s, o),
+                        __shfl_xor_sync(kFullMask, a.cnt, o), __shfl_xor_sync(kFullMask, a.t, o)},
+                scale);
+  return a;
+}
+// As RowStat (t stays relative to the unscaled differences).
+__device__ __forceinline__ RowStat row_stat(const Sums& a) {
+  RowStat r;
+  r.m = a.m;
+  r.s = a.s + (a.cnt - 1.0f);
+  r.t = a.t;
+  return r;
+}
+
+// Launch `kernel` with clusters of `cluster` blocks (1 to 8).
+template <typename... Params, typename... Args>
+int launch_cluster(void (*kernel)(Params...), unsigned grid, int threads, size_t smem, int cluster,
+                   cudaStream_t s, const char* what, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(CIGN_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
+  }
+  count_launch();
+  return CIGN_OK;
+}
+
+// Blocks that share a row of `granules` where there are too few rows to fill
+// the device: as many as leave every thread a full set of loads, at most 8.
+inline int wide_split(int64_t n, int64_t granules, int threads) {
+  int split = 1;
+  while (split < 8 && n * split * 2 <= 2 * sm_count() &&
+         granules >= static_cast<int64_t>(2) * split * threads * kWideLoads)
+    split *= 2;
+  return split;
+}
+
 }  // namespace cign

@@ -7,6 +7,8 @@
 //   grad_j = a_j - p_j G - gh p_j (log p_j + H)
 // Where a_j is not zero, a_j - p_j G is formed as (a_j - G) - G expm1(log p_j),
 // which keeps its digits for p_j near 1.
+#include <cooperative_groups.h>
+
 #include "class_rows.cuh"
 
 namespace cign {
@@ -36,65 +38,248 @@ __device__ __forceinline__ float log_prob_of(float x, float m, float logs) {
   return m == -INFINITY ? (logs == logs ? -INFINITY : logs) : (x - m) - logs;
 }
 
-__device__ __forceinline__ RowStat block_stat(RowStat a, RowStat* part) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) a = stat_merge(a, stat_shfl_xor(a, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
-  __syncthreads();
-  a = part[0];
-#pragma unroll
-  for (int w = 1; w < kLpWarps; ++w) a = stat_merge(a, part[w]);
-  return a;
+__device__ __forceinline__ void write_row(const LogProbOut& out, int64_t row, const RowStat& a,
+                                          int64_t y, float xy, int64_t c) {
+  const float logs = stat_log(a);
+  if (out.stats) *reinterpret_cast<float2*>(out.stats + 2 * row) = make_float2(a.m, logs);
+  if (out.entropy) out.entropy[row] = stat_nothing(a) ? 0.0f : logs - a.t / (1.0f + a.s);
+  if (out.log_prob) {
+    float lp = 0.0f;
+    if (y >= c) lp = __int_as_float(0x7fffffff);
+    else if (y >= 0) lp = log_prob_of(xy, a.m, logs);
+    out.log_prob[row] = lp;
+  }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads)
-log_probs_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld,
-                     const int64_t* __restrict__ labels, int top_k, LogProbOut out) {
-  __shared__ RowStat part[kLpWarps];
-  __shared__ unsigned long long best[kLpWarps];
-  const int64_t row = blockIdx.x;
-  const T* x = logits + row * ld;
-  RowStat a;
-  for (int64_t j = threadIdx.x; j < c; j += kLpThreads) stat_add(a, to_f(x[j]));
-  a = block_stat(a, part);
-  const float logs = stat_log(a);
-  if (threadIdx.x == 0) {
-    if (out.stats) {
-      out.stats[2 * row] = a.m;
-      out.stats[2 * row + 1] = logs;
+// The best classes that one warp has met, best first: place p = 32 i + lane in
+// key[i] of the lane (class_key; 0 = none yet).
+struct BestList {
+  uint64_t key[kLpMaxTop / 32];
+  uint64_t last;  // at place top_k - 1
+  __device__ __forceinline__ BestList() : last(0) {
+#pragma unroll
+    for (int i = 0; i < kLpMaxTop / 32; ++i) key[i] = 0;
+  }
+  // All lanes with the same key, which is larger than `last`.
+  __device__ __forceinline__ void insert(uint64_t k, int top_k) {
+    const int lane = threadIdx.x & 31;
+    uint64_t carry = k;
+#pragma unroll
+    for (int i = 0; i < kLpMaxTop / 32; ++i) {
+      const int place = __popc(__ballot_sync(kFullMask, key[i] > carry));
+      const uint64_t out = __shfl_sync(kFullMask, key[i], 31);
+      const uint64_t up = __shfl_up_sync(kFullMask, key[i], 1);
+      if (lane == place) key[i] = carry;
+      else if (lane > place) key[i] = up;
+      if (place == 32) continue;  // all of these are larger
+      carry = out;
+      if (top_k <= 32 * (i + 1)) break;
     }
-    if (out.entropy) out.entropy[row] = stat_nothing(a) ? 0.0f : logs - a.t / (1.0f + a.s);
-    if (out.log_prob) {
-      const int64_t y = labels[row];
-      float lp = 0.0f;
-      if (y >= c) lp = __int_as_float(0x7fffffff);
-      else if (y >= 0) lp = log_prob_of(to_f(x[y]), a.m, logs);
-      out.log_prob[row] = lp;
+    static_assert(kLpMaxTop == 64, "two keys per lane");
+    last = __shfl_sync(kFullMask, top_k <= 32 ? key[0] : key[1], (top_k - 1) % 32);
+  }
+};
+
+// Team of W warps per row; with W = 8 a cluster of blocks may share a row.
+template <int W>
+struct alignas(16) WideShared {
+  static constexpr int kThreads = 32 * W;
+  uint32_t most[kThreads];     // value keys of the threads' maxima
+  uint32_t floor;              // value key that top_k classes at least reach
+  int count;
+  uint64_t best[W * kLpMaxTop];
+  uint64_t sorted[kLpMaxTop];
+  Sums part[W];
+  Sums sums;
+};
+
+// The top_k largest of `count` different keys, sorted, into `sorted`: a key's
+// place is the number of larger ones.
+template <int W>
+__device__ __forceinline__ void sort_best(WideShared<W>& sh, int count, int top_k, int tid) {
+  for (int i = tid; i < count; i += 32 * W) {
+    const uint64_t k = sh.best[i];
+    int place = 0;
+    for (int j = 0; j < count; ++j) place += sh.best[j] > k ? 1 : 0;
+    if (place < top_k) sh.sorted[place] = k;
+  }
+}
+
+// One pass over the row.  The first loads of all threads give the team's
+// maximum, from which the sums start, and a floor for the best classes: the
+// top_k-th largest of the threads' maxima is reached by top_k classes.  Only
+// what reaches the floor is looked at again: each warp keeps its best top_k,
+// and a full list raises the floor for all.
+template <typename T, int W>
+__global__ void __launch_bounds__(W == 1 ? 128 : 32 * W)
+log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld,
+                          const int64_t* __restrict__ labels, int top_k, int split,
+                          LogProbOut out) {
+  constexpr int V = RowFrame<T>::V;
+  constexpr int kTeams = W == 1 ? 4 : 1;
+  constexpr int kThreads = 32 * W;
+  __shared__ WideShared<W> all[kTeams];
+  const int team = W == 1 ? threadIdx.x >> 5 : 0;
+  const int tid = W == 1 ? threadIdx.x & 31 : threadIdx.x;
+  const int lane = threadIdx.x & 31;
+  WideShared<W>& sh = all[team];
+  const int rank = W == 8 ? blockIdx.x % split : 0;
+  const int64_t row = W == 8 ? blockIdx.x / split : static_cast<int64_t>(blockIdx.x) * kTeams + team;
+  if (row >= n) return;  // a whole team
+  const T* x = logits + row * ld;
+  const RowFrame<T> frame(x, c);
+  const int64_t g0 = W == 8 ? frame.granules * rank / split : 0;
+  const int64_t g1 = W == 8 ? frame.granules * (rank + 1) / split : frame.granules;
+
+  Pack<T, V> q[kWideLoads];
+  F2 v[V / 2];
+  float most = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < kWideLoads; ++u) {
+    const int64_t g = g0 + tid + u * kThreads;
+    q[u] = frame.load(g < g1 ? g : frame.granules, -INFINITY);
+  }
+#pragma unroll
+  for (int u = 0; u < kWideLoads; ++u) {
+    unpack(q[u], v);
+    most = max_nan(most, max_of(v));
+  }
+  float start = warp_max(most);  // skips NaN
+  if (start != start) start = -INFINITY;
+  if (W > 1) {
+    if (lane == 0) sh.part[tid >> 5].m = start;
+    sh.most[tid] = value_key(most);
+    if (tid == 0) sh.floor = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) start = fmaxf(start, sh.part[w].m);
+  } else {
+    sh.most[tid] = value_key(most);
+    if (tid == 0) sh.floor = 0;
+    __syncwarp();
+  }
+  if (top_k > 0 && top_k <= kThreads) {
+    const uint32_t mine = value_key(most);
+    int place = 0;
+    for (int j = 0; j < kThreads; j += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(sh.most + j);
+      place += (o.x > mine || (o.x == mine && j < tid)) + (o.y > mine || (o.y == mine && j + 1 < tid)) +
+               (o.z > mine || (o.z == mine && j + 2 < tid)) + (o.w > mine || (o.w == mine && j + 3 < tid));
+    }
+    if (place == top_k - 1) sh.floor = mine;
+  }
+  if (tid == 0) sh.count = 0;
+  team_sync<W>();
+
+  Stream<T, true> sums(start);
+  BestList best;
+  for (int64_t g = g0 + tid;; g += kWideLoads * kThreads) {
+#pragma unroll
+    for (int u = 0; u < kWideLoads; ++u) {
+      unpack(q[u], v);
+      const float top = max_of(v);
+      sums.add(v, top, kLog2e);
+      if (top_k == 0) continue;
+      const uint32_t floor = *const_cast<const volatile uint32_t*>(&sh.floor);
+      if (!__any_sync(kFullMask, value_key(top) >= floor)) continue;
+      // the lanes' classes that may belong to the best, one per lane at a time
+      const int64_t first = (g + u * kThreads) * V - frame.shift;
+      uint32_t left = 0;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float xe = e % 2 == 0 ? v[e / 2].x : v[e / 2].y;
+        if (value_key(xe) >= floor && first + e >= 0 && first + e < c) left |= 1u << e;
+      }
+      if (g + u * kThreads >= g1) left = 0;
+      while (__any_sync(kFullMask, left != 0)) {
+        const int pick = __ffs(left) - 1;
+        float xe = 0.0f;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (e == pick) xe = e % 2 == 0 ? v[e / 2].x : v[e / 2].y;
+        const uint64_t key =
+            left ? class_key(xe, static_cast<uint32_t>(first + pick)) : 0;
+        left &= left - 1;
+        unsigned who = __ballot_sync(kFullMask, key > best.last);
+        while (who) {
+          const uint64_t k = __shfl_sync(kFullMask, key, __ffs(who) - 1);
+          who &= who - 1;
+          if (k > best.last) best.insert(k, top_k);
+        }
+        const uint32_t reached = static_cast<uint32_t>(best.last >> 32);
+        if (lane == 0 && reached > floor) atomicMax(&sh.floor, reached);
+      }
+    }
+    if (g - tid + kWideLoads * kThreads >= g1) break;  // the same for the whole team
+#pragma unroll
+    for (int u = 0; u < kWideLoads; ++u) {
+      const int64_t h = g + (kWideLoads + u) * kThreads;
+      q[u] = frame.load(h < g1 ? h : frame.granules, -INFINITY);
     }
   }
-  uint64_t last = ~0ull;
-  for (int i = 0; i < top_k; ++i) {
-    uint64_t key = 0;
-    for (int64_t j = threadIdx.x; j < c; j += kLpThreads) {
-      const uint64_t q = class_key(to_f(x[j]), static_cast<uint32_t>(j));
-      if (q < last && q > key) key = q;
-    }
+
+  Sums a{sums.m, sums.s.x + sums.s.y, sums.cnt, sums.t.x + sums.t.y};
+  a = join_warp<T>(a, kLog2e);
+  if (W > 1) {
+    if (lane == 0) sh.part[tid >> 5] = a;
+    __syncthreads();
+    a = sh.part[0];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const uint64_t q = __shfl_xor_sync(kFullMask, key, o);
-      if (q > key) key = q;
+    for (int w = 1; w < W; ++w) a = join<T>(a, sh.part[w], kLog2e);
+  }
+  if (top_k > 0) {
+    const uint32_t floor = *const_cast<const volatile uint32_t*>(&sh.floor);
+#pragma unroll
+    for (int i = 0; i < kLpMaxTop / 32; ++i) {
+      const bool keep = best.key[i] != 0 && 32 * i + lane < top_k &&
+                        static_cast<uint32_t>(best.key[i] >> 32) >= floor;
+      const unsigned who = __ballot_sync(kFullMask, keep);
+      int at = 0;
+      if (lane == 0 && who) at = atomicAdd(&sh.count, __popc(who));
+      at = __shfl_sync(kFullMask, at, 0) + __popc(who & ((1u << lane) - 1u));
+      if (keep) sh.best[at] = best.key[i];
     }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) best[threadIdx.x >> 5] = key;
-    __syncthreads();
-    for (int w = 0; w < kLpWarps; ++w)
-      if (best[w] > key) key = best[w];
-    last = key;
-    if (threadIdx.x == 0) {
-      out.top_index[row * top_k + i] = key_index(key);
-      out.top_log_probs[row * top_k + i] = log_prob_of(key_value(static_cast<uint32_t>(key >> 32)), a.m, logs);
+    if (tid < kLpMaxTop) sh.sorted[tid] = 0;
+    for (int i = tid + kThreads; i < kLpMaxTop; i += kThreads) sh.sorted[i] = 0;
+    team_sync<W>();
+    sort_best<W>(sh, sh.count, top_k, tid);
+  }
+  if (W == 8 && split > 1) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    if (tid == 0) sh.sums = a;
+    cluster.sync();
+    if (rank == 0) {
+      for (int r = 1; r < split; ++r)
+        a = join<T>(a, cluster.map_shared_rank(&sh, r)->sums, kLog2e);
+      if (top_k > 0) {
+        uint64_t own = 0;
+        const int count = split * top_k;
+        for (int i = tid; i < top_k; i += kThreads) own = sh.sorted[i];
+        __syncthreads();
+        if (tid < top_k) sh.best[tid] = own;
+        for (int i = tid + top_k; i < count; i += kThreads)
+          sh.best[i] = cluster.map_shared_rank(&sh, i / top_k)->sorted[i % top_k];
+        __syncthreads();
+        sort_best<W>(sh, count, top_k, tid);
+      }
+    }
+    cluster.sync();  // the others' shared memory is read above
+    if (rank != 0) return;
+  }
+  const RowStat st = row_stat(a);
+  if (tid == 0) {
+    const int64_t y = out.log_prob ? labels[row] : -1;
+    write_row(out, row, st, y, y >= 0 && y < c ? to_f(x[y]) : 0.0f, c);
+  }
+  if (top_k > 0) {
+    team_sync<W>();
+    const float logs = stat_log(st);
+    for (int i = tid; i < top_k; i += kThreads) {
+      const uint64_t k = sh.sorted[i];
+      out.top_index[row * top_k + i] = key_index(k);
+      out.top_log_probs[row * top_k + i] =
+          log_prob_of(key_value(static_cast<uint32_t>(k >> 32)), st.m, logs);
     }
   }
 }
@@ -136,18 +321,9 @@ log_probs_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int6
   a.m = m;
   a.s = group_sum<G>(s2.x + s2.y) + (group_sum<G>(cnt2.x + cnt2.y) - 1.0f);
   a.t = group_sum<G>(t2.x + t2.y);
-  const float logs = stat_log(a);
-  if (live && lane == 0) {
-    if (out.stats) *reinterpret_cast<float2*>(out.stats + 2 * row) = make_float2(m, logs);
-    if (out.entropy) out.entropy[row] = stat_nothing(a) ? 0.0f : logs - a.t / (1.0f + a.s);
-    if (out.log_prob) {
-      float lp = 0.0f;
-      if (y >= c) lp = __int_as_float(0x7fffffff);
-      else if (y >= 0) lp = log_prob_of(to_f(x[y]), m, logs);
-      out.log_prob[row] = lp;
-    }
-  }
+  if (live && lane == 0) write_row(out, row, a, y, y >= 0 && y < c ? to_f(x[y]) : 0.0f, c);
   if (top_k == 0) return;
+  const float logs = stat_log(a);
   // the best class of what is left, top_k times; 0 = not there or taken
   uint32_t key[E];
 #pragma unroll
@@ -352,6 +528,8 @@ int cign_node_log_probs_fwd(int64_t n, int64_t c, int32_t x_type, const void* lo
   CIGN_REQUIRE(logits != nullptr && (log_prob == nullptr || labels != nullptr) &&
                    (top_k == 0 || (top_log_probs && top_index)),
                CIGN_ERR_NULL_POINTER, "node_log_probs_fwd: NULL argument");
+  CIGN_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 8 == 0, CIGN_ERR_ALIGNMENT,
+               "node_log_probs_fwd: stats must be 8-byte aligned");
   const LogProbOut out{log_prob, entropy, stats, top_log_probs, top_index};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c <= kNarrowMax) {
@@ -361,10 +539,25 @@ int cign_node_log_probs_fwd(int64_t n, int64_t c, int32_t x_type, const void* lo
     CIGN_CHECK_LAUNCH("log_probs_narrow_fwd_kernel");
     return CIGN_OK;
   }
-  CIGN_TYPE_DISPATCH(x_type, T,
-      log_probs_fwd_kernel<T><<<static_cast<unsigned>(n), kLpThreads, 0, s>>>(
-          n, c, static_cast<const T*>(logits), ld, labels, top_k, out));
-  CIGN_CHECK_LAUNCH("log_probs_fwd_kernel");
+  // warps of a row by its length: one warp does a row of a few loads per lane
+  // without barriers; eight, and eight blocks where rows are few, a long one
+  const int64_t granules = c * type_size(x_type) / 16;
+  CIGN_TYPE_DISPATCH(x_type, T, {
+    const T* x = static_cast<const T*>(logits);
+    if (granules <= 2 * 32 * kWideLoads) {
+      log_probs_wide_fwd_kernel<T, 1><<<static_cast<unsigned>((n + 3) / 4), 128, 0, s>>>(
+          n, c, x, ld, labels, top_k, 1, out);
+    } else if (granules <= 2 * 128 * kWideLoads) {
+      log_probs_wide_fwd_kernel<T, 4><<<static_cast<unsigned>(n), 128, 0, s>>>(
+          n, c, x, ld, labels, top_k, 1, out);
+    } else {
+      const int split = wide_split(n, granules, 256);
+      return launch_cluster(log_probs_wide_fwd_kernel<T, 8>, static_cast<unsigned>(n * split), 256,
+                            0, split, s, "log_probs_wide_fwd_kernel", n, c, x, ld, labels, top_k,
+                            split, out);
+    }
+  });
+  CIGN_CHECK_LAUNCH("log_probs_wide_fwd_kernel");
   return CIGN_OK;
 }
 
@@ -380,6 +573,8 @@ int cign_node_log_probs_bwd(int64_t n, int64_t c, int32_t x_type, const void* lo
   CIGN_REQUIRE(logits && stats && grad_logits && (!grad_log_prob || labels) &&
                    (!grad_entropy || entropy) && (!grad_top || top_index),
                CIGN_ERR_NULL_POINTER, "node_log_probs_bwd: NULL argument");
+  CIGN_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 8 == 0, CIGN_ERR_ALIGNMENT,
+               "node_log_probs_bwd: stats must be 8-byte aligned");
   const LogProbGrads g{grad_log_prob, grad_log_prob_stride, grad_entropy, grad_entropy_stride,
                        top_k > 0 ? grad_top : nullptr};
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -56,14 +56,15 @@ def test_layer_norm_backward_refuses(kw, code):
 @pytest.mark.parametrize("kw,code", [
     (dict(n=-1), INVALID), (dict(c=0), INVALID), (dict(xt=5), INVALID), (dict(ld=7), INVALID), (dict(k=9), INVALID),
     (dict(k=-1), INVALID), (dict(c=100, ld=100, k=65), UNSUPPORTED), (dict(c=1 << 31, ld=1 << 31), UNSUPPORTED),
-    (dict(x=None), NULL), (dict(labels=None), NULL), (dict(k=2), NULL), (dict(k=2, top=P), NULL)])
+    (dict(x=None), NULL), (dict(labels=None), NULL), (dict(k=2), NULL), (dict(k=2, top=P), NULL),
+    (dict(stats=ctypes.c_void_p(4100)), ALIGNMENT)])
 def test_log_probs_forward_refuses(kw, code):
     assert lp_fwd(**kw) == code
 
 
 @pytest.mark.parametrize("kw,code", [
     (dict(n=-1), INVALID), (dict(ld=3), INVALID), (dict(x=None), NULL), (dict(labels=None), NULL), (dict(stats=None), NULL),
-    (dict(ent=None), NULL), (dict(out=None), NULL), (dict(k=2, gt=P), NULL)])
+    (dict(ent=None), NULL), (dict(out=None), NULL), (dict(k=2, gt=P), NULL), (dict(stats=ctypes.c_void_p(4100)), ALIGNMENT)])
 def test_log_probs_backward_refuses(kw, code):
     assert lp_bwd(**kw) == code
 
