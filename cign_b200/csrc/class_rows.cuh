@@ -304,25 +304,52 @@ struct RowFrame {
   int64_t shift;  // the row begins at element `shift` of the frame
   int64_t end;    // and ends before this one
   int64_t granules;
-  __device__ __forceinline__ RowFrame(const T* row, int64_t c) {
+  int64_t g0, g1;  // the whole granules among those of this team's share
+  int64_t head, tail;  // granules of the share that are not whole, or -1
+  __device__ __forceinline__ RowFrame(const T* row, int64_t c, int rank, int split) {
     shift = static_cast<int64_t>((reinterpret_cast<uintptr_t>(row) % 16) / sizeof(T));
     base = row - shift;
     end = shift + c;
     granules = (end + V - 1) / V;
+    g0 = split > 1 ? granules * rank / split : 0;
+    g1 = split > 1 ? granules * (rank + 1) / split : granules;
+    head = g0 == 0 && shift > 0 ? g0++ : -1;
+    tail = g1 == granules && end % V != 0 ? --g1 : -1;
   }
-  // Granule g as it lies in memory, elements outside of the row as `outside`.
-  __device__ __forceinline__ Pack<T, V> load(int64_t g, float outside) const {
+  // A granule that is not whole, elements outside of the row as `outside`.
+  __device__ __forceinline__ Pack<T, V> edge(int64_t g, float outside) const {
     Pack<T, V> q;
-    if (g * V >= shift && g * V + V <= end) {
-      q = load_pack<T, V>(base + g * V);
-    } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const int64_t f = g * V + e;
-        q.e[e] = f >= shift && f < end ? base[f] : from_f<T>(outside);
-      }
+    for (int e = 0; e < V; ++e) {
+      const int64_t f = g * V + e;
+      q.e[e] = g >= 0 && f >= shift && f < end ? base[f] : from_f<T>(outside);
     }
     return q;
+  }
+  // Thread `tid` of `threads`: whole granules g0 + tid + threads (k kWideLoads + u).
+  __device__ __forceinline__ int64_t granule(int64_t k, int u, int tid, int threads) const {
+    return g0 + tid + threads * (k * kWideLoads + u);
+  }
+  __device__ __forceinline__ int64_t rounds(int threads) const {
+    return (g1 - g0 + threads * kWideLoads - 1) / (threads * kWideLoads);
+  }
+  __device__ __forceinline__ void load(Pack<T, V> (&q)[kWideLoads], int64_t k, int tid,
+                                       int threads, float outside) const {
+    const T* p = base + granule(k, 0, tid, threads) * V;
+    if (g0 + threads * kWideLoads * (k + 1) <= g1) {  // all threads have all of them
+#pragma unroll
+      for (int u = 0; u < kWideLoads; ++u) q[u] = load_pack<T, V>(p + u * threads * V);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kWideLoads; ++u) {
+        if (granule(k, u, tid, threads) < g1) {
+          q[u] = load_pack<T, V>(p + u * threads * V);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) q[u].e[e] = from_f<T>(outside);
+        }
+      }
+    }
   }
 };
 
@@ -349,38 +376,31 @@ __device__ __forceinline__ void team_sync() {
 //   s = sum over x < m of e^((x - m) / T),  cnt = how many x equal m,
 //   t = sum of e^((x - m) / T) (x - m)
 // with `scale` = log2(e) / T.  m may be any value that is not below what was
-// seen (a thread that starts with its team's maximum meets larger ones rarely,
-// and both branches below are rare).
+// seen: a thread starts with its team's maximum and meets larger ones rarely.
 template <typename T, bool ENTROPY>
 struct Stream {
-  float m, cnt;
+  float m, ref, cnt;  // ref = m, or 0 while m is -inf
   F2 s, t;
   __device__ __forceinline__ explicit Stream(float start)
-      : m(start), cnt(0.0f), s{0.0f, 0.0f}, t{0.0f, 0.0f} {}
-  // `most` = max_of(v); NaN makes s NaN.
+      : m(start), ref(start == -INFINITY ? 0.0f : start), cnt(0.0f), s{0.0f, 0.0f}, t{0.0f, 0.0f} {}
+  // `most` = max_of(v); NaN makes s NaN.  Changes v.
   template <int N>
-  __device__ __forceinline__ void add(const F2 (&v)[N], float most, float scale) {
-    if (most > m) raise(most, scale);
-    if (most == m) {  // the maximum's e^0 is counted, not added
+  __device__ __forceinline__ void add(F2 (&v)[N], float most, float scale) {
+    if (most >= m) {
+      if (most > m) raise(most, scale);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const bool px = v[i].x == m, py = v[i].y == m;  // -inf, too
-        F2 d = add2(v[i], both(-m));
-        d = F2{px ? 0.0f : max_nan(d.x, kExpFloor), py ? 0.0f : max_nan(d.y, kExpFloor)};
-        const F2 e = exp_neg2<T>(d, scale);
-        cnt += (px ? 1.0f : 0.0f) + (py ? 1.0f : 0.0f);
-        s = add2(s, F2{px ? 0.0f : e.x, py ? 0.0f : e.y});
-        if (ENTROPY) t = fma2(e, d, t);
+      for (int i = 0; i < N; ++i) {  // the maximum's e^0 is counted, not added
+        if (v[i].x == m) { cnt += 1.0f; v[i].x = -INFINITY; }
+        if (v[i].y == m) { cnt += 1.0f; v[i].y = -INFINITY; }
       }
-    } else {
+    }
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        F2 d = add2(v[i], both(-m));
-        d = F2{max_nan(d.x, kExpFloor), max_nan(d.y, kExpFloor)};
-        const F2 e = exp_neg2<T>(d, scale);
-        s = add2(s, e);
-        if (ENTROPY) t = fma2(e, d, t);
-      }
+    for (int i = 0; i < N; ++i) {
+      F2 d = add2(v[i], both(-ref));
+      d = F2{max_nan(d.x, kExpFloor), max_nan(d.y, kExpFloor)};
+      const F2 e = exp_neg2<T>(d, scale);
+      s = add2(s, e);
+      if (ENTROPY) t = fma2(e, d, t);
     }
   }
   __device__ __forceinline__ void raise(float to, float scale) {
@@ -390,7 +410,7 @@ struct Stream {
     if (ENTROPY) t = F2{fmaf(n, d, f * (t.x + t.y)), 0.0f};
     s = F2{n, 0.0f};
     cnt = 0.0f;
-    m = to;
+    m = ref = to;
   }
 };
 

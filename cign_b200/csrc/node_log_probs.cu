@@ -51,50 +51,64 @@ __device__ __forceinline__ void write_row(const LogProbOut& out, int64_t row, co
   }
 }
 
-// The best classes that one warp has met, best first: place p = 32 i + lane in
-// key[i] of the lane (class_key; 0 = none yet).
-struct BestList {
-  uint64_t key[kLpMaxTop / 32];
-  uint64_t last;  // at place top_k - 1
-  __device__ __forceinline__ BestList() : last(0) {
-#pragma unroll
-    for (int i = 0; i < kLpMaxTop / 32; ++i) key[i] = 0;
-  }
-  // All lanes with the same key, which is larger than `last`.
-  __device__ __forceinline__ void insert(uint64_t k, int top_k) {
-    const int lane = threadIdx.x & 31;
-    uint64_t carry = k;
-#pragma unroll
-    for (int i = 0; i < kLpMaxTop / 32; ++i) {
-      const int place = __popc(__ballot_sync(kFullMask, key[i] > carry));
-      const uint64_t out = __shfl_sync(kFullMask, key[i], 31);
-      const uint64_t up = __shfl_up_sync(kFullMask, key[i], 1);
-      if (lane == place) key[i] = carry;
-      else if (lane > place) key[i] = up;
-      if (place == 32) continue;  // all of these are larger
-      carry = out;
-      if (top_k <= 32 * (i + 1)) break;
-    }
-    static_assert(kLpMaxTop == 64, "two keys per lane");
-    last = __shfl_sync(kFullMask, top_k <= 32 ? key[0] : key[1], (top_k - 1) % 32);
-  }
-};
-
 // Team of W warps per row; with W = 8 a cluster of blocks may share a row.
+constexpr int kLpKept = 128;  // classes that a warp keeps at most before it sorts them out
 template <int W>
 struct alignas(16) WideShared {
   static constexpr int kThreads = 32 * W;
-  uint32_t most[kThreads];     // value keys of the threads' maxima
-  uint32_t floor;              // value key that top_k classes at least reach
+  uint32_t most[kThreads];  // value keys of maxima
+  uint32_t floor;           // value key that top_k classes at least reach
   int count;
+  uint64_t kept[W][kLpKept];
   uint64_t best[W * kLpMaxTop];
   uint64_t sorted[kLpMaxTop];
   Sums part[W];
   Sums sums;
 };
 
-// The top_k largest of `count` different keys, sorted, into `sorted`: a key's
-// place is the number of larger ones.
+// The classes of one warp that may belong to the best: those that reached the
+// floor when they were met, in no order.
+struct Kept {
+  int count = 0;
+  // Appends the lanes' keys where `take` is set; more than the warp can keep
+  // are reduced to the best top_k, whose last raises the floor.
+  __device__ __forceinline__ void add(uint64_t key, bool take, uint64_t* list, int top_k,
+                                      uint32_t* floor) {
+    const int lane = threadIdx.x & 31;
+    const unsigned who = __ballot_sync(kFullMask, take);
+    if (take) list[count + __popc(who & ((1u << lane) - 1u))] = key;
+    count += __popc(who);
+    if (count > kLpKept - 32) reduce(list, top_k, floor);
+  }
+  // A key's place is the number of larger ones (all differ).
+  __device__ __noinline__ void reduce(uint64_t* list, int top_k, uint32_t* floor) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    uint64_t k[kLpKept / 32];
+    int place[kLpKept / 32];
+#pragma unroll
+    for (int i = 0; i < kLpKept / 32; ++i) {
+      k[i] = 32 * i + lane < count ? list[32 * i + lane] : 0;
+      place[i] = 0;
+    }
+    for (int j = 0; j < count; ++j) {
+      const uint64_t o = list[j];
+#pragma unroll
+      for (int i = 0; i < kLpKept / 32; ++i) place[i] += o > k[i] ? 1 : 0;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kLpKept / 32; ++i)
+      if (32 * i + lane < count && place[i] < top_k) {
+        list[place[i]] = k[i];
+        if (place[i] == top_k - 1) atomicMax(floor, static_cast<uint32_t>(k[i] >> 32));
+      }
+    __syncwarp();
+    count = count < top_k ? count : top_k;
+  }
+};
+
+// The top_k largest of `count` different keys, sorted, into `sorted`.
 template <int W>
 __device__ __forceinline__ void sort_best(WideShared<W>& sh, int count, int top_k, int tid) {
   for (int i = tid; i < count; i += 32 * W) {
@@ -105,13 +119,34 @@ __device__ __forceinline__ void sort_best(WideShared<W>& sh, int count, int top_
   }
 }
 
+// A floor for the best classes from the maxima of the team's threads: the
+// top_k-th largest maximum of disjoint sets of classes is reached by top_k
+// classes.  The sets are those of B threads joined, B at least twice top_k
+// where the team has so many, and the threads of a set share its comparisons.
+template <int W>
+__device__ __forceinline__ void first_floor(WideShared<W>& sh, uint32_t mine, int top_k, int tid) {
+  constexpr int kThreads = 32 * W;
+  int sets = kThreads;
+  while (sets > 32 && sets / 2 >= 2 * top_k) sets /= 2;
+  const int join = kThreads / sets;  // at most 8 neighbouring lanes
+  for (int o = 1; o < join; o <<= 1) mine = max(mine, __shfl_xor_sync(kFullMask, mine, o));
+  if (tid % join == 0) sh.most[tid / join] = mine;
+  team_sync<W>();
+  const int share = sets / join;
+  int above = 0;
+  for (int j = tid % join * share; j < (tid % join + 1) * share; j += 4) {
+    const uint4 o = *reinterpret_cast<const uint4*>(sh.most + j);
+    above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+  }
+  for (int o = 1; o < join; o <<= 1) above += __shfl_xor_sync(kFullMask, above, o);
+  if (above < top_k && tid % join == 0) atomicMin(&sh.floor, mine);
+}
+
 // One pass over the row.  The first loads of all threads give the team's
-// maximum, from which the sums start, and a floor for the best classes: the
-// top_k-th largest of the threads' maxima is reached by top_k classes.  Only
-// what reaches the floor is looked at again: each warp keeps its best top_k,
-// and a full list raises the floor for all.
-template <typename T, int W>
-__global__ void __launch_bounds__(W == 1 ? 128 : 32 * W)
+// maximum, from which the sums start, and the floor of the best classes; only
+// what reaches the floor is looked at again.
+template <typename T, int W, bool TOP>
+__global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 8 ? 3 : 6)
 log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld,
                           const int64_t* __restrict__ labels, int top_k, int split,
                           LogProbOut out) {
@@ -127,120 +162,108 @@ log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
   const int64_t row = W == 8 ? blockIdx.x / split : static_cast<int64_t>(blockIdx.x) * kTeams + team;
   if (row >= n) return;  // a whole team
   const T* x = logits + row * ld;
-  const RowFrame<T> frame(x, c);
-  const int64_t g0 = W == 8 ? frame.granules * rank / split : 0;
-  const int64_t g1 = W == 8 ? frame.granules * (rank + 1) / split : frame.granules;
+  const RowFrame<T> frame(x, c, rank, W == 8 ? split : 1);
+  const int64_t rounds = frame.rounds(kThreads);
 
-  Pack<T, V> q[kWideLoads];
+  Pack<T, V> q[kWideLoads], next[kWideLoads];
   F2 v[V / 2];
+  frame.load(q, 0, tid, kThreads, -INFINITY);
+  // the two ends of the row, by the first two threads
+  const int64_t edge = tid == 0 ? frame.head : tid == 1 ? frame.tail : -1;
+  const Pack<T, V> ends = frame.edge(edge, -INFINITY);
   float most = -INFINITY;
-#pragma unroll
-  for (int u = 0; u < kWideLoads; ++u) {
-    const int64_t g = g0 + tid + u * kThreads;
-    q[u] = frame.load(g < g1 ? g : frame.granules, -INFINITY);
-  }
 #pragma unroll
   for (int u = 0; u < kWideLoads; ++u) {
     unpack(q[u], v);
     most = max_nan(most, max_of(v));
   }
+  unpack(ends, v);
+  most = max_nan(most, max_of(v));
   float start = warp_max(most);  // skips NaN
   if (start != start) start = -INFINITY;
+  if (W > 1 && lane == 0) sh.part[tid >> 5].m = start;
+  if (tid == 0) {
+    sh.floor = 0xffffffffu;
+    sh.count = 0;
+  }
+  team_sync<W>();
   if (W > 1) {
-    if (lane == 0) sh.part[tid >> 5].m = start;
-    sh.most[tid] = value_key(most);
-    if (tid == 0) sh.floor = 0;
-    __syncthreads();
 #pragma unroll
     for (int w = 0; w < W; ++w) start = fmaxf(start, sh.part[w].m);
-  } else {
-    sh.most[tid] = value_key(most);
-    if (tid == 0) sh.floor = 0;
-    __syncwarp();
   }
-  if (top_k > 0 && top_k <= kThreads) {
-    const uint32_t mine = value_key(most);
-    int place = 0;
-    for (int j = 0; j < kThreads; j += 4) {
-      const uint4 o = *reinterpret_cast<const uint4*>(sh.most + j);
-      place += (o.x > mine || (o.x == mine && j < tid)) + (o.y > mine || (o.y == mine && j + 1 < tid)) +
-               (o.z > mine || (o.z == mine && j + 2 < tid)) + (o.w > mine || (o.w == mine && j + 3 < tid));
-    }
-    if (place == top_k - 1) sh.floor = mine;
+  if (TOP) {
+    first_floor<W>(sh, value_key(most), top_k, tid);
+    team_sync<W>();
+    if (tid == 0 && top_k > kThreads) sh.floor = 0;  // fewer maxima than classes asked for
+    team_sync<W>();
   }
-  if (tid == 0) sh.count = 0;
-  team_sync<W>();
 
   Stream<T, true> sums(start);
-  BestList best;
-  for (int64_t g = g0 + tid;; g += kWideLoads * kThreads) {
+  Kept kept;
+  // The lanes' granules g (-1: none), whose largest classes are `top`: keep what
+  // reaches the floor.  Few do, so they are read again instead of held.
+  const auto look = [&](int64_t g, float top, float floor) {
+    if (!__any_sync(kFullMask, !(top < floor))) return;
+#pragma unroll 1
+    for (int e = 0; e < V; ++e) {
+      const int64_t f = g * V + e;
+      const bool in = g >= 0 && f >= frame.shift && f < frame.end;
+      const float xe = in ? to_f(frame.base[f]) : 0.0f;
+      const bool take = in && !(xe < floor);
+      if (__any_sync(kFullMask, take))
+        kept.add(class_key(xe, static_cast<uint32_t>(f - frame.shift)), take, sh.kept[tid >> 5],
+                 top_k, &sh.floor);
+    }
+  };
+  {
+    const float top = max_of(v);
+    sums.add(v, top, kLog2e);
+    if (TOP && tid < 32) look(edge, top, key_value(*const_cast<volatile uint32_t*>(&sh.floor)));
+  }
+  for (int64_t k = 0; k < rounds; ++k) {
+    if (k + 1 < rounds) frame.load(next, k + 1, tid, kThreads, -INFINITY);
+    const float floor = TOP ? key_value(*const_cast<volatile uint32_t*>(&sh.floor)) : 0.0f;
 #pragma unroll
     for (int u = 0; u < kWideLoads; ++u) {
       unpack(q[u], v);
       const float top = max_of(v);
       sums.add(v, top, kLog2e);
-      if (top_k == 0) continue;
-      const uint32_t floor = *const_cast<const volatile uint32_t*>(&sh.floor);
-      if (!__any_sync(kFullMask, value_key(top) >= floor)) continue;
-      // the lanes' classes that may belong to the best, one per lane at a time
-      const int64_t first = (g + u * kThreads) * V - frame.shift;
-      uint32_t left = 0;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float xe = e % 2 == 0 ? v[e / 2].x : v[e / 2].y;
-        if (value_key(xe) >= floor && first + e >= 0 && first + e < c) left |= 1u << e;
+      if (TOP) {
+        const int64_t g = frame.granule(k, u, tid, kThreads);
+        look(g < frame.g1 ? g : -1, top, floor);
       }
-      if (g + u * kThreads >= g1) left = 0;
-      while (__any_sync(kFullMask, left != 0)) {
-        const int pick = __ffs(left) - 1;
-        float xe = 0.0f;
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (e == pick) xe = e % 2 == 0 ? v[e / 2].x : v[e / 2].y;
-        const uint64_t key =
-            left ? class_key(xe, static_cast<uint32_t>(first + pick)) : 0;
-        left &= left - 1;
-        unsigned who = __ballot_sync(kFullMask, key > best.last);
-        while (who) {
-          const uint64_t k = __shfl_sync(kFullMask, key, __ffs(who) - 1);
-          who &= who - 1;
-          if (k > best.last) best.insert(k, top_k);
-        }
-        const uint32_t reached = static_cast<uint32_t>(best.last >> 32);
-        if (lane == 0 && reached > floor) atomicMax(&sh.floor, reached);
-      }
-    }
-    if (g - tid + kWideLoads * kThreads >= g1) break;  // the same for the whole team
-#pragma unroll
-    for (int u = 0; u < kWideLoads; ++u) {
-      const int64_t h = g + (kWideLoads + u) * kThreads;
-      q[u] = frame.load(h < g1 ? h : frame.granules, -INFINITY);
+      q[u] = next[u];
     }
   }
 
   Sums a{sums.m, sums.s.x + sums.s.y, sums.cnt, sums.t.x + sums.t.y};
   a = join_warp<T>(a, kLog2e);
   if (W > 1) {
+    __syncthreads();  // part was read above
     if (lane == 0) sh.part[tid >> 5] = a;
-    __syncthreads();
+  }
+  if (TOP) {
+    if (kept.count > kLpMaxTop) kept.reduce(sh.kept[tid >> 5], top_k, &sh.floor);
+    if (tid < kLpMaxTop) sh.sorted[tid] = 0;
+    for (int i = tid + kThreads; i < kLpMaxTop; i += kThreads) sh.sorted[i] = 0;
+  }
+  team_sync<W>();
+  if (W > 1) {
     a = sh.part[0];
 #pragma unroll
     for (int w = 1; w < W; ++w) a = join<T>(a, sh.part[w], kLog2e);
   }
-  if (top_k > 0) {
-    const uint32_t floor = *const_cast<const volatile uint32_t*>(&sh.floor);
-#pragma unroll
-    for (int i = 0; i < kLpMaxTop / 32; ++i) {
-      const bool keep = best.key[i] != 0 && 32 * i + lane < top_k &&
-                        static_cast<uint32_t>(best.key[i] >> 32) >= floor;
+  if (TOP) {
+    const uint32_t floor = *const_cast<volatile uint32_t*>(&sh.floor);
+    for (int i = lane; i - lane < kept.count; i += 32) {
+      const uint64_t k = i < kept.count ? sh.kept[tid >> 5][i] : 0;
+      const bool keep = i < kept.count && static_cast<uint32_t>(k >> 32) >= floor;
       const unsigned who = __ballot_sync(kFullMask, keep);
       int at = 0;
       if (lane == 0 && who) at = atomicAdd(&sh.count, __popc(who));
       at = __shfl_sync(kFullMask, at, 0) + __popc(who & ((1u << lane) - 1u));
-      if (keep) sh.best[at] = best.key[i];
+      if (keep) sh.best[at] = k;
     }
-    if (tid < kLpMaxTop) sh.sorted[tid] = 0;
-    for (int i = tid + kThreads; i < kLpMaxTop; i += kThreads) sh.sorted[i] = 0;
     team_sync<W>();
     sort_best<W>(sh, sh.count, top_k, tid);
   }
@@ -252,10 +275,9 @@ log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
     if (rank == 0) {
       for (int r = 1; r < split; ++r)
         a = join<T>(a, cluster.map_shared_rank(&sh, r)->sums, kLog2e);
-      if (top_k > 0) {
-        uint64_t own = 0;
+      if (TOP) {
         const int count = split * top_k;
-        for (int i = tid; i < top_k; i += kThreads) own = sh.sorted[i];
+        const uint64_t own = tid < top_k ? sh.sorted[tid] : 0;
         __syncthreads();
         if (tid < top_k) sh.best[tid] = own;
         for (int i = tid + top_k; i < count; i += kThreads)
@@ -272,7 +294,7 @@ log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
     const int64_t y = out.log_prob ? labels[row] : -1;
     write_row(out, row, st, y, y >= 0 && y < c ? to_f(x[y]) : 0.0f, c);
   }
-  if (top_k > 0) {
+  if (TOP) {
     team_sync<W>();
     const float logs = stat_log(st);
     for (int i = tid; i < top_k; i += kThreads) {
@@ -544,17 +566,20 @@ int cign_node_log_probs_fwd(int64_t n, int64_t c, int32_t x_type, const void* lo
   const int64_t granules = c * type_size(x_type) / 16;
   CIGN_TYPE_DISPATCH(x_type, T, {
     const T* x = static_cast<const T*>(logits);
-    if (granules <= 2 * 32 * kWideLoads) {
-      log_probs_wide_fwd_kernel<T, 1><<<static_cast<unsigned>((n + 3) / 4), 128, 0, s>>>(
-          n, c, x, ld, labels, top_k, 1, out);
-    } else if (granules <= 2 * 128 * kWideLoads) {
-      log_probs_wide_fwd_kernel<T, 4><<<static_cast<unsigned>(n), 128, 0, s>>>(
-          n, c, x, ld, labels, top_k, 1, out);
+    if (granules <= 2 * 128 * kWideLoads) {
+      const bool one = granules <= 2 * 32 * kWideLoads;
+      const auto kernel = one ? (top_k ? log_probs_wide_fwd_kernel<T, 1, true>
+                                       : log_probs_wide_fwd_kernel<T, 1, false>)
+                              : (top_k ? log_probs_wide_fwd_kernel<T, 4, true>
+                                       : log_probs_wide_fwd_kernel<T, 4, false>);
+      kernel<<<static_cast<unsigned>(one ? (n + 3) / 4 : n), 128, 0, s>>>(n, c, x, ld, labels,
+                                                                         top_k, 1, out);
     } else {
       const int split = wide_split(n, granules, 256);
-      return launch_cluster(log_probs_wide_fwd_kernel<T, 8>, static_cast<unsigned>(n * split), 256,
-                            0, split, s, "log_probs_wide_fwd_kernel", n, c, x, ld, labels, top_k,
-                            split, out);
+      return launch_cluster(top_k ? log_probs_wide_fwd_kernel<T, 8, true>
+                                  : log_probs_wide_fwd_kernel<T, 8, false>,
+                            static_cast<unsigned>(n * split), 256, 0, split, s,
+                            "log_probs_wide_fwd_kernel", n, c, x, ld, labels, top_k, split, out);
     }
   });
   CIGN_CHECK_LAUNCH("log_probs_wide_fwd_kernel");
