@@ -58,6 +58,7 @@ struct alignas(16) WideShared {
   static constexpr int kThreads = 32 * W;
   uint32_t most[kThreads];  // value keys of maxima
   uint32_t floor;           // value key that top_k classes at least reach
+  uint32_t next_floor;
   int count;
   uint64_t kept[W][kLpKept];
   uint64_t best[W * kLpMaxTop];
@@ -119,13 +120,15 @@ __device__ __forceinline__ void sort_best(WideShared<W>& sh, int count, int top_
   }
 }
 
-// A floor for the best classes from the maxima of the team's threads: the
-// top_k-th largest maximum of disjoint sets of classes is reached by top_k
-// classes.  The sets are those of B threads joined, B at least twice top_k
-// where the team has so many, and the threads of a set share its comparisons.
+// Raises the floor of the best classes by the maxima of what the team's threads
+// have seen: the top_k-th largest maximum of disjoint sets of classes is reached
+// by top_k classes.  The sets are those of B threads joined, B at least twice
+// top_k where the team has so many, and the threads of a set share its
+// comparisons.  sh.next_floor is ~0 before and after.
 template <int W>
-__device__ __forceinline__ void first_floor(WideShared<W>& sh, uint32_t mine, int top_k, int tid) {
+__device__ __forceinline__ void raise_floor(WideShared<W>& sh, uint32_t mine, int top_k, int tid) {
   constexpr int kThreads = 32 * W;
+  if (top_k > kThreads) return;  // fewer maxima than classes asked for
   int sets = kThreads;
   while (sets > 32 && sets / 2 >= 2 * top_k) sets /= 2;
   const int join = kThreads / sets;  // at most 8 neighbouring lanes
@@ -139,7 +142,13 @@ __device__ __forceinline__ void first_floor(WideShared<W>& sh, uint32_t mine, in
     above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
   }
   for (int o = 1; o < join; o <<= 1) above += __shfl_xor_sync(kFullMask, above, o);
-  if (above < top_k && tid % join == 0) atomicMin(&sh.floor, mine);
+  if (above < top_k && tid % join == 0) atomicMin(&sh.next_floor, mine);
+  team_sync<W>();
+  if (tid == 0) {
+    atomicMax(&sh.floor, sh.next_floor);
+    sh.next_floor = 0xffffffffu;
+  }
+  team_sync<W>();
 }
 
 // One pass over the row.  The first loads of all threads give the team's
@@ -183,7 +192,8 @@ log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
   if (start != start) start = -INFINITY;
   if (W > 1 && lane == 0) sh.part[tid >> 5].m = start;
   if (tid == 0) {
-    sh.floor = 0xffffffffu;
+    sh.floor = 0;
+    sh.next_floor = 0xffffffffu;
     sh.count = 0;
   }
   team_sync<W>();
@@ -191,28 +201,21 @@ log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
 #pragma unroll
     for (int w = 0; w < W; ++w) start = fmaxf(start, sh.part[w].m);
   }
-  if (TOP) {
-    first_floor<W>(sh, value_key(most), top_k, tid);
-    team_sync<W>();
-    if (tid == 0 && top_k > kThreads) sh.floor = 0;  // fewer maxima than classes asked for
-    team_sync<W>();
-  }
+  if (TOP) raise_floor<W>(sh, value_key(most), top_k, tid);
 
   Stream<T, true> sums(start);
   Kept kept;
   // The lanes' granules g (-1: none), whose largest classes are `top`: keep what
-  // reaches the floor.  Few do, so they are read again instead of held.
+  // reaches the floor.  Few granules do; V lanes read each again.
   const auto look = [&](int64_t g, float top, float floor) {
-    if (!__any_sync(kFullMask, !(top < floor))) return;
-#pragma unroll 1
-    for (int e = 0; e < V; ++e) {
-      const int64_t f = g * V + e;
-      const bool in = g >= 0 && f >= frame.shift && f < frame.end;
+    unsigned who = __ballot_sync(kFullMask, !(top < floor) && g >= 0);
+    while (who) {
+      const int64_t f = __shfl_sync(kFullMask, g, __ffs(who) - 1) * V + lane;
+      who &= who - 1;
+      const bool in = lane < V && f >= frame.shift && f < frame.end;
       const float xe = in ? to_f(frame.base[f]) : 0.0f;
-      const bool take = in && !(xe < floor);
-      if (__any_sync(kFullMask, take))
-        kept.add(class_key(xe, static_cast<uint32_t>(f - frame.shift)), take, sh.kept[tid >> 5],
-                 top_k, &sh.floor);
+      kept.add(class_key(xe, static_cast<uint32_t>(f - frame.shift)), in && !(xe < floor),
+               sh.kept[tid >> 5], top_k, &sh.floor);
     }
   };
   {
@@ -231,9 +234,13 @@ log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
       if (TOP) {
         const int64_t g = frame.granule(k, u, tid, kThreads);
         look(g < frame.g1 ? g : -1, top, floor);
+        most = max_nan(most, top);
       }
       q[u] = next[u];
     }
+    // after 2, 4, 8, ... rounds: each raise halves what the coming rounds keep
+    if (TOP && k > 0 && (k & (k + 1)) == 0 && k + 1 < rounds)
+      raise_floor<W>(sh, value_key(most), top_k, tid);
   }
 
   Sums a{sums.m, sums.s.x + sums.s.y, sums.cnt, sums.t.x + sums.t.y};
