@@ -113,6 +113,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// The largest and the smallest of three.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ float exp2_hw(float t) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
@@ -295,54 +306,59 @@ __device__ __forceinline__ float key_value(uint32_t u) {
 // aligned bytes per thread and load.  A row may start anywhere: granule g of
 // V = 16 / sizeof(T) elements covers the row's elements g V - shift ..., and the
 // two granules at its ends are read by elements.
-constexpr int kWideLoads = 4;  // granules of a thread that are in flight together
+// Granules of a thread that are in flight together (and as many are worked on).
+template <typename T>
+constexpr int kWideLoads = 4;
+
+constexpr int64_t kWideMax = (1ll << 31) - 16;  // classes: positions in a row are 32-bit
 
 template <typename T>
 struct RowFrame {
   static constexpr int V = 16 / sizeof(T);
   const T* base;  // aligned address of granule 0, at most V - 1 elements before the row
-  int64_t shift;  // the row begins at element `shift` of the frame
-  int64_t end;    // and ends before this one
-  int64_t granules;
-  int64_t g0, g1;  // the whole granules among those of this team's share
-  int64_t head, tail;  // granules of the share that are not whole, or -1
+  int shift;      // the row begins at element `shift` of the frame
+  int end;        // and ends before this one
+  int g0, g1;     // the whole granules of this team's share of the row
+  int head, tail; // granules of the share that are not whole, or -1
   __device__ __forceinline__ RowFrame(const T* row, int64_t c, int rank, int split) {
-    shift = static_cast<int64_t>((reinterpret_cast<uintptr_t>(row) % 16) / sizeof(T));
+    shift = static_cast<int>((reinterpret_cast<uintptr_t>(row) % 16) / sizeof(T));
     base = row - shift;
-    end = shift + c;
-    granules = (end + V - 1) / V;
-    g0 = split > 1 ? granules * rank / split : 0;
-    g1 = split > 1 ? granules * (rank + 1) / split : granules;
+    end = shift + static_cast<int>(c);
+    const int granules = (end + V - 1) / V;
+    g0 = split > 1 ? static_cast<int>(static_cast<int64_t>(granules) * rank / split) : 0;
+    g1 = split > 1 ? static_cast<int>(static_cast<int64_t>(granules) * (rank + 1) / split)
+                   : granules;
     head = g0 == 0 && shift > 0 ? g0++ : -1;
-    tail = g1 == granules && end % V != 0 ? --g1 : -1;
+    tail = g1 == granules && end % V != 0 && g1 > g0 ? --g1 : -1;
   }
+  __device__ __forceinline__ bool inside(int f) const { return f >= shift && f < end; }
   // A granule that is not whole, elements outside of the row as `outside`.
-  __device__ __forceinline__ Pack<T, V> edge(int64_t g, float outside) const {
+  __device__ __forceinline__ Pack<T, V> edge(int g, float outside) const {
     Pack<T, V> q;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int64_t f = g * V + e;
-      q.e[e] = g >= 0 && f >= shift && f < end ? base[f] : from_f<T>(outside);
+      const int f = g * V + e;
+      q.e[e] = g >= 0 && inside(f) ? base[f] : from_f<T>(outside);
     }
     return q;
   }
-  // Thread `tid` of `threads`: whole granules g0 + tid + threads (k kWideLoads + u).
-  __device__ __forceinline__ int64_t granule(int64_t k, int u, int tid, int threads) const {
-    return g0 + tid + threads * (k * kWideLoads + u);
+  // Thread `tid` of `threads` has the whole granules g0 + tid + threads (k L + u), u < L.
+  template <int L>
+  __device__ __forceinline__ int rounds(int threads) const {
+    return (g1 - g0 + threads * L - 1) / (threads * L);
   }
-  __device__ __forceinline__ int64_t rounds(int threads) const {
-    return (g1 - g0 + threads * kWideLoads - 1) / (threads * kWideLoads);
-  }
-  __device__ __forceinline__ void load(Pack<T, V> (&q)[kWideLoads], int64_t k, int tid,
-                                       int threads, float outside) const {
-    const T* p = base + granule(k, 0, tid, threads) * V;
-    if (g0 + threads * kWideLoads * (k + 1) <= g1) {  // all threads have all of them
+  template <int L>
+  __device__ __forceinline__ void load(Pack<T, V> (&q)[L], int k, int tid, int threads,
+                                       float outside) const {
+    const int g = g0 + tid + threads * L * k;
+    const T* p = base + static_cast<int64_t>(g) * V;
+    if (g - tid + threads * L <= g1) {  // all threads have all of them
 #pragma unroll
-      for (int u = 0; u < kWideLoads; ++u) q[u] = load_pack<T, V>(p + u * threads * V);
+      for (int u = 0; u < L; ++u) q[u] = load_pack<T, V>(p + u * threads * V);
     } else {
 #pragma unroll
-      for (int u = 0; u < kWideLoads; ++u) {
-        if (granule(k, u, tid, threads) < g1) {
+      for (int u = 0; u < L; ++u) {
+        if (g + u * threads < g1) {
           q[u] = load_pack<T, V>(p + u * threads * V);
         } else {
 #pragma unroll
@@ -362,7 +378,14 @@ template <int N>
 __device__ __forceinline__ float max_of(const F2 (&v)[N]) {
   float m = max_nan(v[0].x, v[0].y);
 #pragma unroll
-  for (int i = 1; i < N; ++i) m = max_nan(m, max_nan(v[i].x, v[i].y));
+  for (int i = 1; i < N; ++i) m = max3_nan(m, v[i].x, v[i].y);
+  return m;
+}
+template <int N>
+__device__ __forceinline__ float min_of(const F2 (&v)[N]) {
+  float m = min3_nan(v[0].x, v[0].y, INFINITY);
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = min3_nan(m, v[i].x, v[i].y);
   return m;
 }
 
@@ -377,12 +400,45 @@ __device__ __forceinline__ void team_sync() {
 //   t = sum of e^((x - m) / T) (x - m)
 // with `scale` = log2(e) / T.  m may be any value that is not below what was
 // seen: a thread starts with its team's maximum and meets larger ones rarely.
+//
+// 16-bit logits take the exponent x scale - m scale in one operation and sum
+// e 2^x's argument instead of e (x - m); what the rounding of m scale leaves,
+// the same factor in every term, is put back when the sums are read.  The
+// kernels are bound by issue: each operation per logit counts.
 template <typename T, bool ENTROPY>
 struct Stream {
-  float m, ref, cnt;  // ref = m, or 0 while m is -inf
-  F2 s, t;
-  __device__ __forceinline__ explicit Stream(float start)
-      : m(start), ref(start == -INFINITY ? 0.0f : start), cnt(0.0f), s{0.0f, 0.0f}, t{0.0f, 0.0f} {}
+  static constexpr bool kOneStep = sizeof(T) == 2;
+  float m, ref, cnt;  // ref = m but where m scale would overflow to -inf
+  float shift;        // kOneStep: ref scale, rounded
+  F2 s, u;            // u: kOneStep: sum of e times the argument; else t
+  __device__ __forceinline__ Stream(float start, float scale)
+      : cnt(0.0f), s{0.0f, 0.0f}, u{0.0f, 0.0f} {
+    set(start, scale);
+  }
+  __device__ __forceinline__ void set(float to, float scale) {
+    m = to;
+    ref = fmaxf(to, -1e30f);
+    shift = ref * scale;
+  }
+  template <bool CLAMP, int N>
+  __device__ __forceinline__ void sum(const F2 (&v)[N], float scale) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (kOneStep) {
+        F2 a = fma2(v[i], both(scale), both(-shift));
+        if (CLAMP) a = F2{max_nan(a.x, kExpFloor), max_nan(a.y, kExpFloor)};
+        const F2 e{exp2_hw(a.x), exp2_hw(a.y)};
+        s = add2(s, e);
+        if (ENTROPY) u = fma2(e, a, u);
+      } else {
+        F2 d = add2(v[i], both(-ref));
+        if (CLAMP) d = F2{max_nan(d.x, kExpFloor), max_nan(d.y, kExpFloor)};
+        const F2 e = exp_neg2<T>(d, scale);
+        s = add2(s, e);
+        if (ENTROPY) u = fma2(e, d, u);
+      }
+    }
+  }
   // `most` = max_of(v); NaN makes s NaN.  Changes v.
   template <int N>
   __device__ __forceinline__ void add(F2 (&v)[N], float most, float scale) {
@@ -394,49 +450,61 @@ struct Stream {
         if (v[i].y == m) { cnt += 1.0f; v[i].y = -INFINITY; }
       }
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      F2 d = add2(v[i], both(-ref));
-      d = F2{max_nan(d.x, kExpFloor), max_nan(d.y, kExpFloor)};
-      const F2 e = exp_neg2<T>(d, scale);
-      s = add2(s, e);
-      if (ENTROPY) t = fma2(e, d, t);
-    }
+    // -inf would make 0 times inf of u; the arithmetic of finite values needs no floor
+    if (min_of(v) - ref < kExpFloor) sum<true>(v, scale);
+    else sum<false>(v, scale);
+  }
+  __device__ __forceinline__ float total_s(float scale) const {
+    const float x = s.x + s.y;
+    return kOneStep ? x * exp2_hw(left(scale)) : x;
+  }
+  __device__ __forceinline__ float total_t(float scale) const {
+    const float x = u.x + u.y;
+    const float r = left(scale);
+    return kOneStep ? exp2_hw(r) * fmaf(r, s.x + s.y, x) / scale : x;
+  }
+  __device__ __forceinline__ float left(float scale) const {  // of rounding ref scale
+    const float r = -fmaf(ref, scale, -shift);
+    return fabsf(shift) < 1e30f ? r : 0.0f;
   }
   __device__ __forceinline__ void raise(float to, float scale) {
     const float d = max_nan(m - to, kExpFloor);
     const float f = exp_neg2<T>(both(d), scale).x;
-    const float n = (s.x + s.y + cnt) * f;
-    if (ENTROPY) t = F2{fmaf(n, d, f * (t.x + t.y)), 0.0f};
+    const float n = (total_s(scale) + cnt) * f;
+    if (ENTROPY) {
+      const float t = fmaf(n, d, f * total_t(scale));
+      u = F2{kOneStep ? t * scale : t, 0.0f};
+    }
     s = F2{n, 0.0f};
     cnt = 0.0f;
-    m = ref = to;
+    set(to, scale);
+    if (kOneStep) {  // as sums whose rounding is still to be put back
+      const float r = left(scale), g = exp2_hw(-r);
+      s.x *= g;
+      u.x = g * u.x - r * s.x;
+    }
   }
 };
 
-// The same of a whole team or row.  (m, s, cnt, t) of two disjoint sets join by
-// raising the lower one.
+// The same of a whole team or row.  Disjoint sets join by raising the lower ones
+// to the highest maximum.
 struct Sums {
   float m, s, cnt, t;
 };
+// Over the warp; every lane gets it.  Lanes that hold nothing have m = -inf and
+// zeros.
 template <typename T>
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b, float scale) {
-  const bool ge = a.m >= b.m;
-  const Sums hi = ge ? a : b, lo = ge ? b : a;
-  if (a.m == b.m) return Sums{hi.m, hi.s + lo.s, hi.cnt + lo.cnt, hi.t + lo.t};
-  const float d = max_nan(lo.m - hi.m, kExpFloor);
-  const float f = exp_neg2<T>(both(d), scale).x;
-  const float n = (lo.s + lo.cnt) * f;
-  return Sums{hi.m, hi.s + n, hi.cnt, hi.t + fmaf(n, d, f * lo.t)};
-}
-template <typename T>
-__device__ __forceinline__ Sums join_warp(Sums a, float scale) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    a = join<T>(a, Sums{__shfl_xor_sync(kFullMask, a.m, o), __shfl_xor_sync(kFullMask, a.s, o),
-                        __shfl_xor_sync(kFullMask, a.cnt, o), __shfl_xor_sync(kFullMask, a.t, o)},
-                scale);
-  return a;
+__device__ __forceinline__ Sums join_warp(const Sums& a, float scale) {
+  Sums r;
+  r.m = warp_max(a.m);
+  const bool top = a.m == r.m;
+  const float d = max_nan(a.m - r.m, kExpFloor);
+  const float f = top ? 1.0f : exp_neg2<T>(both(d), scale).x;
+  const float n = top ? a.s : (a.s + a.cnt) * f;
+  r.s = warp_sum(n);
+  r.cnt = warp_sum(top ? a.cnt : 0.0f);
+  r.t = warp_sum(top ? a.t : fmaf(n, d, f * a.t));
+  return r;
 }
 // As RowStat (t stays relative to the unscaled differences).
 __device__ __forceinline__ RowStat row_stat(const Sums& a) {
@@ -471,12 +539,24 @@ int launch_cluster(void (*kernel)(Params...), unsigned grid, int threads, size_t
   return CIGN_OK;
 }
 
+// Warps of a team.  What a row costs each warp at its ends (the maxima, the
+// sums, the barriers) is as much as about eight rounds of loads, so a team has
+// no more warps than keep the device busy with some rows to spare (48 warps per
+// SM are about two rows per resident team).
+inline int wide_warps(int64_t n, int64_t granules) {
+  const int64_t wanted = static_cast<int64_t>(sm_count()) * 48;
+  int warps = 1;
+  while (warps < 8 && n * warps < wanted && granules >= static_cast<int64_t>(64) * warps)
+    warps = warps == 1 ? 4 : 8;
+  return warps;
+}
+
 // Blocks that share a row of `granules` where there are too few rows to fill
-// the device: as many as leave every thread a full set of loads, at most 8.
+// the device: as many as leave every thread eight loads, at most 8.
 inline int wide_split(int64_t n, int64_t granules, int threads) {
   int split = 1;
   while (split < 8 && n * split * 2 <= 2 * sm_count() &&
-         granules >= static_cast<int64_t>(2) * split * threads * kWideLoads)
+         granules >= static_cast<int64_t>(16) * split * threads)
     split *= 2;
   return split;
 }

@@ -53,113 +53,154 @@ __device__ __forceinline__ void write_row(const LogProbOut& out, int64_t row, co
 
 // Team of W warps per row; with W = 8 a cluster of blocks may share a row.
 constexpr int kLpKept = 128;  // classes that a warp keeps at most before it sorts them out
+constexpr int kLpSlots = 16;  // shares of a thread's part of the row
 template <int W>
 struct alignas(16) WideShared {
   static constexpr int kThreads = 32 * W;
-  uint32_t most[kThreads];  // value keys of maxima
-  uint32_t floor;           // value key that top_k classes at least reach
-  uint32_t next_floor;
-  int count;
-  uint64_t kept[W][kLpKept];
-  uint64_t best[W * kLpMaxTop];
+  static constexpr int kSets = W == 1 ? 128 : kThreads;
+  uint32_t most[kSets];             // value keys of maxima
+  float slot[kLpSlots][kThreads];   // the maximum of each thread's shares
+  alignas(16) uint64_t kept[W][kLpKept];  // a warp's classes that may be among the best, in no order
   uint64_t sorted[kLpMaxTop];
+  int count[W];
+  uint32_t floor;  // value key that top_k classes at least reach
   Sums part[W];
   Sums sums;
 };
+static_assert(offsetof(WideShared<1>, kept) % 16 == 0 && offsetof(WideShared<4>, kept) % 16 == 0 &&
+              offsetof(WideShared<8>, kept) % 16 == 0 && kLpKept % 2 == 0, "read in pairs");
 
-// The classes of one warp that may belong to the best: those that reached the
-// floor when they were met, in no order.
+// Reduces a warp's `count` keys to the best top_k, in order.  A key's place is
+// the number of larger ones.
+__device__ __noinline__ void reduce_kept(uint64_t* list, int count, int top_k) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+  uint64_t k[kLpKept / 32];
+  int place[kLpKept / 32];
+#pragma unroll
+  for (int i = 0; i < kLpKept / 32; ++i) {
+    k[i] = 32 * i + lane < count ? list[32 * i + lane] : 0;
+    place[i] = 0;
+  }
+  for (int j = 0; j < count; ++j) {
+    const uint64_t o = list[j];
+#pragma unroll
+    for (int i = 0; i < kLpKept / 32; ++i) place[i] += o > k[i] ? 1 : 0;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kLpKept / 32; ++i)
+    if (32 * i + lane < count && place[i] < top_k) list[place[i]] = k[i];
+  __syncwarp();
+}
+
+// A warp's classes that may be among the best: keys above `last`.
 struct Kept {
-  int count = 0;
-  // Appends the lanes' keys where `take` is set; more than the warp can keep
-  // are reduced to the best top_k, whose last raises the floor.
-  __device__ __forceinline__ void add(uint64_t key, bool take, uint64_t* list, int top_k,
-                                      uint32_t* floor) {
+  uint64_t* list;
+  uint64_t last;
+  int count;
+  __device__ __forceinline__ void add(uint64_t key, bool valid, int top_k) {
     const int lane = threadIdx.x & 31;
+    const bool take = valid && key > last;
     const unsigned who = __ballot_sync(kFullMask, take);
     if (take) list[count + __popc(who & ((1u << lane) - 1u))] = key;
     count += __popc(who);
-    if (count > kLpKept - 32) reduce(list, top_k, floor);
-  }
-  // A key's place is the number of larger ones (all differ).
-  __device__ __noinline__ void reduce(uint64_t* list, int top_k, uint32_t* floor) {
-    const int lane = threadIdx.x & 31;
-    __syncwarp();
-    uint64_t k[kLpKept / 32];
-    int place[kLpKept / 32];
-#pragma unroll
-    for (int i = 0; i < kLpKept / 32; ++i) {
-      k[i] = 32 * i + lane < count ? list[32 * i + lane] : 0;
-      place[i] = 0;
-    }
-    for (int j = 0; j < count; ++j) {
-      const uint64_t o = list[j];
-#pragma unroll
-      for (int i = 0; i < kLpKept / 32; ++i) place[i] += o > k[i] ? 1 : 0;
-    }
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < kLpKept / 32; ++i)
-      if (32 * i + lane < count && place[i] < top_k) {
-        list[place[i]] = k[i];
-        if (place[i] == top_k - 1) atomicMax(floor, static_cast<uint32_t>(k[i] >> 32));
+    if (count > kLpKept - 32) {
+      reduce_kept(list, count, top_k);
+      if (count >= top_k) {
+        count = top_k;
+        last = list[top_k - 1];
       }
-    __syncwarp();
-    count = count < top_k ? count : top_k;
+    }
   }
 };
 
-// The top_k largest of `count` different keys, sorted, into `sorted`.
+// The top_k largest of the warps' kept keys, sorted.
 template <int W>
 __device__ __forceinline__ void sort_best(WideShared<W>& sh, int count, int top_k, int tid) {
-  for (int i = tid; i < count; i += 32 * W) {
-    const uint64_t k = sh.best[i];
+  const int lane = threadIdx.x & 31, warp = tid >> 5;
+  uint64_t* list = sh.kept[warp];
+  if (lane == 0) {
+    sh.count[warp] = count;
+    if (count % 2 == 1) list[count] = 0;  // read in pairs
+  }
+  team_sync<W>();
+  for (int i = lane; i < count; i += 32) {
+    const uint64_t k = list[i];
     int place = 0;
-    for (int j = 0; j < count; ++j) place += sh.best[j] > k ? 1 : 0;
+    for (int w = 0; w < W; ++w) {
+      const int others = sh.count[w];
+      for (int j = 0; j < others; j += 2) {
+        const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&sh.kept[w][j]);
+        place += (o.x > k ? 1 : 0) + (o.y > k ? 1 : 0);
+      }
+    }
     if (place < top_k) sh.sorted[place] = k;
   }
 }
 
-// Raises the floor of the best classes by the maxima of what the team's threads
-// have seen: the top_k-th largest maximum of disjoint sets of classes is reached
-// by top_k classes.  The sets are those of B threads joined, B at least twice
-// top_k where the team has so many, and the threads of a set share its
-// comparisons.  sh.next_floor is ~0 before and after.
+// The floor of the best classes: the top_k-th largest maximum of disjoint sets
+// of classes is reached by top_k classes.  With B the number of sets, about
+// top_k (1 + top_k / 2 B) classes reach it, so B is at least twice top_k where
+// that is to be had: the sets are those of the threads joined (their threads
+// share the comparisons), or with one warp parts of the threads' sets.
 template <int W>
-__device__ __forceinline__ void raise_floor(WideShared<W>& sh, uint32_t mine, int top_k, int tid) {
+__device__ __forceinline__ void find_floor(WideShared<W>& sh, float most, int slots, int top_k,
+                                           int tid) {
   constexpr int kThreads = 32 * W;
-  if (top_k > kThreads) return;  // fewer maxima than classes asked for
-  int sets = kThreads;
-  while (sets > 32 && sets / 2 >= 2 * top_k) sets /= 2;
-  const int join = kThreads / sets;  // at most 8 neighbouring lanes
-  for (int o = 1; o < join; o <<= 1) mine = max(mine, __shfl_xor_sync(kFullMask, mine, o));
-  if (tid % join == 0) sh.most[tid / join] = mine;
-  team_sync<W>();
-  const int share = sets / join;
-  int above = 0;
-  for (int j = tid % join * share; j < (tid % join + 1) * share; j += 4) {
-    const uint4 o = *reinterpret_cast<const uint4*>(sh.most + j);
-    above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
-  }
-  for (int o = 1; o < join; o <<= 1) above += __shfl_xor_sync(kFullMask, above, o);
-  if (above < top_k && tid % join == 0) atomicMin(&sh.next_floor, mine);
-  team_sync<W>();
-  if (tid == 0) {
-    atomicMax(&sh.floor, sh.next_floor);
-    sh.next_floor = 0xffffffffu;
+  if (W > 1 || top_k <= 16) {
+    uint32_t mine = value_key(most);
+    int sets = kThreads;
+    while (sets > 32 && sets / 2 >= 2 * top_k) sets /= 2;
+    const int join = kThreads / sets;  // at most 8 neighbouring lanes
+    for (int o = 1; o < join; o <<= 1) mine = max(mine, __shfl_xor_sync(kFullMask, mine, o));
+    if (tid % join == 0) sh.most[tid / join] = mine;
+    team_sync<W>();
+    const int share = sets / join;
+    int above = 0;
+    for (int j = tid % join * share; j < (tid % join + 1) * share; j += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(sh.most + j);
+      above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+    }
+    for (int o = 1; o < join; o <<= 1) above += __shfl_xor_sync(kFullMask, above, o);
+    if (above < top_k && tid % join == 0) atomicMin(&sh.floor, mine);
+  } else {
+    constexpr int kParts = WideShared<W>::kSets / kThreads;
+    uint32_t mine[kParts];
+    int above[kParts];
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) {
+      float m = -INFINITY;
+      for (int i = p; i < slots; i += kParts) m = max_nan(m, sh.slot[i][tid]);
+      mine[p] = value_key(m);
+      above[p] = 0;
+      sh.most[p * kThreads + tid] = mine[p];
+    }
+    team_sync<W>();
+    for (int j = 0; j < WideShared<W>::kSets; j += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(sh.most + j);
+#pragma unroll
+      for (int p = 0; p < kParts; ++p)
+        above[p] += (o.x > mine[p]) + (o.y > mine[p]) + (o.z > mine[p]) + (o.w > mine[p]);
+    }
+#pragma unroll
+    for (int p = 0; p < kParts; ++p)
+      if (above[p] < top_k) atomicMin(&sh.floor, mine[p]);
   }
   team_sync<W>();
 }
 
 // One pass over the row.  The first loads of all threads give the team's
-// maximum, from which the sums start, and the floor of the best classes; only
-// what reaches the floor is looked at again.
+// maximum, from which the sums start.  A thread also notes the maxima of up to
+// 16 shares of what it reads; after the pass these give a floor for the best
+// classes, and only the few shares that reach it are read again.
 template <typename T, int W, bool TOP>
 __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 8 ? 3 : 6)
 log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld,
                           const int64_t* __restrict__ labels, int top_k, int split,
                           LogProbOut out) {
   constexpr int V = RowFrame<T>::V;
+  constexpr int L = kWideLoads<T>;
   constexpr int kTeams = W == 1 ? 4 : 1;
   constexpr int kThreads = 32 * W;
   __shared__ WideShared<W> all[kTeams];
@@ -172,107 +213,91 @@ log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
   if (row >= n) return;  // a whole team
   const T* x = logits + row * ld;
   const RowFrame<T> frame(x, c, rank, W == 8 ? split : 1);
-  const int64_t rounds = frame.rounds(kThreads);
+  const int rounds = frame.template rounds<L>(kThreads);
 
-  Pack<T, V> q[kWideLoads], next[kWideLoads];
+  Pack<T, V> q[L], next[L];
   F2 v[V / 2];
   frame.load(q, 0, tid, kThreads, -INFINITY);
   // the two ends of the row, by the first two threads
-  const int64_t edge = tid == 0 ? frame.head : tid == 1 ? frame.tail : -1;
+  const int edge = tid == 0 ? frame.head : tid == 1 ? frame.tail : -1;
   const Pack<T, V> ends = frame.edge(edge, -INFINITY);
   float most = -INFINITY;
 #pragma unroll
-  for (int u = 0; u < kWideLoads; ++u) {
+  for (int u = 0; u < L; ++u) {
     unpack(q[u], v);
     most = max_nan(most, max_of(v));
   }
   unpack(ends, v);
-  most = max_nan(most, max_of(v));
+  const float ends_top = max_of(v);
+  most = max_nan(most, ends_top);
   float start = warp_max(most);  // skips NaN
   if (start != start) start = -INFINITY;
-  if (W > 1 && lane == 0) sh.part[tid >> 5].m = start;
-  if (tid == 0) {
-    sh.floor = 0;
-    sh.next_floor = 0xffffffffu;
-    sh.count = 0;
-  }
-  team_sync<W>();
+  if (TOP && tid == 0) sh.floor = 0xffffffffu;
   if (W > 1) {
+    if (lane == 0) sh.part[tid >> 5].m = start;
+    __syncthreads();
 #pragma unroll
     for (int w = 0; w < W; ++w) start = fmaxf(start, sh.part[w].m);
   }
-  if (TOP) raise_floor<W>(sh, value_key(most), top_k, tid);
 
-  Stream<T, true> sums(start);
-  Kept kept;
-  // The lanes' granules g (-1: none), whose largest classes are `top`: keep what
-  // reaches the floor.  Few granules do; V lanes read each again.
-  const auto look = [&](int64_t g, float top, float floor) {
-    unsigned who = __ballot_sync(kFullMask, !(top < floor) && g >= 0);
-    while (who) {
-      const int64_t f = __shfl_sync(kFullMask, g, __ffs(who) - 1) * V + lane;
-      who &= who - 1;
-      const bool in = lane < V && f >= frame.shift && f < frame.end;
-      const float xe = in ? to_f(frame.base[f]) : 0.0f;
-      kept.add(class_key(xe, static_cast<uint32_t>(f - frame.shift)), in && !(xe < floor),
-               sh.kept[tid >> 5], top_k, &sh.floor);
-    }
-  };
-  {
-    const float top = max_of(v);
-    sums.add(v, top, kLog2e);
-    if (TOP && tid < 32) look(edge, top, key_value(*const_cast<volatile uint32_t*>(&sh.floor)));
-  }
-  for (int64_t k = 0; k < rounds; ++k) {
+  Stream<T, true> sums(start, kLog2e);
+  sums.add(v, ends_top, kLog2e);
+  const int per_slot = (rounds + kLpSlots - 1) / kLpSlots;  // rounds of a share
+  float share = -INFINITY;
+  int slots = 0, rest = per_slot;
+#pragma unroll 1
+  for (int k = 0; k < rounds; ++k) {
     if (k + 1 < rounds) frame.load(next, k + 1, tid, kThreads, -INFINITY);
-    const float floor = TOP ? key_value(*const_cast<volatile uint32_t*>(&sh.floor)) : 0.0f;
 #pragma unroll
-    for (int u = 0; u < kWideLoads; ++u) {
+    for (int u = 0; u < L; ++u) {
       unpack(q[u], v);
       const float top = max_of(v);
       sums.add(v, top, kLog2e);
-      if (TOP) {
-        const int64_t g = frame.granule(k, u, tid, kThreads);
-        look(g < frame.g1 ? g : -1, top, floor);
-        most = max_nan(most, top);
-      }
+      if (TOP) share = max_nan(share, top);
       q[u] = next[u];
     }
-    // after 2, 4, 8, ... rounds: each raise halves what the coming rounds keep
-    if (TOP && k > 0 && (k & (k + 1)) == 0 && k + 1 < rounds)
-      raise_floor<W>(sh, value_key(most), top_k, tid);
+    if (TOP && (--rest == 0 || k + 1 == rounds)) {
+      sh.slot[slots++][tid] = share;
+      most = max_nan(most, share);
+      share = -INFINITY;
+      rest = per_slot;
+    }
   }
 
-  Sums a{sums.m, sums.s.x + sums.s.y, sums.cnt, sums.t.x + sums.t.y};
+  Sums a{sums.m, sums.total_s(kLog2e), sums.cnt, sums.total_t(kLog2e)};
   a = join_warp<T>(a, kLog2e);
   if (W > 1) {
     __syncthreads();  // part was read above
     if (lane == 0) sh.part[tid >> 5] = a;
+    __syncthreads();
+    // the first warp goes on with the sums
+    if (tid < 32)
+      a = join_warp<T>(lane < W ? sh.part[lane] : Sums{-INFINITY, 0.0f, 0.0f, 0.0f}, kLog2e);
   }
   if (TOP) {
-    if (kept.count > kLpMaxTop) kept.reduce(sh.kept[tid >> 5], top_k, &sh.floor);
-    if (tid < kLpMaxTop) sh.sorted[tid] = 0;
-    for (int i = tid + kThreads; i < kLpMaxTop; i += kThreads) sh.sorted[i] = 0;
-  }
-  team_sync<W>();
-  if (W > 1) {
-    a = sh.part[0];
-#pragma unroll
-    for (int w = 1; w < W; ++w) a = join<T>(a, sh.part[w], kLog2e);
-  }
-  if (TOP) {
-    const uint32_t floor = *const_cast<volatile uint32_t*>(&sh.floor);
-    for (int i = lane; i - lane < kept.count; i += 32) {
-      const uint64_t k = i < kept.count ? sh.kept[tid >> 5][i] : 0;
-      const bool keep = i < kept.count && static_cast<uint32_t>(k >> 32) >= floor;
-      const unsigned who = __ballot_sync(kFullMask, keep);
-      int at = 0;
-      if (lane == 0 && who) at = atomicAdd(&sh.count, __popc(who));
-      at = __shfl_sync(kFullMask, at, 0) + __popc(who & ((1u << lane) - 1u));
-      if (keep) sh.best[at] = k;
+    find_floor<W>(sh, most, slots, top_k, tid);
+    const uint32_t floor_key = *const_cast<volatile uint32_t*>(&sh.floor);
+    const float floor = key_value(floor_key);
+    Kept kept{sh.kept[tid >> 5], floor_key ? (static_cast<uint64_t>(floor_key) << 32) - 1 : 0, 0};
+    if (tid < 32) {  // the ends
+      const int f = (lane < V ? frame.head : frame.tail) * V + lane % V;
+      const bool in = lane < 2 * V && f >= 0 && frame.inside(f);
+      kept.add(in ? class_key(to_f(frame.base[f]), f - frame.shift) : 0, in, top_k);
     }
-    team_sync<W>();
-    sort_best<W>(sh, sh.count, top_k, tid);
+    for (int i = 0; i < slots; ++i) {
+      unsigned who = __ballot_sync(kFullMask, !(sh.slot[i][tid] < floor));
+      while (who) {
+        const int from = (tid & ~31) + __ffs(who) - 1;
+        who &= who - 1;
+        for (int k = i * per_slot; k < (i + 1) * per_slot && k < rounds; ++k) {
+          const int g = frame.g0 + from + kThreads * (k * L + lane / V);
+          const bool in = lane < L * V && g < frame.g1;
+          const int f = g * V + lane % V;
+          kept.add(in ? class_key(to_f(frame.base[f]), f - frame.shift) : 0, in, top_k);
+        }
+      }
+    }
+    sort_best<W>(sh, kept.count, top_k, tid);
   }
   if (W == 8 && split > 1) {
     namespace cg = cooperative_groups;
@@ -280,17 +305,16 @@ log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
     if (tid == 0) sh.sums = a;
     cluster.sync();
     if (rank == 0) {
-      for (int r = 1; r < split; ++r)
-        a = join<T>(a, cluster.map_shared_rank(&sh, r)->sums, kLog2e);
-      if (TOP) {
-        const int count = split * top_k;
-        const uint64_t own = tid < top_k ? sh.sorted[tid] : 0;
+      if (tid < 32)
+        a = join_warp<T>(lane < split ? cluster.map_shared_rank(&sh, lane)->sums
+                                      : Sums{-INFINITY, 0.0f, 0.0f, 0.0f}, kLog2e);
+      if (TOP) {  // warp r takes what block r found
+        const int r = tid >> 5;
         __syncthreads();
-        if (tid < top_k) sh.best[tid] = own;
-        for (int i = tid + top_k; i < count; i += kThreads)
-          sh.best[i] = cluster.map_shared_rank(&sh, i / top_k)->sorted[i % top_k];
+        for (int i = lane; i < top_k && r < split; i += 32)
+          sh.kept[r][i] = cluster.map_shared_rank(&sh, r)->sorted[i];
         __syncthreads();
-        sort_best<W>(sh, count, top_k, tid);
+        sort_best<W>(sh, r < split ? top_k : 0, top_k, tid);
       }
     }
     cluster.sync();  // the others' shared memory is read above
@@ -302,13 +326,13 @@ log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
     write_row(out, row, st, y, y >= 0 && y < c ? to_f(x[y]) : 0.0f, c);
   }
   if (TOP) {
+    if (tid == 0) sh.sums = Sums{st.m, stat_log(st), 0.0f, 0.0f};
     team_sync<W>();
-    const float logs = stat_log(st);
     for (int i = tid; i < top_k; i += kThreads) {
       const uint64_t k = sh.sorted[i];
       out.top_index[row * top_k + i] = key_index(k);
       out.top_log_probs[row * top_k + i] =
-          log_prob_of(key_value(static_cast<uint32_t>(k >> 32)), st.m, logs);
+          log_prob_of(key_value(static_cast<uint32_t>(k >> 32)), sh.sums.m, sh.sums.s);
     }
   }
 }
@@ -535,8 +559,8 @@ int lp_check(int64_t n, int64_t c, int32_t x_type, int64_t ld, int32_t top_k, co
                "%s: top_k must be between 0 and the class count", name);
   CIGN_REQUIRE(top_k <= kLpMaxTop, CIGN_ERR_UNSUPPORTED, "%s: top_k is at most %d", name,
                kLpMaxTop);
-  CIGN_REQUIRE(n < (1ll << 31) && c < (1ll << 31), CIGN_ERR_UNSUPPORTED,
-               "%s: at most 2^31 - 1 rows and classes", name);
+  CIGN_REQUIRE(n < (1ll << 31) && c <= kWideMax, CIGN_ERR_UNSUPPORTED,
+               "%s: at most 2^31 - 1 rows of at most 2^31 - 16 classes", name);
   return CIGN_OK;
 }
 
@@ -568,19 +592,17 @@ int cign_node_log_probs_fwd(int64_t n, int64_t c, int32_t x_type, const void* lo
     CIGN_CHECK_LAUNCH("log_probs_narrow_fwd_kernel");
     return CIGN_OK;
   }
-  // warps of a row by its length: one warp does a row of a few loads per lane
-  // without barriers; eight, and eight blocks where rows are few, a long one
   const int64_t granules = c * type_size(x_type) / 16;
   CIGN_TYPE_DISPATCH(x_type, T, {
     const T* x = static_cast<const T*>(logits);
-    if (granules <= 2 * 128 * kWideLoads) {
-      const bool one = granules <= 2 * 32 * kWideLoads;
-      const auto kernel = one ? (top_k ? log_probs_wide_fwd_kernel<T, 1, true>
-                                       : log_probs_wide_fwd_kernel<T, 1, false>)
-                              : (top_k ? log_probs_wide_fwd_kernel<T, 4, true>
-                                       : log_probs_wide_fwd_kernel<T, 4, false>);
-      kernel<<<static_cast<unsigned>(one ? (n + 3) / 4 : n), 128, 0, s>>>(n, c, x, ld, labels,
-                                                                         top_k, 1, out);
+    const int warps = wide_warps(n, granules);
+    if (warps < 8) {
+      const auto kernel = warps == 1 ? (top_k ? log_probs_wide_fwd_kernel<T, 1, true>
+                                              : log_probs_wide_fwd_kernel<T, 1, false>)
+                                     : (top_k ? log_probs_wide_fwd_kernel<T, 4, true>
+                                              : log_probs_wide_fwd_kernel<T, 4, false>);
+      kernel<<<static_cast<unsigned>(warps == 1 ? (n + 3) / 4 : n), 128, 0, s>>>(
+          n, c, x, ld, labels, top_k, 1, out);
     } else {
       const int split = wide_split(n, granules, 256);
       return launch_cluster(top_k ? log_probs_wide_fwd_kernel<T, 8, true>
