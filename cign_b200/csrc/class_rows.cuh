@@ -374,6 +374,16 @@ __device__ __forceinline__ void unpack(const Pack<T, V>& q, F2 (&v)[V / 2]) {
 #pragma unroll
   for (int i = 0; i < V / 2; ++i) v[i] = F2{to_f(q.e[2 * i]), to_f(q.e[2 * i + 1])};
 }
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, 2 * N> pack_of(const F2 (&v)[N]) {
+  Pack<T, 2 * N> q;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    q.e[2 * i] = from_f<T>(v[i].x);
+    q.e[2 * i + 1] = from_f<T>(v[i].y);
+  }
+  return q;
+}
 template <int N>
 __device__ __forceinline__ float max_of(const F2 (&v)[N]) {
   float m = max_nan(v[0].x, v[0].y);
@@ -388,6 +398,101 @@ __device__ __forceinline__ float min_of(const F2 (&v)[N]) {
   for (int i = 1; i < N; ++i) m = min3_nan(m, v[i].x, v[i].y);
   return m;
 }
+
+// One warp's share of a row, the rank-th of `split`, taken through f (which
+// changes pairs of values in place) from x to out, both of c elements.  Whole
+// granules where x and out start at the same place within 16 bytes; elements
+// otherwise.
+template <typename T>
+struct RowShare {
+  static constexpr int V = RowFrame<T>::V;
+  static constexpr int L = kWideLoads<T>;
+  RowFrame<T> frame;
+  T* out;
+  int first, last;  // elements [first, last) of the row
+  __device__ __forceinline__ RowShare(const T* x, T* out, int64_t c, int rank, int split)
+      : frame(x, c, rank, split), out(out) {
+    first = (frame.head >= 0 ? frame.shift : frame.g0 * V) - frame.shift;
+    last = (frame.tail >= 0 ? frame.end : frame.g1 * V) - frame.shift;
+  }
+  __device__ __forceinline__ bool holds(int64_t j) const { return j >= first && j < last; }
+  template <bool READ, typename F>
+  __device__ __forceinline__ void run(F&& f) const {
+    const int lane = threadIdx.x & 31;
+    const T* x = frame.base + frame.shift;
+    if ((reinterpret_cast<uintptr_t>(x) - reinterpret_cast<uintptr_t>(out)) % 16 == 0) {
+      T* o = out - frame.shift;
+      const int edge = lane == 0 ? frame.head : lane == 1 ? frame.tail : -1;
+      F2 v[V / 2];
+      if (edge >= 0) {
+        if (READ) unpack(frame.edge(edge, 0.0f), v);
+        f(v);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (frame.inside(edge * V + e))
+            o[edge * V + e] = from_f<T>(e % 2 == 0 ? v[e / 2].x : v[e / 2].y);
+      }
+      const int rounds = frame.template rounds<L>(32);
+      Pack<T, V> q[L];
+      for (int k = 0; k < rounds; ++k) {
+        if (READ) frame.load(q, k, lane, 32, 0.0f);
+#pragma unroll
+        for (int u = 0; u < L; ++u) {
+          const int g = frame.g0 + lane + 32 * (k * L + u);
+          if (READ) unpack(q[u], v);
+          f(v);
+          if (g < frame.g1) store_pack<T, V>(o + static_cast<int64_t>(g) * V, pack_of<T>(v));
+        }
+      }
+    } else {
+      for (int j = first + lane; j - lane < last; j += 32 * 8) {
+        F2 v[4];
+        if (READ) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            v[i].x = j + 64 * i < last ? to_f(x[j + 64 * i]) : 0.0f;
+            v[i].y = j + 64 * i + 32 < last ? to_f(x[j + 64 * i + 32]) : 0.0f;
+          }
+        }
+        f(v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (j + 64 * i < last) out[j + 64 * i] = from_f<T>(v[i].x);
+          if (j + 64 * i + 32 < last) out[j + 64 * i + 32] = from_f<T>(v[i].y);
+        }
+      }
+    }
+  }
+};
+
+// The grid of a kernel that takes rows through warps: a block of 8 warps has
+// 8 / `split` rows, or one row (with blockIdx.y its next 8 shares).
+constexpr int kMapThreads = 256;
+struct MapGrid {
+  int split, warps;  // shares of a row; warps of a block for one row: 1, 2, 4 or 8
+  dim3 grid;
+};
+inline MapGrid map_grid(int64_t n, int64_t granules) {
+  MapGrid m;
+  // 16 granules per lane amortise what every share reads of its row (more where
+  // the grid's second dimension would not hold the shares)
+  const int64_t share = granules > 512ll * 8 * 65535 ? granules / (8 * 65535) + 1 : 512;
+  m.split = static_cast<int>((granules + share - 1) / share);
+  m.warps = 1;
+  while (m.warps < 8 && m.warps < m.split) m.warps *= 2;
+  m.grid = dim3(static_cast<unsigned>((n * m.warps + 7) / 8),
+                static_cast<unsigned>((m.split + m.warps - 1) / m.warps));
+  return m;
+}
+struct MapPlace {
+  int64_t row;
+  int rank;
+  __device__ __forceinline__ explicit MapPlace(int warps) {
+    const int w = threadIdx.x >> 5;
+    row = static_cast<int64_t>(blockIdx.x) * (8 / warps) + w / warps;
+    rank = blockIdx.y * warps + w % warps;
+  }
+};
 
 template <int W>
 __device__ __forceinline__ void team_sync() {

@@ -14,29 +14,16 @@
 // because sum over kept p + p_rest = 1, and an error of the row's log sum
 // cancels in first order.  W p_j - q_j is q_j (expm1(-d_j) + (W - 1) e^-d_j).
 // d and r are formed in 64 bits from the float32 values.
+#include <cooperative_groups.h>
+
 #include "class_rows.cuh"
 
 namespace cign {
 namespace {
 
-constexpr int kDsThreads = 256;
-constexpr int kDsWarps = kDsThreads / 32;
 constexpr int kDsMaxKept = 256;
 constexpr int kDsStats = 8;
 constexpr int64_t kDsMaxClasses = 1 << 20;  // one bit each in shared memory
-
-template <int WARPS>
-__device__ __forceinline__ double block_sum_f64(double v, double* part) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-  __syncthreads();
-  double s = 0.0;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) s += part[w];
-  return s;
-}
 
 struct Teacher {
   const void* values;
@@ -69,38 +56,6 @@ __device__ __forceinline__ float scaled(float d, const InvT& it) {
   return fmaf(d, it.hi, d == -INFINITY ? 0.0f : d * it.lo);
 }
 
-// Running sum of e^((x - m) / T) - 1, as RowStat without t.
-__device__ __forceinline__ void stat_add_t(RowStat& a, float x, const InvT& it) {
-  if (x > a.m) {
-    a.s = (1.0f + a.s) * expf(scaled(a.m - x, it));
-    a.m = x;
-  } else if (x == a.m) {
-    a.s += 1.0f;
-  } else {
-    a.s += expf(scaled(x - a.m, it));
-  }
-}
-__device__ __forceinline__ RowStat stat_merge_t(const RowStat& a, const RowStat& b,
-                                                const InvT& it) {
-  const bool ge = a.m >= b.m;
-  const RowStat hi = ge ? a : b, lo = ge ? b : a;
-  RowStat r;
-  r.m = hi.m;
-  r.s = hi.s + (1.0f + lo.s) * (a.m == b.m ? 1.0f : expf(scaled(lo.m - hi.m, it)));
-  return r;
-}
-__device__ __forceinline__ RowStat block_stat_t(RowStat a, RowStat* part, const InvT& it) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) a = stat_merge_t(a, stat_shfl_xor(a, o), it);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
-  __syncthreads();
-  a = part[0];
-#pragma unroll
-  for (int w = 1; w < kDsWarps; ++w) a = stat_merge_t(a, part[w], it);
-  return a;
-}
-
 // q (e^-d - 1 + d), which is not negative; by its series where d is small.
 __device__ __forceinline__ float divergence_term(float q, float d) {
   if (fabsf(d) < 0.125f) {
@@ -111,16 +66,18 @@ __device__ __forceinline__ float divergence_term(float q, float d) {
   return q * (expm1f(-d) + d);
 }
 
-// What the forward keeps of a row for the backward.
+// What the forward keeps of a row for the backward.  Outside the kept classes
+// the gradient is T g p_j (W - r / p_rest) = T g spread e^(log p_j + lift): lift
+// is 0 but where p_rest is too small to divide by.
 struct DistillRow {
   float m;       // maximum of the logits
   float logs;    // log sum e^((x - m) / T)
-  float spread;  // W - r / p_rest: the factor of p outside the kept classes
+  float spread;
   float w1;      // W - 1
   float tmax;    // tail "drop": maximum and log sum of the teacher's values
   float tlog;
-  float dup;     // 1 where a class is kept twice
-  float none;    // 1 where the row has no kept class
+  float lift;
+  float kind;    // 0; 1: a class is kept twice; 2: the row has no kept class
 };
 
 __device__ __forceinline__ double log_q(float v, const DistillRow& r, bool bucket,
@@ -134,7 +91,7 @@ __device__ __forceinline__ float kept_gradient(const Teacher& te, int64_t row, i
                                                int64_t idx, float v, double lp,
                                                const DistillRow& r, bool bucket, const InvT& it) {
   const double lq = log_q(v, r, bucket, it);
-  if (r.dup == 0.0f) {
+  if (r.kind == 0.0f) {
     const float d = static_cast<float>(lq - lp);
     return expf(static_cast<float>(lq)) *
            (expm1f(-d) + (r.w1 != 0.0f ? r.w1 * expf(-d) : 0.0f));
@@ -154,143 +111,294 @@ __device__ __forceinline__ DistillRow load_row(const float* stats) {
   return DistillRow{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 }
 
-// The row's loss and statistics from the sum over its entries.
-__device__ __forceinline__ void finish_row(DistillRow r, float sum, float mass_r, float p_rest,
+// The row's loss and statistics from the sum over its entries; log_rest is
+// log p_rest.
+__device__ __forceinline__ void finish_row(DistillRow r, float sum, float mass_r, float log_rest,
                                            bool none, bool bad, bool dup, float temperature,
                                            float* loss, float* stats) {
-  if (mass_r != 0.0f)
-    sum += p_rest > 0.0f ? divergence_term(mass_r, logf(mass_r) - logf(p_rest)) : INFINITY;
-  else
-    sum += p_rest;
+  const float w = 1.0f + r.w1;
+  r.spread = w;
+  r.lift = 0.0f;
+  if (mass_r != 0.0f) {
+    const float d = logf(mass_r) - log_rest;
+    sum += divergence_term(mass_r, d);
+    if (d < 40.0f) {
+      r.spread = w - expf(d);
+    } else if (log_rest > -INFINITY) {
+      r.spread = w * expf(-d) - 1.0f;
+      r.lift = d;
+    }
+  } else {
+    sum += expf(log_rest);
+  }
   float l = temperature * temperature * (sum + r.w1);
-  r.spread = (1.0f + r.w1) - (mass_r != 0.0f && p_rest > 0.0f ? mass_r / p_rest : 0.0f);
-  r.dup = dup ? 1.0f : 0.0f;
-  r.none = none ? 1.0f : 0.0f;
   if (r.m == -INFINITY && r.logs == r.logs) l = INFINITY;  // the student has no class left
   if (none) l = 0.0f;
-  if (bad) {
-    l = r.logs = r.spread = __int_as_float(0x7fffffff);
-    r.none = 0.0f;
-  }
+  if (bad) l = r.logs = r.spread = __int_as_float(0x7fffffff);
+  r.kind = none && !bad ? 2.0f : dup ? 1.0f : 0.0f;
   *loss = l;
   if (stats) {
     reinterpret_cast<float4*>(stats)[0] = make_float4(r.m, r.logs, r.spread, r.w1);
-    reinterpret_cast<float4*>(stats)[1] = make_float4(r.tmax, r.tlog, r.dup, r.none);
+    reinterpret_cast<float4*>(stats)[1] = make_float4(r.tmax, r.tlog, r.lift, r.kind);
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kDsThreads)
-distill_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld, Teacher te,
-                   float temperature, InvT it, int bucket, float* __restrict__ loss,
-                   float* __restrict__ stats) {
-  extern __shared__ uint32_t kept_bits[];
-  __shared__ RowStat part[kDsWarps];
-  __shared__ float fpart[kDsWarps];
-  __shared__ double dpart[kDsWarps];
-  __shared__ int64_t kidx[kDsMaxKept];
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x;
+// What tail "bucket" leaves to the other classes (r) and W - 1, from the
+// teacher's summed probabilities; no class is left to take it where all are kept.
+__device__ __forceinline__ float rest_mass(double mass, bool all_kept, float& w1) {
+  // a small difference where the teacher is sure of its kept classes
+  const float raw = static_cast<float>(1.0 - mass);
+  w1 = 0.0f;
+  if (all_kept || raw < 0.0f) w1 = -raw;
+  return all_kept || raw < 0.0f ? 0.0f : raw;
+}
+
+// Rows of more than kNarrowMax classes: a team of W warps per row, with W = 8 a
+// cluster of blocks where rows are few.  The kept classes are bits in shared
+// memory, at their places in the row's frame, so that a thread finds those of
+// its 16 bytes in one byte or half of one.
+template <int W>
+struct alignas(16) DistillShared {
+  int64_t index[kDsMaxKept];  // -1: absent
+  float value[kDsMaxKept];
+  float x[kDsMaxKept];
+  Sums part[W];
+  Sums sums;
+  int bad, dup, distinct;
+};
+
+template <typename T, int W>
+__global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 8 ? 3 : 6)
+distill_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld, Teacher te,
+                        float temperature, InvT it, int bucket, int split, int words,
+                        float* __restrict__ loss, float* __restrict__ stats) {
+  constexpr int V = RowFrame<T>::V;
+  constexpr int L = kWideLoads<T>;
+  constexpr int kTeams = W == 1 ? 4 : 1;
+  constexpr int kThreads = 32 * W;
+  extern __shared__ uint32_t all_bits[];
+  __shared__ DistillShared<W> all[kTeams];
+  const int team = W == 1 ? threadIdx.x >> 5 : 0;
+  const int tid = W == 1 ? threadIdx.x & 31 : threadIdx.x;
+  const int lane = threadIdx.x & 31;
+  DistillShared<W>& sh = all[team];
+  uint32_t* bits = all_bits + team * words;
+  const int rank = W == 8 ? blockIdx.x % split : 0;
+  const int64_t row = W == 8 ? blockIdx.x / split : static_cast<int64_t>(blockIdx.x) * kTeams + team;
+  if (row >= n) return;  // a whole team
   const T* x = logits + row * ld;
-  for (int64_t i = tid; i < (c + 31) / 32; i += kDsThreads) kept_bits[i] = 0;
-  // the teacher's entries, one per thread
-  int64_t idx = -1;
-  float v = -INFINITY;
-  if (tid < te.k) {
-    idx = teacher_index(te, row, tid);
-    v = teacher_value(te, row, tid);
-    if (v == -INFINITY) idx = -1;
-    kidx[tid] = idx;
-  }
-  const bool bad = idx >= c;
-  const bool valid = idx >= 0 && !bad;
-  __syncthreads();
-  bool first = false;
-  if (valid) first = !((atomicOr(&kept_bits[idx >> 5], 1u << (idx & 31)) >> (idx & 31)) & 1u);
-  const int any_bad = __syncthreads_or(bad);
-  const int any_dup = __syncthreads_or(valid && !first);
-  const int distinct = __syncthreads_count(first);
-  if (any_dup) {  // the first of equal entries by its place, not by the race above
-    first = valid;
-    for (int i = 0; i < tid && first; ++i) first = kidx[i] != idx;
-  }
-  // student: classes that are not kept, then kept ones
-  RowStat rest;
-  for (int64_t j = tid; j < c; j += kDsThreads)
-    if (!((kept_bits[j >> 5] >> (j & 31)) & 1u)) stat_add_t(rest, to_f(x[j]), it);
-  rest = block_stat_t(rest, part, it);
-  RowStat all;
-  const float xi = valid ? to_f(x[idx]) : 0.0f;
-  if (first) stat_add_t(all, xi, it);
-  all = stat_merge_t(block_stat_t(all, part, it), rest, it);
-  DistillRow r;
-  r.m = all.m;
-  r.logs = all.m == INFINITY ? __int_as_float(0x7fffffff) : log1pf(all.s);
-  const float p_rest = (1.0f + rest.s) *
-                       (rest.m == all.m ? 1.0f : expf(scaled(rest.m - all.m, it))) /
-                       (1.0f + all.s);
-  // teacher
-  RowStat ts;
-  if (valid) stat_add_t(ts, v, it);
-  ts = block_stat_t(ts, part, it);
-  r.tmax = ts.m;
-  r.tlog = log1pf(ts.s);
-  const float lq = valid ? static_cast<float>(log_q(v, r, bucket, it)) : -INFINITY;
-  const float q = expf(lq);
-  float mass_r = 0.0f;
-  r.w1 = 0.0f;
-  if (bucket) {
-    // a small difference where the teacher is sure of its kept classes: 64 bits
-    const float raw = static_cast<float>(
-        1.0 - block_sum_f64<kDsWarps>(valid ? exp(static_cast<double>(v)) : 0.0, dpart));
-    if (raw == raw && raw < 0.0f) r.w1 = -raw;
-    else mass_r = raw;
-    if (distinct == c) {  // no class is left to take the rest
-      r.w1 = -raw;
-      mass_r = 0.0f;
+  const RowFrame<T> frame(x, c, rank, W == 8 ? split : 1);
+  const int rounds = frame.template rounds<L>(kThreads);
+  const float scale = kLog2e * it.hi;
+
+  Pack<T, V> q[L], next[L];
+  frame.load(q, 0, tid, kThreads, -INFINITY);
+  for (int i = tid; i < words; i += kThreads) bits[i] = 0;
+  if (tid == 0) sh.bad = sh.dup = sh.distinct = 0;
+  team_sync<W>();
+  for (int e = tid; e < te.k; e += kThreads) {
+    int64_t idx = teacher_index(te, row, e);
+    const float v = teacher_value(te, row, e);
+    if (idx < 0 || v == -INFINITY) idx = -1;
+    if (idx >= c) {
+      atomicOr(&sh.bad, 1);
+      idx = -1;
+    }
+    sh.index[e] = idx;
+    sh.value[e] = v;
+    if (idx >= 0) {
+      const int f = static_cast<int>(idx) + frame.shift;
+      const uint32_t bit = 1u << (f & 31);
+      if (atomicOr(bits + (f >> 5), bit) & bit) atomicOr(&sh.dup, 1);
+      else atomicAdd(&sh.distinct, 1);
+      sh.x[e] = to_f(x[idx]);
     }
   }
-  float term = 0.0f;
-  if (valid) {
-    const double lp = (static_cast<double>(xi) - all.m) * it.full - static_cast<double>(r.logs);
-    const float d = static_cast<float>(log_q(v, r, bucket, it) - lp);
-    term = first ? divergence_term(q, d) : q * (d - 1.0f);
+  team_sync<W>();
+  // the values of a granule that is not whole or of a whole one, kept classes as -inf
+  F2 v[V / 2];
+  const auto drop_kept = [&](int g) {
+    const uint32_t mine = (bits[(g * V) >> 5] >> ((g * V) & 31)) & ((1u << V) - 1u);
+    if (mine != 0) {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        if ((mine >> (2 * i)) & 1u) v[i].x = -INFINITY;
+        if ((mine >> (2 * i + 1)) & 1u) v[i].y = -INFINITY;
+      }
+    }
+  };
+  const int edge = tid == 0 ? frame.head : tid == 1 ? frame.tail : -1;
+  const Pack<T, V> ends = frame.edge(edge, -INFINITY);
+  float most = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < L; ++u) {
+    const int g = frame.g0 + tid + kThreads * u;
+    unpack(q[u], v);
+    if (g < frame.g1) drop_kept(g);
+    most = max_nan(most, max_of(v));
   }
-  const float sum = block_sum<kDsWarps>(term, fpart);
-  if (tid == 0)
-    finish_row(r, sum, mass_r, p_rest, distinct == 0, any_bad, any_dup, temperature, loss + row,
-               stats ? stats + row * kDsStats : nullptr);
+  unpack(ends, v);
+  if (edge >= 0) drop_kept(edge);
+  const float ends_top = max_of(v);
+  float start = warp_max(max_nan(most, ends_top));  // skips NaN
+  if (start != start) start = -INFINITY;
+  if (W > 1) {
+    if (lane == 0) sh.part[tid >> 5].m = start;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) start = fmaxf(start, sh.part[w].m);
+  }
+  Stream<T, false> sums(start, scale);
+  sums.add(v, ends_top, scale);
+#pragma unroll 1
+  for (int k = 0; k < rounds; ++k) {
+    if (k + 1 < rounds) frame.load(next, k + 1, tid, kThreads, -INFINITY);
+#pragma unroll
+    for (int u = 0; u < L; ++u) {
+      const int g = frame.g0 + tid + kThreads * (k * L + u);
+      unpack(q[u], v);
+      if (g < frame.g1) drop_kept(g);
+      sums.add(v, max_of(v), scale);
+      q[u] = next[u];
+    }
+  }
+  Sums rest{sums.m, sums.total_s(scale), sums.cnt, 0.0f};
+  rest = join_warp<T>(rest, scale);
+  if (W > 1) {
+    __syncthreads();  // part was read above
+    if (lane == 0) sh.part[tid >> 5] = rest;
+    __syncthreads();
+    if (tid < 32)
+      rest = join_warp<T>(lane < W ? sh.part[lane] : Sums{-INFINITY, 0.0f, 0.0f, 0.0f}, scale);
+  }
+  if (W == 8 && split > 1) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    if (tid == 0) sh.sums = rest;
+    cluster.sync();
+    if (rank == 0 && tid < 32)
+      rest = join_warp<T>(lane < split ? cluster.map_shared_rank(&sh, lane)->sums
+                                       : Sums{-INFINITY, 0.0f, 0.0f, 0.0f}, scale);
+    cluster.sync();  // the others' shared memory is read above
+    if (rank != 0) return;
+  }
+  if (tid >= 32) return;
+  // one warp finishes the row: the kept classes of the student, the teacher
+  const bool dup = sh.dup != 0;
+  const auto first_of = [&](int e) {  // of the entries of a class, by its place
+    if (!dup) return true;
+    for (int i = 0; i < e; ++i)
+      if (sh.index[i] == sh.index[e]) return false;
+    return true;
+  };
+  Sums kept{-INFINITY, 0.0f, 0.0f, 0.0f};
+  float tmax = -INFINITY, xmax = -INFINITY;
+  for (int e = lane; e < te.k; e += 32) {
+    if (sh.index[e] < 0) continue;
+    xmax = fmaxf(xmax, sh.x[e]);
+    tmax = fmaxf(tmax, sh.value[e]);
+  }
+  DistillRow r;
+  r.tmax = warp_max(tmax);
+  kept.m = warp_max(xmax);
+  float tsum = 0.0f, tcnt = 0.0f;
+  double mass = 0.0;
+  for (int e = lane; e < te.k; e += 32) {
+    if (sh.index[e] < 0) continue;
+    if (first_of(e)) {
+      if (sh.x[e] == kept.m) kept.cnt += 1.0f;
+      else kept.s += expf(scaled(sh.x[e] - kept.m, it));
+    }
+    const float tv = sh.value[e];
+    if (bucket) mass += exp(static_cast<double>(tv));
+    else if (tv == r.tmax) tcnt += 1.0f;
+    else tsum += expf(scaled(tv - r.tmax, it));
+  }
+  kept.s = warp_sum(kept.s);
+  kept.cnt = warp_sum(kept.cnt);
+  r.tlog = log1pf(warp_sum(tsum) + (warp_sum(tcnt) - 1.0f));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(kFullMask, mass, o);
+  const RowStat st =
+      row_stat(join_warp<T>(lane == 0 ? rest : lane == 1 ? kept : Sums{-INFINITY, 0.0f, 0.0f, 0.0f},
+                            scale));
+  r.m = st.m;
+  r.logs = st.m == INFINITY ? __int_as_float(0x7fffffff) : log1pf(st.s);
+  rest.m = __shfl_sync(kFullMask, rest.m, 0);
+  const float log_rest = rest.m == -INFINITY
+                             ? -INFINITY
+                             : log1pf(rest.s + (rest.cnt - 1.0f)) +
+                                   (rest.m == r.m ? 0.0f : scaled(rest.m - r.m, it)) - r.logs;
+  const float mass_r = bucket ? rest_mass(mass, sh.distinct == c, r.w1) : (r.w1 = 0.0f);
+  float sum = 0.0f;
+  for (int e = lane; e < te.k; e += 32) {
+    if (sh.index[e] < 0) continue;
+    const double lq = log_q(sh.value[e], r, bucket, it);
+    const double lp = (static_cast<double>(sh.x[e]) - r.m) * it.full - static_cast<double>(r.logs);
+    const float p = expf(static_cast<float>(lq));
+    const float d = static_cast<float>(lq - lp);
+    sum += first_of(e) ? divergence_term(p, d) : p * (d - 1.0f);
+  }
+  sum = warp_sum(sum);
+  if (lane == 0)
+    finish_row(r, sum, mass_r, log_rest, sh.distinct == 0, sh.bad != 0, dup, temperature,
+               loss + row, stats ? stats + row * kDsStats : nullptr);
 }
 
+// Rows of more than kNarrowMax classes, a warp per share of a row.
 template <typename T>
-__global__ void __launch_bounds__(kDsThreads)
-distill_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld, Teacher te,
-                   float temperature, InvT it, int bucket, const float* __restrict__ stats,
-                   const float* __restrict__ g_loss, int64_t g_stride, T* __restrict__ grad) {
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x;
+__global__ void __launch_bounds__(kMapThreads)
+distill_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld, Teacher te,
+                        float temperature, InvT it, int bucket, const float* __restrict__ stats,
+                        const float* __restrict__ g_loss, int64_t g_stride, int split, int warps,
+                        T* __restrict__ grad) {
+  const MapPlace at(warps);
+  if (at.row >= n || at.rank >= split) return;  // a whole warp
+  const int64_t row = at.row;
   const T* x = logits + row * ld;
   T* out = grad + row * c;
+  const RowShare<T> share(x, out, c, at.rank, split);
   const DistillRow r = load_row(stats + row * kDsStats);
   const float g = g_loss[row * g_stride] * temperature;
-  if (r.none != 0.0f || g == 0.0f || (r.m == -INFINITY && r.logs == r.logs)) {
-    for (int64_t j = tid; j < c; j += kDsThreads) out[j] = from_f<T>(0.0f);
+  if (r.kind == 2.0f || g == 0.0f || (r.m == -INFINITY && r.logs == r.logs)) {
+    share.template run<false>([](auto& v) {
+#pragma unroll
+      for (auto& p : v) p = both(0.0f);
+    });
     return;
   }
-  const float f = g * r.spread;
-  for (int64_t j = tid; j < c; j += kDsThreads) {
-    const float p = expf(scaled(to_f(x[j]) - r.m, it) - r.logs);
-    out[j] = from_f<T>(p * f);
+  const F2 f = both(g * r.spread);
+  if (sizeof(T) == 2 && r.m > -1e30f && r.m < 1e30f) {
+    // one operation on the logit (its rounding is far below the gradient's)
+    const F2 scale = both(kLog2e * it.hi);
+    const F2 shift = both(-(r.m * it.hi + (r.logs - r.lift)) * kLog2e);
+    share.template run<true>([&](auto& v) {
+#pragma unroll
+      for (auto& p : v) {
+        const F2 a = fma2(p, scale, shift);
+        p = mul2(F2{exp2_hw(a.x), exp2_hw(a.y)}, f);
+      }
+    });
+  } else {
+    share.template run<true>([&](auto& v) {
+#pragma unroll
+      for (auto& p : v) {
+        const F2 d = add2(p, both(-r.m));
+        F2 a{scaled(d.x, it) - (r.logs - r.lift), scaled(d.y, it) - (r.logs - r.lift)};
+        a = F2{max_nan(a.x, kExpFloor), max_nan(a.y, kExpFloor)};
+        p = mul2(exp_neg2<T>(a, kLog2e), f);
+      }
+    });
   }
-  __syncthreads();  // orders the writes above before those below
-  if (tid < te.k) {
-    const int64_t idx = teacher_index(te, row, tid);
-    const float v = teacher_value(te, row, tid);
-    if (idx >= 0 && idx < c && v != -INFINITY) {
-      const double lp = (static_cast<double>(to_f(x[idx])) - r.m) * it.full -
-                        static_cast<double>(r.logs);
-      out[idx] = from_f<T>(g * kept_gradient(te, row, c, idx, v, lp, r, bucket, it));
-    }
+  __syncwarp();  // orders the writes above before those below
+  for (int e = threadIdx.x & 31; e < te.k; e += 32) {
+    const int64_t idx = teacher_index(te, row, e);
+    if (!share.holds(idx)) continue;
+    const float v = teacher_value(te, row, e);
+    if (v == -INFINITY) continue;
+    const double lp = (static_cast<double>(to_f(x[idx])) - r.m) * it.full -
+                      static_cast<double>(r.logs);
+    out[idx] = from_f<T>(g * kept_gradient(te, row, c, idx, v, lp, r, bucket, it));
   }
 }
 
@@ -359,38 +467,46 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
   for (int i = 1; i < E; ++i) m = fmaxf(m, v[i]);
   m = group_max<G>(m);
   if (m != m) m = -INFINITY;
-  float s_rest = 0.0f, c_rest = 0.0f, s_kept = 0.0f, c_kept = 0.0f;
+  float m_rest = -INFINITY;
+  uint32_t kept_here = 0;
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     const int j = lane + G * i;
-    const bool kept = (bits[j >> 5] >> (j & 31)) & 1u;
-    const float one = j < c && v[i] == m ? 1.0f : 0.0f;
-    const float e = v[i] == m ? 0.0f : expf(scaled(v[i] - m, it));
+    if ((bits[j >> 5] >> (j & 31)) & 1u) kept_here |= 1u << i;
+    else m_rest = fmaxf(m_rest, v[i]);
+  }
+  m_rest = group_max<G>(m_rest);
+  // relative to their own maxima: that of the rest may be far below the row's
+  float s_rest = 0.0f, c_rest = 0.0f, s_kept = 0.0f, c_kept = 0.0f;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const bool kept = (kept_here >> i) & 1u;
+    const float ref = kept ? m : m_rest;
+    const bool top = v[i] == ref && lane + G * i < c;
+    const float d = v[i] - ref;
+    const float e = v[i] == ref ? 0.0f : expf(scaled(d, it));
     s_kept += kept ? e : 0.0f;
-    c_kept += kept ? one : 0.0f;
+    c_kept += kept && top ? 1.0f : 0.0f;
     s_rest += kept ? 0.0f : e;
-    c_rest += kept ? 0.0f : one;
+    c_rest += !kept && top ? 1.0f : 0.0f;
   }
   s_rest = group_sum<G>(s_rest);
   c_rest = group_sum<G>(c_rest);
-  const float s = s_rest + group_sum<G>(s_kept) + (group_sum<G>(c_kept) + c_rest - 1.0f);
+  s_kept = group_sum<G>(s_kept);
+  c_kept = group_sum<G>(c_kept);
   r.m = m;
+  // the sum of both relative to m, without one of its maxima
+  const bool low = m_rest < m;
+  const float fall = low ? scaled(m_rest - m, it) : 0.0f;
+  const float s = low ? s_kept + (c_kept - 1.0f) + (s_rest + c_rest) * expf(fall)
+                      : s_kept + s_rest + (c_kept + c_rest - 1.0f);
   r.logs = m == INFINITY ? __int_as_float(0x7fffffff) : log1pf(s);
-  const float p_rest = (s_rest + c_rest) / (1.0f + s);
-  float mass_r = 0.0f;
-  r.w1 = 0.0f;
-  if (bucket) {
+  const float log_rest =
+      m_rest == -INFINITY ? -INFINITY : log1pf(s_rest + (c_rest - 1.0f)) + fall - r.logs;
 #pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) mass += __shfl_xor_sync(kFullMask, mass, o);
-    // a small difference where the teacher is sure of its kept classes: 64 bits
-    const float raw = static_cast<float>(1.0 - mass);
-    if (raw == raw && raw < 0.0f) r.w1 = -raw;
-    else mass_r = raw;
-    if (distinct == static_cast<float>(c)) {  // no class is left to take the rest
-      r.w1 = -raw;
-      mass_r = 0.0f;
-    }
-  }
+  for (int o = G / 2; o > 0; o >>= 1) mass += __shfl_xor_sync(kFullMask, mass, o);
+  const float mass_r =
+      bucket ? rest_mass(mass, distinct == static_cast<float>(c), r.w1) : (r.w1 = 0.0f);
   float sum = 0.0f;
   for (int e = lane; e < te.k; e += G) {
     const int64_t idx = teacher_index(te, row, e);
@@ -408,7 +524,7 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
     sum += first ? divergence_term(q, d) : q * (d - 1.0f);
   }
   sum = group_sum<G>(sum);
-  if (live && lane == 0) finish_row(r, sum, mass_r, p_rest, distinct == 0.0f, bad, dup,
+  if (live && lane == 0) finish_row(r, sum, mass_r, log_rest, distinct == 0.0f, bad, dup,
                                     temperature, loss + row,
                                     stats ? stats + row * kDsStats : nullptr);
 }
@@ -431,13 +547,13 @@ distill_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
     v[i] = lane + G * i < c ? to_f(x[lane + G * i]) : -INFINITY;
   const DistillRow r = load_row(stats + row * kDsStats);
   const float g = g_loss[row * g_stride] * temperature;
-  const bool zero = r.none != 0.0f || g == 0.0f || (r.m == -INFINITY && r.logs == r.logs);
+  const bool zero = r.kind == 2.0f || g == 0.0f || (r.m == -INFINITY && r.logs == r.logs);
   const float f = g * r.spread;
 #pragma unroll
   for (int i = 0; i < E; ++i)
     if (lane + G * i < c)
       out[lane + G * i] =
-          from_f<T>(zero ? 0.0f : f * expf(scaled(v[i] - r.m, it) - r.logs));
+          from_f<T>(zero ? 0.0f : f * expf(scaled(v[i] - r.m, it) - (r.logs - r.lift)));
   if (zero) return;
   __syncwarp(mine);  // orders the writes above before those below
   for (int e = lane; e < te.k; e += G) {
@@ -509,19 +625,26 @@ int cign_distill_fwd(int64_t n, int64_t c, int32_t x_type, const void* logits, i
     CIGN_CHECK_LAUNCH("distill_narrow_fwd_kernel");
     return CIGN_OK;
   }
-  const size_t smem = static_cast<size_t>((c + 31) / 32) * 4;
+  const int words = static_cast<int>((c + 15) / 32 + 1);  // a bit per element of the frame
+  const int64_t granules = c * type_size(x_type) / 16;
+  int warps = wide_warps(n, granules);
+  if (warps == 1 && c > 8192) warps = 4;  // four rows' bits would crowd out blocks
   CIGN_TYPE_DISPATCH(x_type, T, {
-    if (smem > 32768)
-      CIGN_CHECK_CUDA(cudaFuncSetAttribute(distill_fwd_kernel<T>,
-                                           cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           static_cast<int>(kDsMaxClasses / 8)),
+    const T* x = static_cast<const T*>(logits);
+    const auto kernel = warps == 1   ? distill_wide_fwd_kernel<T, 1>
+                        : warps == 4 ? distill_wide_fwd_kernel<T, 4>
+                                     : distill_wide_fwd_kernel<T, 8>;
+    const size_t smem = static_cast<size_t>(words) * 4 * (warps == 1 ? 4 : 1);
+    if (smem > 32768)  // beyond what a kernel has by default, with its own 5 KB
+      CIGN_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           static_cast<int>(kDsMaxClasses / 8 + 64)),
                       "distill_fwd: shared memory");
-    distill_fwd_kernel<T><<<static_cast<unsigned>(n), kDsThreads, smem, s>>>(
-        n, c, static_cast<const T*>(logits), ld, te, temperature, inverse(temperature), tail, loss,
-        stats);
+    const int split = warps == 8 ? wide_split(n, granules, 256) : 1;
+    return launch_cluster(kernel, static_cast<unsigned>(warps == 1 ? (n + 3) / 4 : n * split),
+                          warps == 8 ? 256 : 128, smem, split, s, "distill_wide_fwd_kernel", n, c,
+                          x, ld, te, temperature, inverse(temperature), tail, split, words, loss,
+                          stats);
   });
-  CIGN_CHECK_LAUNCH("distill_fwd_kernel");
-  return CIGN_OK;
 }
 
 int cign_distill_bwd(int64_t n, int64_t c, int32_t x_type, const void* logits, int64_t ld,
@@ -547,11 +670,12 @@ int cign_distill_bwd(int64_t n, int64_t c, int32_t x_type, const void* logits, i
     CIGN_CHECK_LAUNCH("distill_narrow_bwd_kernel");
     return CIGN_OK;
   }
+  const MapGrid m = map_grid(n, c * type_size(x_type) / 16 + 2);
   CIGN_TYPE_DISPATCH(x_type, T,
-      distill_bwd_kernel<T><<<static_cast<unsigned>(n), kDsThreads, 0, s>>>(
+      distill_wide_bwd_kernel<T><<<m.grid, kMapThreads, 0, s>>>(
           n, c, static_cast<const T*>(logits), ld, te, temperature, inverse(temperature), tail,
-          stats, grad_loss, grad_loss_stride, static_cast<T*>(grad_logits)));
-  CIGN_CHECK_LAUNCH("distill_bwd_kernel");
+          stats, grad_loss, grad_loss_stride, m.split, m.warps, static_cast<T*>(grad_logits)));
+  CIGN_CHECK_LAUNCH("distill_wide_bwd_kernel");
   return CIGN_OK;
 }
 

@@ -14,8 +14,6 @@
 namespace cign {
 namespace {
 
-constexpr int kLpThreads = 256;
-constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpMaxTop = 64;
 
 struct LogProbOut {
@@ -414,53 +412,6 @@ struct LogProbGrads {
   const float* top;  // [n, top_k] contiguous
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads)
-log_probs_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld,
-                     const int64_t* __restrict__ labels, const float* __restrict__ stats,
-                     const float* __restrict__ entropy, int top_k,
-                     const int64_t* __restrict__ top_index, LogProbGrads g,
-                     T* __restrict__ grad) {
-  const int64_t row = blockIdx.x;
-  const T* x = logits + row * ld;
-  T* out = grad + row * c;
-  const float nan = __int_as_float(0x7fffffff);
-  const int64_t y = (g.log_prob && labels) ? labels[row] : -1;
-  const float gl = y >= 0 ? (y < c ? g.log_prob[row * g.log_prob_stride] : nan) : 0.0f;
-  const float gh = g.entropy ? g.entropy[row * g.entropy_stride] : 0.0f;
-  const float m = stats[2 * row], logs = stats[2 * row + 1];
-  float G = gl;
-  bool any = !(gl == 0.0f) || !(gh == 0.0f);
-  if (g.top)
-    for (int i = 0; i < top_k; ++i) {
-      const float v = g.top[row * top_k + i];
-      G += v;
-      any |= !(v == 0.0f);
-    }
-  const float H = g.entropy ? entropy[row] : 0.0f;
-  // no gradient reaches the row, or it has no distribution
-  const bool zero = !any || (m == -INFINITY && logs == logs);
-  for (int64_t j = threadIdx.x; j < c; j += kLpThreads) {
-    float v = 0.0f;
-    if (!zero) {
-      const float lp = (to_f(x[j]) - m) - logs;
-      const float p = expf(lp);
-      const float spread = p > 0.0f ? gh * p * (lp + H) : gh * p;
-      float a = 0.0f;
-      bool special = j == y;
-      if (special) a = gl;
-      if (g.top)
-        for (int i = 0; i < top_k; ++i)
-          if (top_index[row * top_k + i] == j) {
-            a += g.top[row * top_k + i];
-            special = true;
-          }
-      v = special ? (a - G) - G * expm1f(lp) - spread : -p * G - spread;
-    }
-    out[j] = from_f<T>(v);
-  }
-}
-
 // What reaches a row: the sum G of the gradients of its log probabilities, the
 // entropy's, and whether there is any at all.
 struct RowGrads {
@@ -546,6 +497,78 @@ log_probs_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int6
     for (int i = 0; i < top_k; ++i) {
       const int64_t j = top_index[row * top_k + i];
       if ((j & (G - 1)) == lane)
+        out[j] = from_f<T>(special_grad<T>(g, r, top_index, top_k, row, j,
+                                           (to_f(x[j]) - st.x) - st.y));
+    }
+}
+
+// Rows of more than kNarrowMax classes, a warp per share of a row.
+template <typename T>
+__global__ void __launch_bounds__(kMapThreads)
+log_probs_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld,
+                          const int64_t* __restrict__ labels, const float* __restrict__ stats,
+                          const float* __restrict__ entropy, int top_k,
+                          const int64_t* __restrict__ top_index, LogProbGrads g, int split,
+                          int warps, T* __restrict__ grad) {
+  const MapPlace at(warps);
+  if (at.row >= n || at.rank >= split) return;  // a whole warp
+  const int64_t row = at.row;
+  const T* x = logits + row * ld;
+  T* out = grad + row * c;
+  const RowShare<T> share(x, out, c, at.rank, split);
+  const float2 st = *reinterpret_cast<const float2*>(stats + 2 * row);
+  const RowGrads r = row_grads(g, labels, entropy, top_k, row, c);
+  // no gradient reaches the row, or it has no distribution
+  if (!r.any || (st.x == -INFINITY && st.y == st.y)) {
+    share.template run<false>([](auto& v) {
+#pragma unroll
+      for (auto& p : v) p = both(0.0f);
+    });
+    return;
+  }
+  // -p G - gh p (lp + H) = p (A + B lp)
+  const F2 A = both(-(r.all + r.gh * r.H)), B = both(-r.gh);
+  if (sizeof(T) == 2 && st.x > -1e30f && st.x < 1e30f) {
+    // e^lp by one operation on the logit (its rounding is far below the gradient's)
+    const F2 scale = both(kLog2e), shift = both(-(st.x + st.y) * kLog2e);
+    const F2 B2 = both(B.x * 0.693147181f);
+    if (r.gh == 0.0f) {
+      share.template run<true>([&](auto& v) {
+#pragma unroll
+        for (auto& p : v) {
+          const F2 a = fma2(p, scale, shift);
+          p = mul2(F2{exp2_hw(a.x), exp2_hw(a.y)}, A);
+        }
+      });
+    } else {
+      share.template run<true>([&](auto& v) {
+#pragma unroll
+        for (auto& p : v) {
+          F2 a = fma2(p, scale, shift);
+          a = F2{max_nan(a.x, kExpFloor), max_nan(a.y, kExpFloor)};  // -inf: p = 0
+          p = mul2(F2{exp2_hw(a.x), exp2_hw(a.y)}, fma2(B2, a, A));
+        }
+      });
+    }
+  } else {
+    share.template run<true>([&](auto& v) {
+#pragma unroll
+      for (auto& p : v) {
+        F2 lp = add2(add2(p, both(-st.x)), both(-st.y));
+        lp = F2{max_nan(lp.x, kExpFloor), max_nan(lp.y, kExpFloor)};
+        p = mul2(exp_neg2<T>(lp, kLog2e), fma2(B, lp, A));
+      }
+    });
+  }
+  __syncwarp();  // orders the writes above before those below
+  const int lane = threadIdx.x & 31;
+  if (lane == 0 && r.y >= 0 && r.y < c && share.holds(r.y))
+    out[r.y] = from_f<T>(special_grad<T>(g, r, top_index, top_k, row, r.y,
+                                         (to_f(x[r.y]) - st.x) - st.y));
+  if (g.top)
+    for (int i = lane; i < top_k; i += 32) {
+      const int64_t j = top_index[row * top_k + i];
+      if (share.holds(j))
         out[j] = from_f<T>(special_grad<T>(g, r, top_index, top_k, row, j,
                                            (to_f(x[j]) - st.x) - st.y));
     }
@@ -640,11 +663,12 @@ int cign_node_log_probs_bwd(int64_t n, int64_t c, int32_t x_type, const void* lo
     CIGN_CHECK_LAUNCH("log_probs_narrow_bwd_kernel");
     return CIGN_OK;
   }
+  const MapGrid m = map_grid(n, c * type_size(x_type) / 16 + 2);
   CIGN_TYPE_DISPATCH(x_type, T,
-      log_probs_bwd_kernel<T><<<static_cast<unsigned>(n), kLpThreads, 0, s>>>(
+      log_probs_wide_bwd_kernel<T><<<m.grid, kMapThreads, 0, s>>>(
           n, c, static_cast<const T*>(logits), ld, labels, stats, entropy, top_k, top_index, g,
-          static_cast<T*>(grad_logits)));
-  CIGN_CHECK_LAUNCH("log_probs_bwd_kernel");
+          m.split, m.warps, static_cast<T*>(grad_logits)));
+  CIGN_CHECK_LAUNCH("log_probs_wide_bwd_kernel");
   return CIGN_OK;
 }
 

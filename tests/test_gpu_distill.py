@@ -52,11 +52,15 @@ def reference(x, v, i, temp, tail, g):
     mass, r = q.sum(1), torch.zeros_like(loss)
     if tail == "bucket":
         r = torch.where(kept.all(1), 0.0, (1 - mass).clamp(min=0.0))
-        loss = loss + torch.where(r > 0, r * (r.log() - p_rest.log()), 0.0)
+        # by logarithms: p_rest may be far below what its exponentials can hold
+        log_rest = torch.logsumexp(logp.masked_fill(kept, -INF), 1)
+        loss = loss + torch.where(r > 0, r * (r.log() - log_rest), 0.0)
+        spread = torch.where(kept | (logp == -INF), 0.0, r[:, None] * (logp - log_rest[:, None]).exp())
+    else:
+        spread = torch.zeros_like(p)
     W = mass + r
-    ratio = torch.where(r > 0, r / p_rest, 0.0)
-    grad = W[:, None] * p - target - torch.where(kept, 0.0, p * ratio[:, None])
-    grad = torch.where((W[:, None] * p == target), 0.0, grad) * temp * g[:, None]
+    grad = W[:, None] * p - target - spread
+    grad = grad * temp * g[:, None]
     # k roundings on the way of each probability; those of the log sum cancel in the loss to first order,
     # what is left is weighted with |p - q|, which is at most sqrt(2 KL) in all (Pinsker)
     d = torch.where(torch.isfinite(z), z.amax(1, keepdim=True) - z, 0.0)
@@ -69,7 +73,7 @@ def reference(x, v, i, temp, tail, g):
     # leave terms q (d - 1) of either sign, whose roundings count with their magnitudes
     twice = (kept.sum(1) < here.sum(1))
     tloss = tloss + torch.where(twice, temp ** 2 * ku * torch.where(q > 0, q * (1 + delta.abs()), 0.0).sum(1), 0.0)
-    tgrad = temp * g.abs()[:, None] * (ku * (dmax[:, None] + d) * (p * (1 + ratio[:, None]) + 0 * p)
+    tgrad = temp * g.abs()[:, None] * (ku * (dmax[:, None] + d) * (p + spread)
                                        + ku * (target + (W[:, None] * p - target).abs()))
     return temp ** 2 * loss, grad, tloss, tgrad
 
@@ -184,8 +188,9 @@ def test_masked_students(cuda, c, tail):
     check(loss[[0, 4]], want[[0, 2]], tl[[0, 2]], "loss")
     check(grad[[0, 3, 4]], wgrad, torch.where(torch.isfinite(tg), tg, 64 * U), "grad")
     for row in (2, 5):
-        # the others have probability 0: with a rest to place the divergence is infinite
-        if tail == "bucket":
+        # the others have probability 0: with a rest to place the divergence is infinite (row 2), or, as the
+        # lowest value is finite, r times its distance
+        if tail == "bucket" and row == 2:
             assert loss[row] == INF
         else:
             e, eg, te, tge = reference(x[row:row + 1, :], v[row:row + 1], i[row:row + 1], 1.0, tail, torch.ones(1, device=cuda))
@@ -304,3 +309,26 @@ def test_refusals(cuda):
                         ((x, v[:, :1].expand(4, 257), i[:, :1].expand(4, 257)), ValueError)):
         with pytest.raises(error):
             distill_top_logits(*args)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c", [6, 60, 900, 30000])
+def test_far_rest_keeps_its_share(cuda, c, dtype):
+    """The student's other classes are e^-95 and e^-190 below its kept ones, less than float32 can hold: the rest's
+    part of the loss and its gradient are those of the logarithms."""
+    k = 3
+    x, v, i, gen = make(cuda, 4, c, k, torch.float32, "bucket", 1.0)
+    kept = torch.zeros(4, c, dtype=torch.bool, device=cuda).scatter_(1, i, True)
+    gap = torch.tensor([[30.0], [95.0], [190.0], [60.0]], device=cuda)
+    x = torch.where(kept, x, x - gap).to(dtype).requires_grad_()
+    v = v - 0.5
+    g = 0.5 + torch.rand(4, generator=gen, device=cuda)
+    want, wgrad, tl, tg = reference(x, v, i, 1.0, "bucket", g)
+    # the gradient of the others is r times their distribution among themselves, known to the roundings of the
+    # exponents, which are relative to the gap
+    rest = torch.where(kept, 0.0, torch.softmax(x.detach().double().masked_fill(kept, -INF), 1))
+    tg = torch.where(kept, tg, 512 * U * (1 + gap.double() / 8) * rest * g.double()[:, None])
+    loss = distill_top_logits(x, v, i, 1.0, "bucket")
+    check(loss, want, 512 * U * want.abs(), "loss")
+    (grad,) = torch.autograd.grad(loss, x, g)
+    check(grad, wgrad, tg, "grad")

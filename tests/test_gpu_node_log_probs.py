@@ -135,6 +135,21 @@ def test_equal_logits_go_to_the_lower_class(cuda, c):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,c,k", [(4, 30, 10), (4, 300, 40), (300, 5000, 64), (2, 70001, 20), (4000, 1500, 50)])
+def test_fewer_classes_left_than_asked_for(cuda, n, c, k, dtype):
+    """All but three classes are masked: the best are these, then masked ones by their index."""
+    g = torch.Generator(device=cuda).manual_seed(c)
+    x = torch.full((n, c), -INF, device=cuda, dtype=dtype)
+    at = torch.rand(n, c, generator=g, device=cuda).topk(3, 1)[1]
+    x.scatter_(1, at, torch.randn(n, 3, generator=g, device=cuda).to(dtype))
+    out = node_log_probs(x, None, k)
+    order = torch.sort(x.float(), dim=1, descending=True, stable=True)[1][:, :k]
+    assert torch.equal(out.top_index, order)
+    logp = torch.log_softmax(x.double(), 1).gather(1, order)
+    check(out.top_log_probs, logp, 64 * U * (1 + torch.where(torch.isfinite(logp), logp.abs(), 0.0)), "top")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("c", [1, 5, 90, 600, 20000])
 def test_masked_rows_and_lowest_values(cuda, c, dtype):
     low = torch.finfo(dtype).min
