@@ -646,14 +646,12 @@ int launch_cluster(void (*kernel)(Params...), unsigned grid, int threads, size_t
 
 // Warps of a team.  What a row costs each warp at its ends (the maxima, the
 // sums, the barriers) is as much as about eight rounds of loads, so a team has
-// no more warps than keep the device busy with some rows to spare (48 warps per
-// SM are about two rows per resident team).
+// no more warps than it takes to fill the device: single warps want two rows
+// per resident warp to even out, teams of four one row per resident team.
 inline int wide_warps(int64_t n, int64_t granules) {
-  const int64_t wanted = static_cast<int64_t>(sm_count()) * 48;
-  int warps = 1;
-  while (warps < 8 && n * warps < wanted && granules >= static_cast<int64_t>(64) * warps)
-    warps = warps == 1 ? 4 : 8;
-  return warps;
+  const int64_t sms = sm_count();
+  if (n >= 48 * sms || granules < 64) return 1;
+  return n >= 4 * sms || granules < 256 ? 4 : 8;
 }
 
 // Blocks that share a row of `granules` where there are too few rows to fill
