@@ -306,9 +306,19 @@ __device__ __forceinline__ float key_value(uint32_t u) {
 // aligned bytes per thread and load.  A row may start anywhere: granule g of
 // V = 16 / sizeof(T) elements covers the row's elements g V - shift ..., and the
 // two granules at its ends are read by elements.
-// Granules of a thread that are in flight together (and as many are worked on).
+// Granules of a thread that are worked on together.
 template <typename T>
 constexpr int kWideLoads = 4;
+// Rounds of them that a streaming thread has in its own slots of shared memory
+// (cp.async, no barriers: a thread reads only what it asked for).  Held there
+// instead of in registers, the round that is under way leaves 64 registers to a
+// thread and room for a third more warps (2048 x 65537 bf16 with 20 best
+// classes: 87 us, 109 with registers; 95 with three rounds).
+constexpr int kRingRounds = 2;
+template <typename T>
+__host__ __device__ constexpr size_t ring_bytes(int threads) {
+  return static_cast<size_t>(kRingRounds) * kWideLoads<T> * 16 * threads;
+}
 
 constexpr int64_t kWideMax = (1ll << 31) - 16;  // classes: positions in a row are 32-bit
 
@@ -369,6 +379,51 @@ struct RowFrame {
   }
 };
 
+// A thread's granules of a frame, round by round through shared memory.
+template <typename T, int THREADS>
+struct Ring {
+  static constexpr int V = RowFrame<T>::V;
+  static constexpr int L = kWideLoads<T>;
+  uint32_t slots;  // this thread's first slot
+  const T* ask;    // the first granule of the next round to ask for
+  int ask_g, ask_slot, read_slot;
+  int g1;
+  __device__ __forceinline__ Ring(const RowFrame<T>& f, void* smem, int tid)
+      : slots(smem_u32(smem) + 16 * tid), ask(f.base + static_cast<int64_t>(f.g0 + tid) * V),
+        ask_g(f.g0 + tid), ask_slot(0), read_slot(0), g1(f.g1) {
+#pragma unroll
+    for (int k = 0; k < kRingRounds - 1; ++k) next();
+  }
+  __device__ __forceinline__ void next() {
+#pragma unroll
+    for (int u = 0; u < L; ++u)
+      if (ask_g + u * THREADS < g1)
+        cp_async16_s(slots + (ask_slot + u) * 16 * THREADS, ask + u * THREADS * V);
+    cp_async_commit();
+    ask += L * THREADS * V;
+    ask_g += L * THREADS;
+    ask_slot = ask_slot + L == kRingRounds * L ? 0 : ask_slot + L;
+  }
+  // The round at read_slot, whose first granule of this thread is g, with AHEAD
+  // rounds asked for behind it.
+  template <int AHEAD>
+  __device__ __forceinline__ void read(Pack<T, V> (&q)[L], int g, float outside) {
+    cp_async_wait<AHEAD>();
+#pragma unroll
+    for (int u = 0; u < L; ++u) {
+      const float4 w = lds_f4(slots + (read_slot + u) * 16 * THREADS);
+      q[u] = *reinterpret_cast<const Pack<T, V>*>(&w);
+      if (g + u * THREADS >= g1) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) q[u].e[e] = from_f<T>(outside);
+      }
+    }
+  }
+  __device__ __forceinline__ void advance() {
+    read_slot = read_slot + L == kRingRounds * L ? 0 : read_slot + L;
+  }
+};
+
 template <typename T, int V>
 __device__ __forceinline__ void unpack(const Pack<T, V>& q, F2 (&v)[V / 2]) {
 #pragma unroll
@@ -384,19 +439,19 @@ __device__ __forceinline__ Pack<T, 2 * N> pack_of(const F2 (&v)[N]) {
   }
   return q;
 }
-template <int N>
-__device__ __forceinline__ float max_of(const F2 (&v)[N]) {
-  float m = max_nan(v[0].x, v[0].y);
-#pragma unroll
-  for (int i = 1; i < N; ++i) m = max3_nan(m, v[i].x, v[i].y);
-  return m;
+__device__ __forceinline__ float max_of(const F2 (&v)[2]) {
+  return max3_nan(max_nan(v[0].x, v[0].y), v[1].x, v[1].y);
 }
-template <int N>
-__device__ __forceinline__ float min_of(const F2 (&v)[N]) {
-  float m = min3_nan(v[0].x, v[0].y, INFINITY);
-#pragma unroll
-  for (int i = 1; i < N; ++i) m = min3_nan(m, v[i].x, v[i].y);
-  return m;
+__device__ __forceinline__ float max_of(const F2 (&v)[4]) {
+  return max3_nan(max3_nan(v[0].x, v[0].y, v[1].x), max3_nan(v[1].y, v[2].x, v[2].y),
+                  max_nan(v[3].x, v[3].y));
+}
+__device__ __forceinline__ float min_of(const F2 (&v)[2]) {
+  return min3_nan(min3_nan(v[0].x, v[0].y, v[1].x), v[1].y, INFINITY);
+}
+__device__ __forceinline__ float min_of(const F2 (&v)[4]) {
+  return min3_nan(min3_nan(v[0].x, v[0].y, v[1].x), min3_nan(v[1].y, v[2].x, v[2].y),
+                  min3_nan(v[3].x, v[3].y, INFINITY));
 }
 
 // One warp's share of a row, the rank-th of `split`, taken through f (which
@@ -515,9 +570,9 @@ struct Stream {
   static constexpr bool kOneStep = sizeof(T) == 2;
   float m, ref, cnt;  // ref = m but where m scale would overflow to -inf
   float shift;        // kOneStep: ref scale, rounded
-  F2 s, u;            // u: kOneStep: sum of e times the argument; else t
-  __device__ __forceinline__ Stream(float start, float scale)
-      : cnt(0.0f), s{0.0f, 0.0f}, u{0.0f, 0.0f} {
+  F2 s[2], u[2];      // two chains each; u: kOneStep: sum of e times the argument; else t
+  __device__ __forceinline__ Stream(float start, float scale) : cnt(0.0f) {
+    s[0] = s[1] = u[0] = u[1] = both(0.0f);
     set(start, scale);
   }
   __device__ __forceinline__ void set(float to, float scale) {
@@ -533,14 +588,14 @@ struct Stream {
         F2 a = fma2(v[i], both(scale), both(-shift));
         if (CLAMP) a = F2{max_nan(a.x, kExpFloor), max_nan(a.y, kExpFloor)};
         const F2 e{exp2_hw(a.x), exp2_hw(a.y)};
-        s = add2(s, e);
-        if (ENTROPY) u = fma2(e, a, u);
+        s[i % 2] = add2(s[i % 2], e);
+        if (ENTROPY) u[i % 2] = fma2(e, a, u[i % 2]);
       } else {
         F2 d = add2(v[i], both(-ref));
         if (CLAMP) d = F2{max_nan(d.x, kExpFloor), max_nan(d.y, kExpFloor)};
         const F2 e = exp_neg2<T>(d, scale);
-        s = add2(s, e);
-        if (ENTROPY) u = fma2(e, d, u);
+        s[i % 2] = add2(s[i % 2], e);
+        if (ENTROPY) u[i % 2] = fma2(e, d, u[i % 2]);
       }
     }
   }
@@ -559,14 +614,15 @@ struct Stream {
     if (min_of(v) - ref < kExpFloor) sum<true>(v, scale);
     else sum<false>(v, scale);
   }
+  __device__ __forceinline__ static float all(const F2 (&p)[2]) {
+    return (p[0].x + p[0].y) + (p[1].x + p[1].y);
+  }
   __device__ __forceinline__ float total_s(float scale) const {
-    const float x = s.x + s.y;
-    return kOneStep ? x * exp2_hw(left(scale)) : x;
+    return kOneStep ? all(s) * exp2_hw(left(scale)) : all(s);
   }
   __device__ __forceinline__ float total_t(float scale) const {
-    const float x = u.x + u.y;
     const float r = left(scale);
-    return kOneStep ? exp2_hw(r) * fmaf(r, s.x + s.y, x) / scale : x;
+    return kOneStep ? exp2_hw(r) * fmaf(r, all(s), all(u)) / scale : all(u);
   }
   __device__ __forceinline__ float left(float scale) const {  // of rounding ref scale
     const float r = -fmaf(ref, scale, -shift);
@@ -575,19 +631,18 @@ struct Stream {
   __device__ __forceinline__ void raise(float to, float scale) {
     const float d = max_nan(m - to, kExpFloor);
     const float f = exp_neg2<T>(both(d), scale).x;
-    const float n = (total_s(scale) + cnt) * f;
-    if (ENTROPY) {
-      const float t = fmaf(n, d, f * total_t(scale));
-      u = F2{kOneStep ? t * scale : t, 0.0f};
-    }
-    s = F2{n, 0.0f};
-    cnt = 0.0f;
+    float n = (total_s(scale) + cnt) * f;
+    float w = ENTROPY ? fmaf(n, d, f * total_t(scale)) : 0.0f;
     set(to, scale);
     if (kOneStep) {  // as sums whose rounding is still to be put back
       const float r = left(scale), g = exp2_hw(-r);
-      s.x *= g;
-      u.x = g * u.x - r * s.x;
+      n *= g;
+      w = g * (w * scale) - r * n;
     }
+    s[0] = F2{n, 0.0f};
+    u[0] = F2{w, 0.0f};
+    s[1] = u[1] = both(0.0f);
+    cnt = 0.0f;
   }
 };
 

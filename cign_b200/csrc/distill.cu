@@ -168,7 +168,7 @@ struct alignas(16) DistillShared {
 };
 
 template <typename T, int W>
-__global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 8 ? 3 : 6)
+__global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 8 ? 4 : 8)
 distill_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld, Teacher te,
                         float temperature, InvT it, int bucket, int split, int words,
                         float* __restrict__ loss, float* __restrict__ stats) {
@@ -176,7 +176,9 @@ distill_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
   constexpr int L = kWideLoads<T>;
   constexpr int kTeams = W == 1 ? 4 : 1;
   constexpr int kThreads = 32 * W;
-  extern __shared__ uint32_t all_bits[];
+  // the ring of the loads, then the teams' bits
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  uint32_t* all_bits = reinterpret_cast<uint32_t*>(dynamic + ring_bytes<T>(kTeams * kThreads));
   __shared__ DistillShared<W> all[kTeams];
   const int team = W == 1 ? threadIdx.x >> 5 : 0;
   const int tid = W == 1 ? threadIdx.x & 31 : threadIdx.x;
@@ -191,8 +193,8 @@ distill_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
   const int rounds = frame.template rounds<L>(kThreads);
   const float scale = kLog2e * it.hi;
 
-  Pack<T, V> q[L], next[L];
-  frame.load(q, 0, tid, kThreads, -INFINITY);
+  Pack<T, V> q[L];
+  Ring<T, kThreads> ring(frame, dynamic + team * ring_bytes<T>(kThreads), tid);
   for (int i = tid; i < words; i += kThreads) bits[i] = 0;
   if (tid == 0) sh.bad = sh.dup = sh.distinct = 0;
   team_sync<W>();
@@ -230,6 +232,7 @@ distill_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
   const int edge = tid == 0 ? frame.head : tid == 1 ? frame.tail : -1;
   const Pack<T, V> ends = frame.edge(edge, -INFINITY);
   float most = -INFINITY;
+  ring.template read<kRingRounds - 2>(q, frame.g0 + tid, -INFINITY);
 #pragma unroll
   for (int u = 0; u < L; ++u) {
     const int g = frame.g0 + tid + kThreads * u;
@@ -252,14 +255,15 @@ distill_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
   sums.add(v, ends_top, scale);
 #pragma unroll 1
   for (int k = 0; k < rounds; ++k) {
-    if (k + 1 < rounds) frame.load(next, k + 1, tid, kThreads, -INFINITY);
+    ring.next();
+    ring.template read<kRingRounds - 1>(q, frame.g0 + tid + kThreads * L * k, -INFINITY);
+    ring.advance();
 #pragma unroll
     for (int u = 0; u < L; ++u) {
       const int g = frame.g0 + tid + kThreads * (k * L + u);
       unpack(q[u], v);
       if (g < frame.g1) drop_kept(g);
       sums.add(v, max_of(v), scale);
-      q[u] = next[u];
     }
   }
   Sums rest{sums.m, sums.total_s(scale), sums.cnt, 0.0f};
@@ -634,11 +638,12 @@ int cign_distill_fwd(int64_t n, int64_t c, int32_t x_type, const void* logits, i
     const auto kernel = warps == 1   ? distill_wide_fwd_kernel<T, 1>
                         : warps == 4 ? distill_wide_fwd_kernel<T, 4>
                                      : distill_wide_fwd_kernel<T, 8>;
-    const size_t smem = static_cast<size_t>(words) * 4 * (warps == 1 ? 4 : 1);
-    if (smem > 32768)  // beyond what a kernel has by default, with its own 5 KB
-      CIGN_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           static_cast<int>(kDsMaxClasses / 8 + 64)),
-                      "distill_fwd: shared memory");
+    const size_t smem = ring_bytes<T>(warps == 8 ? 256 : 128) +
+                        static_cast<size_t>(words) * 4 * (warps == 1 ? 4 : 1);
+    CIGN_CHECK_CUDA(
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(ring_bytes<T>(256) + kDsMaxClasses / 8 + 64)),
+        "distill_fwd: shared memory");
     const int split = warps == 8 ? wide_split(n, granules, 256) : 1;
     return launch_cluster(kernel, static_cast<unsigned>(warps == 1 ? (n + 3) / 4 : n * split),
                           warps == 8 ? 256 : 128, smem, split, s, "distill_wide_fwd_kernel", n, c,

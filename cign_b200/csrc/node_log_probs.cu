@@ -193,7 +193,7 @@ __device__ __forceinline__ void find_floor(WideShared<W>& sh, float most, int sl
 // 16 shares of what it reads; after the pass these give a floor for the best
 // classes, and only the few shares that reach it are read again.
 template <typename T, int W, bool TOP>
-__global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 8 ? 3 : 6)
+__global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 8 ? 4 : 8)
 log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld,
                           const int64_t* __restrict__ labels, int top_k, int split,
                           LogProbOut out) {
@@ -201,6 +201,7 @@ log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
   constexpr int L = kWideLoads<T>;
   constexpr int kTeams = W == 1 ? 4 : 1;
   constexpr int kThreads = 32 * W;
+  extern __shared__ __align__(16) unsigned char ring_slots[];
   __shared__ WideShared<W> all[kTeams];
   const int team = W == 1 ? threadIdx.x >> 5 : 0;
   const int tid = W == 1 ? threadIdx.x & 31 : threadIdx.x;
@@ -213,13 +214,14 @@ log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
   const RowFrame<T> frame(x, c, rank, W == 8 ? split : 1);
   const int rounds = frame.template rounds<L>(kThreads);
 
-  Pack<T, V> q[L], next[L];
+  Pack<T, V> q[L];
   F2 v[V / 2];
-  frame.load(q, 0, tid, kThreads, -INFINITY);
+  Ring<T, kThreads> ring(frame, ring_slots + team * ring_bytes<T>(kThreads), tid);
   // the two ends of the row, by the first two threads
   const int edge = tid == 0 ? frame.head : tid == 1 ? frame.tail : -1;
   const Pack<T, V> ends = frame.edge(edge, -INFINITY);
   float most = -INFINITY;
+  ring.template read<kRingRounds - 2>(q, frame.g0 + tid, -INFINITY);
 #pragma unroll
   for (int u = 0; u < L; ++u) {
     unpack(q[u], v);
@@ -245,14 +247,15 @@ log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
   int slots = 0, rest = per_slot;
 #pragma unroll 1
   for (int k = 0; k < rounds; ++k) {
-    if (k + 1 < rounds) frame.load(next, k + 1, tid, kThreads, -INFINITY);
+    ring.next();
+    ring.template read<kRingRounds - 1>(q, frame.g0 + tid + kThreads * L * k, -INFINITY);
+    ring.advance();
 #pragma unroll
     for (int u = 0; u < L; ++u) {
       unpack(q[u], v);
       const float top = max_of(v);
       sums.add(v, top, kLog2e);
       if (TOP) share = max_nan(share, top);
-      q[u] = next[u];
     }
     if (TOP && (--rest == 0 || k + 1 == rounds)) {
       sh.slot[slots++][tid] = share;
@@ -624,13 +627,17 @@ int cign_node_log_probs_fwd(int64_t n, int64_t c, int32_t x_type, const void* lo
                                               : log_probs_wide_fwd_kernel<T, 1, false>)
                                      : (top_k ? log_probs_wide_fwd_kernel<T, 4, true>
                                               : log_probs_wide_fwd_kernel<T, 4, false>);
-      kernel<<<static_cast<unsigned>(warps == 1 ? (n + 3) / 4 : n), 128, 0, s>>>(
+      kernel<<<static_cast<unsigned>(warps == 1 ? (n + 3) / 4 : n), 128, ring_bytes<T>(128), s>>>(
           n, c, x, ld, labels, top_k, 1, out);
     } else {
       const int split = wide_split(n, granules, 256);
-      return launch_cluster(top_k ? log_probs_wide_fwd_kernel<T, 8, true>
-                                  : log_probs_wide_fwd_kernel<T, 8, false>,
-                            static_cast<unsigned>(n * split), 256, 0, split, s,
+      const auto kernel = top_k ? log_probs_wide_fwd_kernel<T, 8, true>
+                                : log_probs_wide_fwd_kernel<T, 8, false>;
+      CIGN_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           static_cast<int>(ring_bytes<T>(256))),
+                      "node_log_probs_fwd: shared memory");
+      return launch_cluster(kernel, static_cast<unsigned>(n * split), 256, ring_bytes<T>(256),
+                            split, s,
                             "log_probs_wide_fwd_kernel", n, c, x, ld, labels, top_k, split, out);
     }
   });
