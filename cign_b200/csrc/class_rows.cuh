@@ -221,10 +221,9 @@ __device__ __forceinline__ RowStat stat_shfl_xor(const RowStat& a, int o) {
 // Rows of at most E G classes are held by a group of G lanes (a power of two),
 // class lane + G i in register i < E: a row is read once, and the 32 / G rows
 // of a warp are neighbours.  A row costs a warp E of its steps, the sums over
-// the group and one logarithm, so a kernel that reads rows is cheapest with few
-// lanes and many classes per lane (2.45M x 47 float32: 132 us with 4 lanes, 177
-// with 8, 159 with 2, whose loads are too scattered); one that writes rows has
-// no sums and wants whole sectors (205 us with 8 lanes, 244 with 4, 291 with 16).
+// the group, one logarithm and what is read once per row, so few lanes and many
+// classes per lane are cheapest (2.45M x 47 float32 forward: 132 us with 4
+// lanes, 177 with 8, 159 with 2, whose loads are too scattered).
 constexpr int kNarrowThreads = 256;
 constexpr int64_t kNarrowMax = 256;
 
@@ -254,8 +253,7 @@ inline unsigned narrow_grid(int64_t n, int G) {
 #define CIGN_GROUP_CASE(G_, E_, ...) \
   { constexpr int G = G_, E = E_; __VA_ARGS__; }
 // CALL with `G` and `E` bound to the lanes and registers of a row of
-// c <= kNarrowMax classes, in a kernel that reads rows and in one that writes
-// them.
+// c <= kNarrowMax classes.
 #define CIGN_GROUP_DISPATCH(c, ...)                            \
   do {                                                          \
     if ((c) <= 8) CIGN_GROUP_CASE(1, 8, __VA_ARGS__)            \
@@ -268,18 +266,24 @@ inline unsigned narrow_grid(int64_t n, int G) {
     else if ((c) <= 192) CIGN_GROUP_CASE(16, 12, __VA_ARGS__)   \
     else CIGN_GROUP_CASE(16, 16, __VA_ARGS__)                   \
   } while (0)
-#define CIGN_GROUP_DISPATCH_WRITE(c, ...)                      \
-  do {                                                          \
-    if ((c) <= 8) CIGN_GROUP_CASE(1, 8, __VA_ARGS__)            \
-    else if ((c) <= 16) CIGN_GROUP_CASE(2, 8, __VA_ARGS__)      \
-    else if ((c) <= 32) CIGN_GROUP_CASE(4, 8, __VA_ARGS__)      \
-    else if ((c) <= 48) CIGN_GROUP_CASE(8, 6, __VA_ARGS__)      \
-    else if ((c) <= 64) CIGN_GROUP_CASE(8, 8, __VA_ARGS__)      \
-    else if ((c) <= 96) CIGN_GROUP_CASE(16, 6, __VA_ARGS__)     \
-    else if ((c) <= 128) CIGN_GROUP_CASE(16, 8, __VA_ARGS__)    \
-    else if ((c) <= 192) CIGN_GROUP_CASE(32, 6, __VA_ARGS__)    \
-    else CIGN_GROUP_CASE(32, 8, __VA_ARGS__)                    \
-  } while (0)
+
+// The rows of a block of a kernel that writes rows: formed in shared memory
+// (at most E kNarrowThreads elements), then written as one piece, 16 bytes per
+// thread.  A block has at least 16 rows, so its piece starts on 16 bytes if the
+// matrix does.
+template <typename T>
+__device__ __forceinline__ void write_piece(T* out, const T* piece, int64_t count) {
+  __syncthreads();
+  constexpr int V = 16 / sizeof(T);
+  if (reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+    const int whole = static_cast<int>(count / V);
+    for (int i = threadIdx.x; i < whole; i += kNarrowThreads)
+      reinterpret_cast<uint4*>(out)[i] = reinterpret_cast<const uint4*>(piece)[i];
+    for (int i = whole * V + threadIdx.x; i < count; i += kNarrowThreads) out[i] = piece[i];
+  } else {
+    for (int i = threadIdx.x; i < count; i += kNarrowThreads) out[i] = piece[i];
+  }
+}
 
 // ---------------------------------------------------------------- ordering
 // Classes are ordered by value, larger first (NaN before everything, as

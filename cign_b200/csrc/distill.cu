@@ -539,35 +539,45 @@ distill_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
                           float temperature, InvT it, int bucket,
                           const float* __restrict__ stats, const float* __restrict__ g_loss,
                           int64_t g_stride, T* __restrict__ grad) {
+  __shared__ __align__(16) T piece[E * kNarrowThreads];
+  constexpr int kRows = kNarrowThreads / G;
   const int lane = threadIdx.x & (G - 1);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kNarrowThreads / G) + threadIdx.x / G;
-  const unsigned mine = group_mask<G>();
-  if (row >= n) return;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kRows;
+  const int64_t row = first + threadIdx.x / G < n ? first + threadIdx.x / G : n - 1;
   const T* x = logits + row * ld;
-  T* out = grad + row * c;
-  float v[E];
+  T* out = piece + threadIdx.x / G * c;
+  const int own = c - lane;
+  F2 v[E / 2];
 #pragma unroll
-  for (int i = 0; i < E; ++i)
-    v[i] = lane + G * i < c ? to_f(x[lane + G * i]) : -INFINITY;
+  for (int i = 0; i < E / 2; ++i) {
+    v[i].x = 2 * i * G < own ? to_f(x[lane + 2 * i * G]) : 0.0f;
+    v[i].y = (2 * i + 1) * G < own ? to_f(x[lane + (2 * i + 1) * G]) : 0.0f;
+  }
   const DistillRow r = load_row(stats + row * kDsStats);
   const float g = g_loss[row * g_stride] * temperature;
   const bool zero = r.kind == 2.0f || g == 0.0f || (r.m == -INFINITY && r.logs == r.logs);
-  const float f = g * r.spread;
+  const F2 f = both(g * r.spread), shift = both(-(r.logs - r.lift));
 #pragma unroll
-  for (int i = 0; i < E; ++i)
-    if (lane + G * i < c)
-      out[lane + G * i] =
-          from_f<T>(zero ? 0.0f : f * expf(scaled(v[i] - r.m, it) - (r.logs - r.lift)));
-  if (zero) return;
-  __syncwarp(mine);  // orders the writes above before those below
-  for (int e = lane; e < te.k; e += G) {
-    const int64_t idx = teacher_index(te, row, e);
-    const float tv = teacher_value(te, row, e);
-    if (idx < 0 || idx >= c || tv == -INFINITY) continue;
-    const double lp = (static_cast<double>(to_f(x[idx])) - r.m) * it.full -
-                      static_cast<double>(r.logs);
-    out[idx] = from_f<T>(g * kept_gradient(te, row, c, idx, tv, lp, r, bucket, it));
+  for (int i = 0; i < E / 2; ++i) {
+    const F2 d = add2(v[i], both(-r.m));
+    F2 a = add2(F2{scaled(d.x, it), scaled(d.y, it)}, shift);
+    a = F2{max_nan(a.x, kExpFloor), max_nan(a.y, kExpFloor)};
+    const F2 w = mul2(exp_neg2<T>(a, kLog2e), f);
+    if (2 * i * G < own) out[lane + 2 * i * G] = from_f<T>(zero ? 0.0f : w.x);
+    if ((2 * i + 1) * G < own) out[lane + (2 * i + 1) * G] = from_f<T>(zero ? 0.0f : w.y);
   }
+  __syncwarp();  // orders the writes above before those below
+  if (!zero) {
+    for (int e = lane; e < te.k; e += G) {
+      const int64_t idx = teacher_index(te, row, e);
+      const float tv = teacher_value(te, row, e);
+      if (idx < 0 || idx >= c || tv == -INFINITY) continue;
+      const double lp = (static_cast<double>(to_f(x[idx])) - r.m) * it.full -
+                        static_cast<double>(r.logs);
+      out[idx] = from_f<T>(g * kept_gradient(te, row, c, idx, tv, lp, r, bucket, it));
+    }
+  }
+  write_piece(grad + first * c, piece, (n - first < kRows ? n - first : kRows) * c);
 }
 
 int ds_check(int64_t n, int64_t c, int32_t x_type, int64_t ld, int32_t k, int32_t value_type,
@@ -640,10 +650,11 @@ int cign_distill_fwd(int64_t n, int64_t c, int32_t x_type, const void* logits, i
                                      : distill_wide_fwd_kernel<T, 8>;
     const size_t smem = ring_bytes<T>(warps == 8 ? 256 : 128) +
                         static_cast<size_t>(words) * 4 * (warps == 1 ? 4 : 1);
-    CIGN_CHECK_CUDA(
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(ring_bytes<T>(256) + kDsMaxClasses / 8 + 64)),
-        "distill_fwd: shared memory");
+    if (smem > 40960)  // more than a kernel has by default, beside its own 5 KB
+      CIGN_CHECK_CUDA(
+          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(ring_bytes<T>(256) + kDsMaxClasses / 8 + 64)),
+          "distill_fwd: shared memory");
     const int split = warps == 8 ? wide_split(n, granules, 256) : 1;
     return launch_cluster(kernel, static_cast<unsigned>(warps == 1 ? (n + 3) / 4 : n * split),
                           warps == 8 ? 256 : 128, smem, split, s, "distill_wide_fwd_kernel", n, c,
@@ -667,7 +678,7 @@ int cign_distill_bwd(int64_t n, int64_t c, int32_t x_type, const void* logits, i
   const Teacher te{values, index, ld_values, ld_index, k, value_type, index_type};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c <= kNarrowMax) {
-    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH_WRITE(c,
+    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c,
         distill_narrow_bwd_kernel<T, G, E><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
             n, static_cast<int>(c), static_cast<const T*>(logits), ld, te, temperature,
             inverse(temperature), tail, stats, grad_loss, grad_loss_stride,

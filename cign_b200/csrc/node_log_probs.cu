@@ -463,11 +463,13 @@ log_probs_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int6
                             const float* __restrict__ entropy, int top_k,
                             const int64_t* __restrict__ top_index, LogProbGrads g,
                             T* __restrict__ grad) {
+  __shared__ __align__(16) T piece[E * kNarrowThreads];
+  constexpr int kRows = kNarrowThreads / G;
   const int lane = threadIdx.x & (G - 1);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kNarrowThreads / G) + threadIdx.x / G;
-  if (row >= n) return;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kRows;
+  const int64_t row = first + threadIdx.x / G < n ? first + threadIdx.x / G : n - 1;
   const T* x = logits + row * ld;
-  T* out = grad + row * c;
+  T* out = piece + threadIdx.x / G * c;
   const int own = c - lane;
   // the logits are asked for before it is known whether any gradient reaches
   // the row: waiting for that costs more than the reads it would save
@@ -491,18 +493,20 @@ log_probs_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int6
     if (2 * i * G < own) out[lane + 2 * i * G] = from_f<T>(none ? 0.0f : w.x);
     if ((2 * i + 1) * G < own) out[lane + (2 * i + 1) * G] = from_f<T>(none ? 0.0f : w.y);
   }
-  if (none) return;
-  // the label and the best classes, by the lanes that wrote them above
-  if (r.y >= 0 && r.y < c && (r.y & (G - 1)) == lane)
-    out[r.y] = from_f<T>(special_grad<T>(g, r, top_index, top_k, row, r.y,
-                                         (to_f(x[r.y]) - st.x) - st.y));
-  if (g.top)
-    for (int i = 0; i < top_k; ++i) {
-      const int64_t j = top_index[row * top_k + i];
-      if ((j & (G - 1)) == lane)
-        out[j] = from_f<T>(special_grad<T>(g, r, top_index, top_k, row, j,
-                                           (to_f(x[j]) - st.x) - st.y));
-    }
+  if (!none) {
+    // the label and the best classes, by the lanes that wrote them above
+    if (r.y >= 0 && r.y < c && (r.y & (G - 1)) == lane)
+      out[r.y] = from_f<T>(special_grad<T>(g, r, top_index, top_k, row, r.y,
+                                           (to_f(x[r.y]) - st.x) - st.y));
+    if (g.top)
+      for (int i = 0; i < top_k; ++i) {
+        const int64_t j = top_index[row * top_k + i];
+        if ((j & (G - 1)) == lane)
+          out[j] = from_f<T>(special_grad<T>(g, r, top_index, top_k, row, j,
+                                             (to_f(x[j]) - st.x) - st.y));
+      }
+  }
+  write_piece(grad + first * c, piece, (n - first < kRows ? n - first : kRows) * c);
 }
 
 // Rows of more than kNarrowMax classes, a warp per share of a row.
@@ -663,7 +667,7 @@ int cign_node_log_probs_bwd(int64_t n, int64_t c, int32_t x_type, const void* lo
                        top_k > 0 ? grad_top : nullptr};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c <= kNarrowMax) {
-    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH_WRITE(c,
+    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c,
         log_probs_narrow_bwd_kernel<T, G, E><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
             n, static_cast<int>(c), static_cast<const T*>(logits), ld, labels, stats, entropy,
             top_k, top_index, g, static_cast<T*>(grad_logits))));
