@@ -176,47 +176,6 @@ struct RowStat {
   float m = -INFINITY, s = -1.0f, t = 0.0f;
 };
 
-__device__ __forceinline__ void stat_add(RowStat& a, float x) {
-  if (x > a.m) {
-    const float f = expf(a.m - x);  // 0 where nothing (or only -inf) was seen
-    const float all = (1.0f + a.s) * f;
-    a.t = f > 0.0f ? fmaf(all, a.m - x, f * a.t) : 0.0f;
-    a.s = all;
-    a.m = x;
-  } else if (x == a.m) {
-    a.s += 1.0f;
-  } else {
-    const float d = x - a.m;  // NaN where x is NaN
-    const float e = expf(d);
-    a.s += e;
-    if (e > 0.0f) a.t = fmaf(e, d, a.t);
-  }
-}
-
-// The union of two disjoint sets of values.
-__device__ __forceinline__ RowStat stat_merge(const RowStat& a, const RowStat& b) {
-  const bool ge = a.m >= b.m;
-  const RowStat hi = ge ? a : b, lo = ge ? b : a;
-  const bool eq = a.m == b.m;
-  const float dm = eq ? 0.0f : lo.m - hi.m;
-  const float f = eq ? 1.0f : expf(dm);
-  const float n = (1.0f + lo.s) * f;
-  RowStat r;
-  r.m = hi.m;
-  r.s = hi.s + n;
-  r.t = hi.t;
-  if (f > 0.0f) r.t += fmaf(n, dm, f * lo.t);
-  return r;
-}
-
-__device__ __forceinline__ RowStat stat_shfl_xor(const RowStat& a, int o) {
-  RowStat b;
-  b.m = __shfl_xor_sync(kFullMask, a.m, o);
-  b.s = __shfl_xor_sync(kFullMask, a.s, o);
-  b.t = __shfl_xor_sync(kFullMask, a.t, o);
-  return b;
-}
-
 // ---------------------------------------------------------------- narrow rows
 // Rows of at most E G classes are held by a group of G lanes (a power of two),
 // class lane + G i in register i < E: a row is read once, and the 32 / G rows

@@ -29,6 +29,7 @@ constexpr int kLnBlockThreads = 512;  // of a block that holds one row; the wide
 constexpr int kLnMaxBlocks = 1776;    // partial sums of the parameter gradients (148 SMs x 12)
 constexpr int kLnWideThreads = 256;
 constexpr int kLnWideWarps = kLnWideThreads / 32;
+constexpr int64_t kLnMaxColumns = 65535ll * kLnWideThreads;  // the grid's second dimension
 
 // How a row lies in a block.  LANES lanes hold it, load i of lane l covering
 // columns (l + LANES i) V ...; LANES == 0: the block's threads, known at launch.
@@ -555,8 +556,9 @@ int ln_check(int64_t n, int64_t d, int32_t x_type, int32_t param_type, const cha
   CIGN_REQUIRE(n >= 0 && d > 0, CIGN_ERR_INVALID_ARGUMENT, "%s: bad sizes", name);
   CIGN_REQUIRE(known_type(x_type) && known_type(param_type), CIGN_ERR_INVALID_ARGUMENT,
                "%s: unknown element type", name);
-  CIGN_REQUIRE(n < (1ll << 31) && d < (1ll << 24), CIGN_ERR_UNSUPPORTED,
-               "%s: at most 2^31 - 1 rows of at most 2^24 - 1 columns", name);
+  CIGN_REQUIRE(n < (1ll << 31) && d <= kLnMaxColumns, CIGN_ERR_UNSUPPORTED,
+               "%s: at most 2^31 - 1 rows of at most %lld columns", name,
+               static_cast<long long>(kLnMaxColumns));
   return CIGN_OK;
 }
 
@@ -601,7 +603,6 @@ int ln_bwd(int64_t n, int64_t d, const T* gy, int64_t ldg, const T* x, int64_t l
       const int64_t chunk = ln_wide_chunk(n);
       sums = static_cast<int>((n + chunk - 1) / chunk);
       const unsigned cols = static_cast<unsigned>((d + kLnWideThreads - 1) / kLnWideThreads);
-      CIGN_REQUIRE(cols < 65536, CIGN_ERR_UNSUPPORTED, "layer_norm_bwd: too many columns");
       layer_norm_wide_param_kernel<T><<<dim3(sums, cols), kLnWideThreads, 0, s>>>(
           n, d, chunk, gy, ldg, x, ldx, mean, rstd, partial);
       CIGN_CHECK_LAUNCH("layer_norm_wide_param_kernel");

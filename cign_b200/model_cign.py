@@ -31,10 +31,14 @@ autograd node (block_node.cign_block), whose backward accumulates the
 gradients of H_norm and H in-kernel instead of with separate add passes.
 Net (model_cign.py:1160-1212): dropout, dual input projection + SiLU, L
 blocks, JK concat, LayerNorm, dropout, classifier.
+Beyond the reference's forward, node_loss (labels and a teacher's kept classes)
+and classify (log probabilities, entropy and best classes of the nodes) end the
+net in node_log_probs and distill_top_logits.
 """
 from __future__ import annotations
 
 import math
+from typing import Optional
 
 import torch
 import torch.nn as nn
@@ -52,6 +56,9 @@ from .block_node import block_node_applies, cign_block
 from .jk_norm import jk_layer_norm, jk_norm_supported
 from .hop_gate import fused_hop_gate
 from .linear import linear
+from .layer_norm import layer_norm
+from .node_log_probs import NodeLogProbs, node_log_probs
+from .distill import distill_top_logits
 
 
 def _glorot_(t: torch.Tensor) -> None:
@@ -244,6 +251,10 @@ class GraphCliffordBlock(nn.Module):
 
 
 class GraphCliffordNet(nn.Module):
+    # True: output rows that jk_layer_norm does not take (wider than 2048 floats) go
+    # through layer_norm instead of torch's; the two differ by float32 roundings
+    native_wide_norm = False
+
     def __init__(self, in_dim: int, hidden_dim: int, out_dim: int, num_layers: int = 4,
                  order_set=(1, 2, 3), dropout: float = 0.28, gat_heads: int = 6,
                  gat_dropout: float = 0.32, init_gamma: float = 0.49, init_input_eta: float = 0.1,
@@ -295,10 +306,48 @@ class GraphCliffordNet(nn.Module):
         if jk_norm_supported(states):  # LayerNorm of the cat, without the cat
             H_out = jk_layer_norm(states, self.output_norm.weight, self.output_norm.bias,
                                   self.output_norm.eps)
+        elif self.native_wide_norm and H.is_cuda:
+            H_out = layer_norm(torch.cat(states, dim=-1), self.output_norm.weight,
+                               self.output_norm.bias, self.output_norm.eps)
         else:
             H_out = self.output_norm(torch.cat(states, dim=-1))
         H_out = F.dropout(H_out, p=self.dropout, training=self.training)
         return _linear_padded(H_out, self.classifier.weight, self.classifier.bias).float()
+
+    def node_loss(self, x: torch.Tensor, graph_operator, labels: torch.Tensor,
+                  teacher=None, distill_weight: float = 0.5, temperature: float = 1.0,
+                  tail: str = "drop", normalizer=None) -> torch.Tensor:
+        """Training loss of the nodes (a scalar): the cross entropy of the labelled nodes,
+        divided by their number, as train_cign.py:2103-2148 forms it on the train mask, and
+        with teacher = (values, index), as distill_top_logits takes them,
+        (1 - distill_weight) * that + distill_weight * distillation / number of nodes.
+
+        labels: int64 [N], negative for nodes without one (those outside of the train mask),
+        so no row is gathered and the call can be captured (GraphedStep).  normalizer: the
+        (labelled, all) node counts of the whole job where x is one rank's part of the nodes."""
+        logits = self(x, graph_operator)
+        log_prob = node_log_probs(logits, labels).log_prob
+        count, nodes = normalizer if normalizer is not None else (
+            (labels >= 0).sum().clamp(min=1), logits.size(0))
+        loss = -log_prob.sum() / count
+        if teacher is None:
+            return loss
+        values, index = teacher
+        distill = distill_top_logits(logits, values, index, temperature, tail).sum() / nodes
+        return (1.0 - distill_weight) * loss + distill_weight * distill
+
+    @torch.no_grad()
+    def classify(self, x: torch.Tensor, graph_operator, labels: Optional[torch.Tensor] = None,
+                 top_k: int = 1) -> NodeLogProbs:
+        """Without dropout: the nodes' log probability of their labels (if given), entropy and
+        top_k best classes.  A teacher's top_log_probs and top_index are what node_loss takes
+        (tail "bucket", temperature 1, or "drop")."""
+        training = self.training
+        self.eval()
+        try:
+            return node_log_probs(self(x, graph_operator), labels, top_k)
+        finally:
+            self.train(training)
 
 
 def build_model(in_dim: int, hidden_dim: int, out_dim: int, num_layers: int = 4,

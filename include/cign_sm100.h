@@ -675,7 +675,7 @@ enum { CIGN_F32 = 0, CIGN_BF16 = 1, CIGN_F16 = 2 };
 
 /* y = (x - mean) * (var + eps)^-1/2 * w + b per row (biased variance).
  * x: [n, d], row stride ldx; w, b: [d] or NULL (1 and 0); mean, rstd: [n]
- * for the backward, or both NULL.  n < 2^31, d < 2^24. */
+ * for the backward, or both NULL.  n < 2^31, d <= 16776960. */
 CIGN_API int cign_layer_norm_fwd(int64_t n, int64_t d, int32_t x_type, int32_t param_type,
                         const void* x, int64_t ldx, const void* w, const void* b, float eps,
                         void* y, float* mean, float* rstd, cign_stream_t stream);
@@ -697,6 +697,7 @@ CIGN_API int cign_layer_norm_bwd(int64_t n, int64_t d, int32_t x_type, int32_t p
  *   labels: int64 [n]; negative = no label (log_prob 0, no gradient);
  *     >= c = log_prob NaN.  labels and log_prob may both be NULL.
  *   entropy, stats ([n, 2], 8-byte aligned, for the backward) may be NULL.
+ *   n < 2^31, c <= 2^31 - 16.
  *   A class with logit -inf has probability 0.  A row of -inf only has
  *     log_prob -inf (0 without a label), entropy 0 and gradient 0; a row with
  *     a NaN or +inf gives NaN. */
