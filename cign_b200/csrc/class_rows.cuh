@@ -182,9 +182,12 @@ struct RowStat {
 // of a warp are neighbours.  A row costs a warp E of its steps, the sums over
 // the group, one logarithm and what is read once per row, so few lanes and many
 // classes per lane are cheapest (2.45M x 47 float32 forward: 132 us with 4
-// lanes, 177 with 8, 159 with 2, whose loads are too scattered).
+// lanes, 177 with 8, 159 with 2, whose loads are too scattered).  Up to 512
+// classes this beats a warp that streams the row (200000 rows of 512: forward
+// 102 us and 143 in float32, 125 and 204 in bf16; of 1000: 209 and 199, 338 and
+// 207).
 constexpr int kNarrowThreads = 256;
-constexpr int64_t kNarrowMax = 256;
+constexpr int64_t kNarrowMax = 512;
 
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
@@ -223,12 +226,14 @@ inline unsigned narrow_grid(int64_t n, int G) {
     else if ((c) <= 96) CIGN_GROUP_CASE(8, 12, __VA_ARGS__)     \
     else if ((c) <= 128) CIGN_GROUP_CASE(8, 16, __VA_ARGS__)    \
     else if ((c) <= 192) CIGN_GROUP_CASE(16, 12, __VA_ARGS__)   \
-    else CIGN_GROUP_CASE(16, 16, __VA_ARGS__)                   \
+    else if ((c) <= 256) CIGN_GROUP_CASE(16, 16, __VA_ARGS__)   \
+    else if ((c) <= 384) CIGN_GROUP_CASE(32, 12, __VA_ARGS__)   \
+    else CIGN_GROUP_CASE(32, 16, __VA_ARGS__)                   \
   } while (0)
 
 // The rows of a block of a kernel that writes rows: formed in shared memory
 // (at most E kNarrowThreads elements), then written as one piece, 16 bytes per
-// thread.  A block has at least 16 rows, so its piece starts on 16 bytes if the
+// thread.  A block has a multiple of 8 rows, so its piece starts on 16 bytes if the
 // matrix does.
 template <typename T>
 __device__ __forceinline__ void write_piece(T* out, const T* piece, int64_t count) {
@@ -665,11 +670,14 @@ int launch_cluster(void (*kernel)(Params...), unsigned grid, int threads, size_t
 // Warps of a team.  What a row costs each warp at its ends (the maxima, the
 // sums, the barriers) is as much as about eight rounds of loads, so a team has
 // no more warps than it takes to fill the device: single warps want two rows
-// per resident warp to even out, teams of four one row per resident team.
+// per resident warp to even out, or rows of at most 16 loads per lane (1500
+// rows of 1000 bf16: 5 us, 10 with teams of four), teams of four one row per
+// resident team (777 rows of 10007 fp16: 14 us, 21 with teams of eight).
 inline int wide_warps(int64_t n, int64_t granules) {
   const int64_t sms = sm_count();
   if (n >= 48 * sms || granules < 64) return 1;
-  return n >= 4 * sms || granules < 256 ? 4 : 8;
+  if (n >= 4 * sms) return granules <= 512 ? 1 : 4;
+  return granules < 256 ? 4 : 8;
 }
 
 // Blocks that share a row of `granules` where there are too few rows to fill
