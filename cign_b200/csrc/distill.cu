@@ -356,6 +356,8 @@ distill_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
                         float temperature, InvT it, int bucket, const float* __restrict__ stats,
                         const float* __restrict__ g_loss, int64_t g_stride, int split, int warps,
                         T* __restrict__ grad) {
+  static_assert(kDsMaxKept <= 256, "entries are bytes");
+  __shared__ uint8_t entries[kMapThreads / 32][kDsMaxKept];
   const MapPlace at(warps);
   if (at.row >= n || at.rank >= split) return;  // a whole warp
   const int64_t row = at.row;
@@ -394,15 +396,26 @@ distill_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
       }
     });
   }
-  __syncwarp();  // orders the writes above before those below
-  for (int e = threadIdx.x & 31; e < te.k; e += 32) {
+  // the kept classes of this share, gathered first so that few lanes' worth of
+  // arithmetic in 64 bits is issued once
+  uint8_t* mine = entries[threadIdx.x >> 5];
+  const int lane = threadIdx.x & 31;
+  int count = 0;
+  for (int e0 = 0; e0 < te.k; e0 += 32) {
+    const bool here = e0 + lane < te.k && share.holds(teacher_index(te, row, e0 + lane)) &&
+                      teacher_value(te, row, e0 + lane) != -INFINITY;
+    const unsigned who = __ballot_sync(kFullMask, here);
+    if (here) mine[count + __popc(who & ((1u << lane) - 1u))] = static_cast<uint8_t>(e0 + lane);
+    count += __popc(who);
+  }
+  __syncwarp();  // also orders the writes of the gradient above before those below
+  for (int i = lane; i < count; i += 32) {
+    const int e = mine[i];
     const int64_t idx = teacher_index(te, row, e);
-    if (!share.holds(idx)) continue;
-    const float v = teacher_value(te, row, e);
-    if (v == -INFINITY) continue;
     const double lp = (static_cast<double>(to_f(x[idx])) - r.m) * it.full -
                       static_cast<double>(r.logs);
-    out[idx] = from_f<T>(g * kept_gradient(te, row, c, idx, v, lp, r, bucket, it));
+    out[idx] = from_f<T>(
+        g * kept_gradient(te, row, c, idx, teacher_value(te, row, e), lp, r, bucket, it));
   }
 }
 
