@@ -435,30 +435,50 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
   const int64_t row = live ? at : n - 1;  // the last warp's idle groups follow along
   const T* x = logits + row * ld;
   uint32_t* bits = all_bits + threadIdx.x / G * kWords;
-  float v[E];
+  const int own = c - lane;
+  const float scale = kLog2e * it.hi;
+  F2 v[E / 2];
 #pragma unroll
-  for (int i = 0; i < E; ++i)
-    v[i] = lane + G * i < c ? to_f(x[lane + G * i]) : -INFINITY;
+  for (int i = 0; i < E / 2; ++i) {
+    v[i].x = 2 * i * G < own ? to_f(x[lane + 2 * i * G]) : -INFINITY;
+    v[i].y = (2 * i + 1) * G < own ? to_f(x[lane + (2 * i + 1) * G]) : -INFINITY;
+  }
+  // The lane's entries, the first two of them held: class (-1: absent, -2: wrong),
+  // value and logit.
+  struct Entry {
+    int idx;
+    float v, x;
+  };
+  const auto load_entry = [&](int e) {
+    Entry t{-1, -INFINITY, 0.0f};
+    if (e < te.k) {
+      const int64_t idx = teacher_index(te, row, e);
+      t.v = teacher_value(te, row, e);
+      t.idx = idx < 0 || t.v == -INFINITY ? -1 : idx >= c ? -2 : static_cast<int>(idx);
+      if (t.idx >= 0) t.x = to_f(x[t.idx]);
+    }
+    return t;
+  };
+  const Entry first_entry = load_entry(lane), second_entry = load_entry(lane + G);
+  const auto entry = [&](int e) {
+    return e == lane ? first_entry : e == lane + G ? second_entry : load_entry(e);
+  };
   for (int i = lane; i < kWords; i += G) bits[i] = 0;
   __syncwarp();
-  // teacher: kept classes, maximum, log sum, sum of probabilities
+  // teacher: kept classes, maximum
   bool bad = false, dup = false;
   float tmax = -INFINITY, nan = 0.0f;
   float distinct = 0.0f;
   for (int e = lane; e < te.k; e += G) {
-    const int64_t idx = teacher_index(te, row, e);
-    const float tv = teacher_value(te, row, e);
-    if (idx < 0 || tv == -INFINITY) continue;
-    if (idx >= c) {
-      bad = true;
-      continue;
-    }
-    const uint32_t bit = 1u << (idx & 31);
-    const bool first = !(atomicOr(bits + (idx >> 5), bit) & bit);
+    const Entry t = entry(e);
+    bad |= t.idx == -2;
+    if (t.idx < 0) continue;
+    const uint32_t bit = 1u << (t.idx & 31);
+    const bool first = !(atomicOr(bits + (t.idx >> 5), bit) & bit);
     dup |= !first;
     distinct += first ? 1.0f : 0.0f;
-    tmax = fmaxf(tmax, tv);
-    if (tv != tv) nan = tv;
+    tmax = fmaxf(tmax, t.v);
+    if (t.v != t.v) nan = t.v;
   }
   const unsigned mine = group_mask<G>();
   bad = __ballot_sync(kFullMask, bad) & mine;
@@ -467,45 +487,47 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
   distinct = group_sum<G>(distinct);
   DistillRow r;
   r.tmax = group_max<G>(tmax);
+  // log sum, or the sum of probabilities
   float tsum = 0.0f, tcnt = 0.0f;
   double mass = 0.0;
   for (int e = lane; e < te.k; e += G) {
-    const int64_t idx = teacher_index(te, row, e);
-    const float tv = teacher_value(te, row, e);
-    if (idx < 0 || idx >= c || tv == -INFINITY) continue;
-    if (bucket) mass += exp(static_cast<double>(tv));
-    else if (tv == r.tmax) tcnt += 1.0f;
-    else tsum += expf(scaled(tv - r.tmax, it));
+    const Entry t = entry(e);
+    if (t.idx < 0) continue;
+    if (bucket) mass += exp(static_cast<double>(t.v));
+    else if (t.v == r.tmax) tcnt += 1.0f;
+    else tsum += expf(scaled(t.v - r.tmax, it));
   }
   r.tlog = log1pf(group_sum<G>(tsum + nan) + (group_sum<G>(tcnt) - 1.0f));
-  // student: the sums over the classes that are not kept and over the kept ones
-  float m = v[0];
-#pragma unroll
-  for (int i = 1; i < E; ++i) m = fmaxf(m, v[i]);
-  m = group_max<G>(m);
-  if (m != m) m = -INFINITY;
-  float m_rest = -INFINITY;
+  // student: the sums over the classes that are not kept and over the kept ones,
+  // relative to their own maxima: that of the rest may be far below the row's
+  float m = -INFINITY, m_rest = -INFINITY;
   uint32_t kept_here = 0;
 #pragma unroll
   for (int i = 0; i < E; ++i) {
+    const float vi = i % 2 == 0 ? v[i / 2].x : v[i / 2].y;
     const int j = lane + G * i;
+    m = fmaxf(m, vi);
     if ((bits[j >> 5] >> (j & 31)) & 1u) kept_here |= 1u << i;
-    else m_rest = fmaxf(m_rest, v[i]);
+    else m_rest = fmaxf(m_rest, vi);
   }
+  m = group_max<G>(m);
   m_rest = group_max<G>(m_rest);
-  // relative to their own maxima: that of the rest may be far below the row's
   float s_rest = 0.0f, c_rest = 0.0f, s_kept = 0.0f, c_kept = 0.0f;
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const bool kept = (kept_here >> i) & 1u;
-    const float ref = kept ? m : m_rest;
-    const bool top = v[i] == ref && lane + G * i < c;
-    const float d = v[i] - ref;
-    const float e = v[i] == ref ? 0.0f : expf(scaled(d, it));
-    s_kept += kept ? e : 0.0f;
-    c_kept += kept && top ? 1.0f : 0.0f;
-    s_rest += kept ? 0.0f : e;
-    c_rest += !kept && top ? 1.0f : 0.0f;
+  for (int i = 0; i < E / 2; ++i) {
+    const bool kx = (kept_here >> (2 * i)) & 1u, ky = (kept_here >> (2 * i + 1)) & 1u;
+    const float rx = kx ? m : m_rest, ry = ky ? m : m_rest;
+    const bool px = v[i].x == rx, py = v[i].y == ry;  // a maximum's e^0 is counted, not added
+    F2 d = add2(v[i], F2{-rx, -ry});
+    d = F2{px ? 0.0f : max_nan(d.x, kExpFloor), py ? 0.0f : max_nan(d.y, kExpFloor)};
+    const F2 e = exp_neg2<T>(d, scale);
+    const float ex = px ? 0.0f : e.x, ey = py ? 0.0f : e.y;
+    const float ox = px && 2 * i * G < own ? 1.0f : 0.0f;
+    const float oy = py && (2 * i + 1) * G < own ? 1.0f : 0.0f;
+    s_kept += (kx ? ex : 0.0f) + (ky ? ey : 0.0f);
+    c_kept += (kx ? ox : 0.0f) + (ky ? oy : 0.0f);
+    s_rest += (kx ? 0.0f : ex) + (ky ? 0.0f : ey);
+    c_rest += (kx ? 0.0f : ox) + (ky ? 0.0f : oy);
   }
   s_rest = group_sum<G>(s_rest);
   c_rest = group_sum<G>(c_rest);
@@ -526,16 +548,14 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
       bucket ? rest_mass(mass, distinct == static_cast<float>(c), r.w1) : (r.w1 = 0.0f);
   float sum = 0.0f;
   for (int e = lane; e < te.k; e += G) {
-    const int64_t idx = teacher_index(te, row, e);
-    const float tv = teacher_value(te, row, e);
-    if (idx < 0 || idx >= c || tv == -INFINITY) continue;
+    const Entry t = entry(e);
+    if (t.idx < 0) continue;
     bool first = true;
     if (dup)  // the first of equal entries by its place
       for (int q = 0; q < e && first; ++q)
-        first = teacher_index(te, row, q) != idx || teacher_value(te, row, q) == -INFINITY;
-    const double lq = log_q(tv, r, bucket, it);
-    const double lp = (static_cast<double>(to_f(x[idx])) - m) * it.full -
-                      static_cast<double>(r.logs);
+        first = teacher_index(te, row, q) != t.idx || teacher_value(te, row, q) == -INFINITY;
+    const double lq = log_q(t.v, r, bucket, it);
+    const double lp = (static_cast<double>(t.x) - m) * it.full - static_cast<double>(r.logs);
     const float q = expf(static_cast<float>(lq));
     const float d = static_cast<float>(lq - lp);
     sum += first ? divergence_term(q, d) : q * (d - 1.0f);
