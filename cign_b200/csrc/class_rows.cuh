@@ -131,14 +131,15 @@ __device__ __forceinline__ float exp2_hw(float t) {
 }
 
 // e^(d / T) of two values d <= 0 by the hardware's 2^x, `scale` = log2(e) / T;
-// below 2^-126 zero.  d must be finite (callers raise it to kExpFloor).  For
-// 16-bit logits the argument d scale is rounded to float32, which leaves a
+// below 2^-126 zero.  d must be finite (callers raise it to exp_floor(scale),
+// where the result is 0).  For 16-bit logits the argument d scale is rounded to float32, which leaves a
 // relative error of about |d| 2^-23: the terms of a softmax sum weigh e^d, and
 // a gradient is rounded to 16 bits.  For float32 logits what the rounding
 // drops is put back, so that the small probabilities beside a sure class keep
 // their digits.
-constexpr float kExpFloor = -1e4f;
 constexpr float kLog2e = 1.44269504f;
+__device__ __forceinline__ float exp_floor(float scale) { return -160.0f / scale; }
+constexpr float kExpFloor = -160.0f / kLog2e;  // T = 1
 template <typename T>
 __device__ __forceinline__ F2 exp_neg2(F2 d, float scale) {
   const F2 t = mul2(d, both(scale));
@@ -538,9 +539,11 @@ struct Stream {
   static constexpr bool kOneStep = sizeof(T) == 2;
   float m, ref, cnt;  // ref = m but where m scale would overflow to -inf
   float shift;        // kOneStep: ref scale, rounded
+  float floor;        // of x - m
   F2 s[2], u[2];      // two chains each; u: kOneStep: sum of e times the argument; else t
   __device__ __forceinline__ Stream(float start, float scale) : cnt(0.0f) {
     s[0] = s[1] = u[0] = u[1] = both(0.0f);
+    floor = exp_floor(scale);
     set(start, scale);
   }
   __device__ __forceinline__ void set(float to, float scale) {
@@ -554,13 +557,13 @@ struct Stream {
     for (int i = 0; i < N; ++i) {
       if constexpr (kOneStep) {
         F2 a = fma2(v[i], both(scale), both(-shift));
-        if (CLAMP) a = F2{max_nan(a.x, kExpFloor), max_nan(a.y, kExpFloor)};
+        if (CLAMP) a = F2{max_nan(a.x, -160.0f), max_nan(a.y, -160.0f)};
         const F2 e{exp2_hw(a.x), exp2_hw(a.y)};
         s[i % 2] = add2(s[i % 2], e);
         if (ENTROPY) u[i % 2] = fma2(e, a, u[i % 2]);
       } else {
         F2 d = add2(v[i], both(-ref));
-        if (CLAMP) d = F2{max_nan(d.x, kExpFloor), max_nan(d.y, kExpFloor)};
+        if (CLAMP) d = F2{max_nan(d.x, floor), max_nan(d.y, floor)};
         const F2 e = exp_neg2<T>(d, scale);
         s[i % 2] = add2(s[i % 2], e);
         if (ENTROPY) u[i % 2] = fma2(e, d, u[i % 2]);
@@ -579,7 +582,7 @@ struct Stream {
       }
     }
     // -inf would make 0 times inf of u; the arithmetic of finite values needs no floor
-    if (min_of(v) - ref < kExpFloor) sum<true>(v, scale);
+    if (min_of(v) - ref < floor) sum<true>(v, scale);
     else sum<false>(v, scale);
   }
   __device__ __forceinline__ static float all(const F2 (&p)[2]) {
@@ -592,12 +595,13 @@ struct Stream {
     const float r = left(scale);
     return kOneStep ? exp2_hw(r) * fmaf(r, all(s), all(u)) / scale : all(u);
   }
-  __device__ __forceinline__ float left(float scale) const {  // of rounding ref scale
-    const float r = -fmaf(ref, scale, -shift);
-    return fabsf(shift) < 1e30f ? r : 0.0f;
+  // What rounding ref scale has left.  Where that is large, a 16-bit logit's
+  // next lower value is 2^-11 of it and more below m: every term is 0.
+  __device__ __forceinline__ float left(float scale) const {
+    return fabsf(shift) < 4194304.0f ? -fmaf(ref, scale, -shift) : 0.0f;
   }
   __device__ __forceinline__ void raise(float to, float scale) {
-    const float d = max_nan(m - to, kExpFloor);
+    const float d = max_nan(m - to, floor);
     const float f = exp_neg2<T>(both(d), scale).x;
     float n = (total_s(scale) + cnt) * f;
     float w = ENTROPY ? fmaf(n, d, f * total_t(scale)) : 0.0f;
@@ -626,7 +630,7 @@ __device__ __forceinline__ Sums join_warp(const Sums& a, float scale) {
   Sums r;
   r.m = warp_max(a.m);
   const bool top = a.m == r.m;
-  const float d = max_nan(a.m - r.m, kExpFloor);
+  const float d = max_nan(a.m - r.m, exp_floor(scale));
   const float f = top ? 1.0f : exp_neg2<T>(both(d), scale).x;
   const float n = top ? a.s : (a.s + a.cnt) * f;
   r.s = warp_sum(n);

@@ -374,10 +374,11 @@ distill_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
     return;
   }
   const F2 f = both(g * r.spread);
-  if (sizeof(T) == 2 && r.m > -1e30f && r.m < 1e30f) {
-    // one operation on the logit (its rounding is far below the gradient's)
-    const F2 scale = both(kLog2e * it.hi);
-    const F2 shift = both(-(r.m * it.hi + (r.logs - r.lift)) * kLog2e);
+  const F2 scale = both(kLog2e * it.hi);
+  const F2 shift = both(-(r.m * it.hi + (r.logs - r.lift)) * kLog2e);
+  if (sizeof(T) == 2 && !(fabsf(shift.x) > 8192.0f)) {
+    // one operation on the logit; the rounding of the shift, 2^-11 log 2 at
+    // most, is below the gradient's
     share.template run<true>([&](auto& v) {
 #pragma unroll
       for (auto& p : v) {
@@ -436,7 +437,7 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
   const T* x = logits + row * ld;
   uint32_t* bits = all_bits + threadIdx.x / G * kWords;
   const int own = c - lane;
-  const float scale = kLog2e * it.hi;
+  const float scale = kLog2e * it.hi, floor = exp_floor(scale);
   F2 v[E / 2];
 #pragma unroll
   for (int i = 0; i < E / 2; ++i) {
@@ -519,7 +520,7 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
     const float rx = kx ? m : m_rest, ry = ky ? m : m_rest;
     const bool px = v[i].x == rx, py = v[i].y == ry;  // a maximum's e^0 is counted, not added
     F2 d = add2(v[i], F2{-rx, -ry});
-    d = F2{px ? 0.0f : max_nan(d.x, kExpFloor), py ? 0.0f : max_nan(d.y, kExpFloor)};
+    d = F2{px ? 0.0f : max_nan(d.x, floor), py ? 0.0f : max_nan(d.y, floor)};
     const F2 e = exp_neg2<T>(d, scale);
     const float ex = px ? 0.0f : e.x, ey = py ? 0.0f : e.y;
     const float ox = px && 2 * i * G < own ? 1.0f : 0.0f;
@@ -625,8 +626,8 @@ int ds_check(int64_t n, int64_t c, int32_t x_type, int64_t ld, int32_t k, int32_
   CIGN_REQUIRE(k >= 1, CIGN_ERR_INVALID_ARGUMENT, "%s: no kept classes", name);
   CIGN_REQUIRE(ld_values >= k && ld_index >= k, CIGN_ERR_INVALID_ARGUMENT,
                "%s: row stride of the teacher's entries below their number", name);
-  CIGN_REQUIRE(temperature > 0.0f && temperature <= 3.402823466e38f, CIGN_ERR_INVALID_ARGUMENT,
-               "%s: temperature must be positive and finite", name);
+  CIGN_REQUIRE(temperature >= 1e-3f && temperature <= 1e6f, CIGN_ERR_INVALID_ARGUMENT,
+               "%s: temperature must be between 1e-3 and 1e6", name);
   CIGN_REQUIRE(tail == 0 || tail == 1, CIGN_ERR_INVALID_ARGUMENT,
                "%s: tail must be 0 (drop) or 1 (bucket)", name);
   CIGN_REQUIRE(k <= kDsMaxKept, CIGN_ERR_UNSUPPORTED, "%s: at most %d kept classes", name,

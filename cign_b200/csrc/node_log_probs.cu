@@ -535,9 +535,10 @@ log_probs_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
   }
   // -p G - gh p (lp + H) = p (A + B lp)
   const F2 A = both(-(r.all + r.gh * r.H)), B = both(-r.gh);
-  if (sizeof(T) == 2 && st.x > -1e30f && st.x < 1e30f) {
-    // e^lp by one operation on the logit (its rounding is far below the gradient's)
-    const F2 scale = both(kLog2e), shift = both(-(st.x + st.y) * kLog2e);
+  const F2 scale = both(kLog2e), shift = both(-(st.x + st.y) * kLog2e);
+  if (sizeof(T) == 2 && !(fabsf(shift.x) > 8192.0f)) {
+    // e^lp by one operation on the logit; the rounding of the shift, 2^-11 log 2
+    // at most, is below the gradient's
     const F2 B2 = both(B.x * 0.693147181f);
     if (r.gh == 0.0f) {
       share.template run<true>([&](auto& v) {
@@ -552,7 +553,7 @@ log_probs_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
 #pragma unroll
         for (auto& p : v) {
           F2 a = fma2(p, scale, shift);
-          a = F2{max_nan(a.x, kExpFloor), max_nan(a.y, kExpFloor)};  // -inf: p = 0
+          a = F2{max_nan(a.x, -160.0f), max_nan(a.y, -160.0f)};  // -inf: p = 0
           p = mul2(F2{exp2_hw(a.x), exp2_hw(a.y)}, fma2(B2, a, A));
         }
       });

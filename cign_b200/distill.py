@@ -59,7 +59,8 @@ def distill_top_logits(logits: torch.Tensor, teacher_values: torch.Tensor,
     """temperature^2 * KL(teacher || student) per node, float32 [N].
 
     logits: [N, C], CUDA float32, bfloat16 or float16 (rows may lie in a wider
-    buffer, C <= 2^20); the student is softmax(logits / temperature).
+    buffer, C <= 2^20); the student is softmax(logits / temperature), temperature
+    between 1e-3 and 1e6.
     teacher_values, teacher_index: [N, K] (K <= 256; float32, bfloat16 or
     float16; int32 or int64), the kept classes in any order.  An entry with a
     negative index or the value -inf is absent; an index >= C makes its row
@@ -91,8 +92,8 @@ def distill_top_logits(logits: torch.Tensor, teacher_values: torch.Tensor,
     if teacher_values.requires_grad:
         raise ValueError("teacher_values are constants here: detach them")
     temperature = float(temperature)
-    if not (0.0 < temperature < float("inf")):
-        raise ValueError("temperature must be positive and finite")
+    if not (1e-3 <= temperature <= 1e6):
+        raise ValueError(f"temperature must be between 1e-3 and 1e6, got {temperature}")
     if tail not in _TAILS:
         raise ValueError(f"tail must be 'drop' or 'bucket', got {tail!r}")
     if torch.is_grad_enabled() and logits.requires_grad:

@@ -727,7 +727,7 @@ CIGN_API int cign_node_log_probs_bwd(int64_t n, int64_t c, int32_t x_type, const
  *     probability of all classes that are not kept.
  *   A row without entries has loss 0 and gradient 0.
  *   loss [n]; stats [n, 8] (16-byte aligned, for the backward) or NULL.
- *   c <= 2^20. */
+ *   n < 2^31, c <= 2^20, 1e-3 <= temperature <= 1e6. */
 CIGN_API int cign_distill_fwd(int64_t n, int64_t c, int32_t x_type, const void* logits, int64_t ld,
                      int32_t k, int32_t value_type, const void* values, int64_t ld_values,
                      int32_t index_type, const void* index, int64_t ld_index, float temperature,

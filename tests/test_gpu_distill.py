@@ -61,8 +61,8 @@ def reference(x, v, i, temp, tail, g):
     W = mass + r
     grad = W[:, None] * p - target - spread
     grad = grad * temp * g[:, None]
-    # k roundings on the way of each probability; those of the log sum cancel in the loss to first order,
-    # what is left is weighted with |p - q|, which is at most sqrt(2 KL) in all (Pinsker)
+    # k roundings on the way of each probability (and below 2^-126, the smallest normal number, an exponential
+    # is 0, so a gradient is off by up to that); those of the log sum cancel in the loss to first order, what is left is weighted with |p - q|, which is at most sqrt(2 KL) in all (Pinsker)
     d = torch.where(torch.isfinite(z), z.amax(1, keepdim=True) - z, 0.0)
     ku = 2 * (sum_ulps(c) + sum_ulps(i.size(1)) + 16) * U
     dmax = (p * (1 + d)).sum(1) + 1
@@ -73,7 +73,7 @@ def reference(x, v, i, temp, tail, g):
     # leave terms q (d - 1) of either sign, whose roundings count with their magnitudes
     twice = (kept.sum(1) < here.sum(1))
     tloss = tloss + torch.where(twice, temp ** 2 * ku * torch.where(q > 0, q * (1 + delta.abs()), 0.0).sum(1), 0.0)
-    tgrad = temp * g.abs()[:, None] * (ku * (dmax[:, None] + d) * (p + spread)
+    tgrad = temp * g.abs()[:, None] * (2.0 ** -125 + ku * (dmax[:, None] + d) * (p + spread)
                                        + ku * (target + (W[:, None] * p - target).abs()))
     return temp ** 2 * loss, grad, tloss, tgrad
 
@@ -257,6 +257,35 @@ def test_broadcast_gradient_and_constant_teacher(cuda):
         distill_top_logits(x, v.requires_grad_(), i)
 
 
+@pytest.mark.parametrize("tail", ["drop", "bucket"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c", [6, 60, 900, 20000])
+@pytest.mark.parametrize("temp", [0.02, 500.0, 20000.0])
+def test_far_temperatures_and_masks(cuda, c, temp, dtype, tail):
+    """Masked classes have no probability at any temperature; far logits come near at a high one."""
+    def edit(x, v, i):
+        kept = torch.zeros_like(x, dtype=torch.bool).scatter_(1, i.long(), True)
+        x[0] = torch.where(kept[0], x[0], torch.full_like(x[0], -INF))  # all but the kept ones
+        x[1, :c // 2] = torch.where(kept[1, :c // 2], x[1, :c // 2], torch.full_like(x[1, :c // 2], -INF))
+        x[2] *= 300.0
+        if tail == "bucket":
+            v[0] += 0.2 / 3  # nothing to place on masked classes
+            v[0] -= torch.logsumexp(v[0], 0)
+    if tail == "bucket":
+        # row 0 has no rest: r is 1 - sum q, a rounding; only the loss of a rest that exists is compared
+        x, v, i, gen = make(cuda, 4, c, 3, dtype, tail, temp)
+        edit(x, v, i)
+        want, wgrad, tl, tg = reference(x[1:], v[1:], i[1:], temp, tail, torch.ones(3, device=cuda))
+        x.requires_grad_()
+        loss = distill_top_logits(x, v, i, temp, tail)
+        (grad,) = torch.autograd.grad(loss[1:].sum(), x)
+        check(loss[1:], want, tl, "loss")
+        check(grad[1:], wgrad, tg, "grad")
+        assert not grad[0].any()
+    else:
+        run_case(cuda, 4, c, 3, dtype, tail, temp, edit=edit)
+
+
 def test_empty(cuda):
     x = torch.zeros(0, 9, device=cuda, requires_grad=True)
     loss = distill_top_logits(x, torch.zeros(0, 2, device=cuda), torch.zeros(0, 2, dtype=torch.int32, device=cuda))
@@ -305,7 +334,7 @@ def test_refusals(cuda):
                         ((x, v, i.float()), TypeError), ((x, v.cpu(), i), TypeError), ((x, v, i[:, :5]), ValueError),
                         ((x, v[:3], i[:3]), ValueError), ((x, v[:, :0], i[:, :0]), ValueError), ((x[0], v, i), ValueError),
                         ((x, v, i, 0.0), ValueError), ((x, v, i, float("inf")), ValueError), ((x, v, i, float("nan")), ValueError),
-                        ((x, v, i, 1.0, "rest"), ValueError),
+                        ((x, v, i, 1e-4), ValueError), ((x, v, i, 2e6), ValueError), ((x, v, i, 1.0, "rest"), ValueError),
                         ((x, v[:, :1].expand(4, 257), i[:, :1].expand(4, 257)), ValueError)):
         with pytest.raises(error):
             distill_top_logits(*args)

@@ -173,6 +173,33 @@ def test_masked_rows_and_lowest_values(cuda, c, dtype):
     assert torch.isfinite(grad).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c", [6, 90, 900, 20000])
+def test_far_logits(cuda, c, dtype):
+    """Rows far from 0: all equal, two values a step apart, a mask of -1e4 and a spread of thousands."""
+    big = 3.0e4 if dtype == torch.float16 else 1.0e20
+    x = torch.full((6, c), -big, device=cuda, dtype=dtype)
+    x[1] = big
+    x[2] = torch.where(torch.arange(c, device=cuda) % 3 == 0, 2048.0, 2040.0)
+    x[3] = torch.where(torch.arange(c, device=cuda) % 2 == 0, -1e4, 1.0)
+    x[4] = torch.linspace(-3e3, 3e3, c, device=cuda)
+    x[5] = torch.where(torch.arange(c, device=cuda) % 3 == 0, 30000.0, 29968.0)
+    labels = torch.tensor([0, 1, 3, 1, c - 1, 0], device=cuda)
+    x = x.to(dtype).requires_grad_()
+    logp, p, lp, H = reference(x, labels)
+    out = node_log_probs(x, labels, 2)
+    k = 2 * (sum_ulps(c) + 16) * U
+    check(out.log_prob, lp, k * (1 + lp.abs()), "log_prob")
+    check(out.entropy, H, k * (1 + H), "entropy")
+    g = torch.ones(6, device=cuda)
+    (grad,) = torch.autograd.grad((out.log_prob, out.entropy), x, (g, g))
+    plogp = torch.where(p > 0, p * (logp + H[:, None]), 0.0)
+    want = torch.zeros_like(p).scatter_(1, labels[:, None], 1.0) - p - plogp
+    # 16 bits: the exponent's shift is rounded to 2^-11 at most, below half a step of the gradient
+    room = (k + (2.0 ** -11 if dtype != torch.float32 else 0.0)) * (p * (1 + torch.where(p > 0, (logp + H[:, None]).abs(), 0.0)))
+    check(grad, want, room + 8 * U * (1 - p).clamp(min=0) * (want > 0), "grad")
+
+
 @pytest.mark.parametrize("c", [4, 90, 3000, 20001])
 def test_nan_infinity_and_wrong_labels(cuda, c):
     x = torch.randn(6, c, device=cuda)
