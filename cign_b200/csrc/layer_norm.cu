@@ -184,6 +184,9 @@ layer_norm_fwd_kernel(int64_t n, int d, const T* __restrict__ x, int64_t ldx,
 }
 
 // partial: [gridDim.x, 2, d] sums of g xh and g over the block's rows, or NULL.
+// Rows that take more than kLnBlockThreads threads (BLOCK 2) leave these to a
+// kernel of their own: with them a thread would need more than the 64 registers
+// that a block of 1024 has.
 template <typename T, int V, int NV, int SLACK, int LANES, int BLOCK>
 __global__ void __launch_bounds__(BLOCK ? BLOCK * kLnBlockThreads : kLnGroupThreads)
 layer_norm_bwd_kernel(int64_t n, int d, const T* __restrict__ gy, int64_t ldg,
@@ -217,12 +220,20 @@ layer_norm_bwd_kernel(int64_t n, int d, const T* __restrict__ gy, int64_t ldg,
   const T* xp = x + loaded * ldx + at_lane * V;
   const T* gp = gy + loaded * ldg + at_lane * V;
   T* op = gx + row * d + lane * V;
+  // (the widest rows have no registers for the next one)
+  constexpr bool kAhead = BLOCK != 2;
   Pack<T, V> xn[NV], gn[NV];
-  load_row<T, V, NV, SLACK>(xn, xp, loads, lanes);
-  load_row<T, V, NV, SLACK>(gn, gp, loads, lanes);
-  float mu_next = mean[loaded], rs_next = rstd[loaded];
+  float mu_next = 0.0f, rs_next = 0.0f;
+  const auto ask = [&]() {
+    load_row<T, V, NV, SLACK>(xn, xp, loads, lanes);
+    load_row<T, V, NV, SLACK>(gn, gp, loads, lanes);
+    mu_next = mean[loaded];
+    rs_next = rstd[loaded];
+  };
+  if (kAhead) ask();
   for (; row - L::group() < n; row += step, op += step * d) {
     const bool live = BLOCK != 0 || row < n;
+    if (!kAhead) ask();
     const float mu = mu_next, rs = rs_next;
     // with e = x - mean and h = g rstd: u = g w, u xh = rstd u e, g xh = h e and
     // grad_x = h w - rstd <u> - e rstd^3 <u e>.  Loads behind the last repeat it:
@@ -239,7 +250,7 @@ layer_norm_bwd_kernel(int64_t n, int d, const T* __restrict__ gy, int64_t ldg,
         const float u = g * wv[i][e];
         s1 += u;
         s2 = fmaf(u, ev[i][e], s2);
-        if (live) {
+        if (BLOCK != 2 && live) {
           aw[i][e] = fmaf(hv[i][e], ev[i][e], aw[i][e]);
           ab[i][e] += g;
         }
@@ -249,10 +260,7 @@ layer_norm_bwd_kernel(int64_t n, int d, const T* __restrict__ gy, int64_t ldg,
       gp += step * ldg;
       loaded = row + step;
     }
-    load_row<T, V, NV, SLACK>(xn, xp, loads, lanes);
-    load_row<T, V, NV, SLACK>(gn, gp, loads, lanes);
-    mu_next = mean[loaded];
-    rs_next = rstd[loaded];
+    if (kAhead) ask();
     if (gx != nullptr) {
       row_sum2<LANES, BLOCK>(s1, s2, part, slot);
       s1 *= -rs * inv_d;
@@ -267,7 +275,7 @@ layer_norm_bwd_kernel(int64_t n, int d, const T* __restrict__ gy, int64_t ldg,
       }
     }
   }
-  if (partial == nullptr) return;
+  if (BLOCK == 2 || partial == nullptr) return;
   float* pw = partial + static_cast<int64_t>(blockIdx.x) * 2 * d;
   if constexpr (BLOCK != 0) {
 #pragma unroll
@@ -389,26 +397,50 @@ layer_norm_wide_bwd_kernel(int64_t n, int64_t d, const T* __restrict__ gy, int64
   }
 }
 
-// Partial sums of the parameter gradients over a chunk of rows, rows in order.
-template <typename T>
+// Partial sums of the parameter gradients over a chunk of rows, rows in order;
+// a thread has V neighbouring columns.
+template <typename T, int V>
 __global__ void __launch_bounds__(kLnWideThreads)
 layer_norm_wide_param_kernel(int64_t n, int64_t d, int64_t chunk, const T* __restrict__ gy,
                              int64_t ldg, const T* __restrict__ x, int64_t ldx,
                              const float* __restrict__ mean, const float* __restrict__ rstd,
                              float* __restrict__ partial) {
-  const int64_t j = static_cast<int64_t>(blockIdx.y) * kLnWideThreads + threadIdx.x;
+  const int64_t j = (static_cast<int64_t>(blockIdx.y) * kLnWideThreads + threadIdx.x) * V;
   if (j >= d) return;
   const int64_t r0 = blockIdx.x * chunk;
   const int64_t r1 = r0 + chunk < n ? r0 + chunk : n;
-  float aw = 0.0f, ab = 0.0f;
-  for (int64_t r = r0; r < r1; ++r) {
-    const float g = to_f(gy[r * ldg + j]);
-    aw = fmaf(g, (to_f(x[r * ldx + j]) - mean[r]) * rstd[r], aw);
-    ab += g;
+  float aw[V], ab[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) aw[e] = ab[e] = 0.0f;
+  constexpr int kG = V == 1 ? 8 : 4;  // rows whose loads are in flight together
+  for (int64_t rb = r0; rb < r1; rb += kG) {
+    Pack<T, V> g[kG], v[kG];
+    float mu[kG], rs[kG];
+#pragma unroll
+    for (int u = 0; u < kG; ++u) {
+      const int64_t r = rb + u < r1 ? rb + u : r1 - 1;
+      g[u] = load_pack<T, V>(gy + r * ldg + j);
+      v[u] = load_pack<T, V>(x + r * ldx + j);
+      mu[u] = mean[r];
+      rs[u] = rstd[r];
+    }
+#pragma unroll
+    for (int u = 0; u < kG; ++u)
+      if (rb + u < r1) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float ge = to_f(g[u].e[e]);
+          aw[e] = fmaf(ge, (to_f(v[u].e[e]) - mu[u]) * rs[u], aw[e]);
+          ab[e] += ge;
+        }
+      }
   }
   float* pw = partial + static_cast<int64_t>(blockIdx.x) * 2 * d;
-  pw[j] = aw;
-  pw[d + j] = ab;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    pw[j + e] = aw[e];
+    pw[d + j + e] = ab[e];
+  }
 }
 
 // How a row of nvec loads is spread: over a group of lanes (4 to 32) or the
@@ -592,6 +624,8 @@ int ln_bwd(int64_t n, int64_t d, const T* gy, int64_t ldg, const T* x, int64_t l
   const int64_t lds[] = {ldx, ldg, d};
   const LnPlan plan = ln_plan<T>(n, d, ptrs, lds, 3);
   const bool params = gw != nullptr || gb != nullptr;
+  // the parameter gradients of the widest rows, by columns
+  const bool apart = !plan.shape.fits || plan.shape.lanes > kLnBlockThreads;
   int sums = 0;
   if (!plan.shape.fits) {
     if (gx) {
@@ -599,15 +633,7 @@ int ln_bwd(int64_t n, int64_t d, const T* gy, int64_t ldg, const T* x, int64_t l
           n, d, gy, ldg, x, ldx, w, param_type, mean, rstd, gx);
       CIGN_CHECK_LAUNCH("layer_norm_wide_bwd_kernel");
     }
-    if (params) {
-      const int64_t chunk = ln_wide_chunk(n);
-      sums = static_cast<int>((n + chunk - 1) / chunk);
-      const unsigned cols = static_cast<unsigned>((d + kLnWideThreads - 1) / kLnWideThreads);
-      layer_norm_wide_param_kernel<T><<<dim3(sums, cols), kLnWideThreads, 0, s>>>(
-          n, d, chunk, gy, ldg, x, ldx, mean, rstd, partial);
-      CIGN_CHECK_LAUNCH("layer_norm_wide_param_kernel");
-    }
-  } else if (gx || params) {
+  } else if (gx || (params && !apart)) {
     CIGN_LN_DISPATCH(T, plan, {
       constexpr auto kernel = layer_norm_bwd_kernel<T, V, NV, SLACK, LANES, BLOCK>;
       const size_t smem = BLOCK != 0 ? 0 : kLnGroupThreads * NV * V * sizeof(float);
@@ -616,9 +642,23 @@ int ln_bwd(int64_t n, int64_t d, const T* gy, int64_t ldg, const T* x, int64_t l
       sums = static_cast<int>(plan.blocks < resident ? plan.blocks : resident);
       kernel<<<sums, plan.threads, smem, s>>>(n, static_cast<int>(d), gy, ldg, x, ldx, w,
                                               param_type, mean, rstd, gx,
-                                              params ? partial : nullptr);
+                                              params && !apart ? partial : nullptr);
     });
     CIGN_CHECK_LAUNCH("layer_norm_bwd_kernel");
+  }
+  if (params && apart) {
+    const int64_t chunk = ln_wide_chunk(n);
+    sums = static_cast<int>((n + chunk - 1) / chunk);
+    const int64_t loads = plan.wide ? d / (16 / sizeof(T)) : d;
+    const unsigned cols = static_cast<unsigned>((loads + kLnWideThreads - 1) / kLnWideThreads);
+    if (plan.wide)
+      layer_norm_wide_param_kernel<T, 16 / sizeof(T)>
+          <<<dim3(sums, cols), kLnWideThreads, 0, s>>>(n, d, chunk, gy, ldg, x, ldx, mean, rstd,
+                                                       partial);
+    else
+      layer_norm_wide_param_kernel<T, 1><<<dim3(sums, cols), kLnWideThreads, 0, s>>>(
+          n, d, chunk, gy, ldg, x, ldx, mean, rstd, partial);
+    CIGN_CHECK_LAUNCH("layer_norm_wide_param_kernel");
   }
   if (params) {
     const dim3 grid(static_cast<unsigned>((d + 31) / 32), 2);

@@ -61,8 +61,9 @@ def reference(x, v, i, temp, tail, g):
     W = mass + r
     grad = W[:, None] * p - target - spread
     grad = grad * temp * g[:, None]
-    # k roundings on the way of each probability (and below 2^-126, the smallest normal number, an exponential
-    # is 0, so a gradient is off by up to that); those of the log sum cancel in the loss to first order, what is left is weighted with |p - q|, which is at most sqrt(2 KL) in all (Pinsker)
+    # k roundings on the way of each probability (and below 2^-126, the smallest normal number, an exponential is
+    # 0, so a gradient is off by up to that); those of the log sum cancel in the loss to first order, what is left
+    # is weighted with |p - q|, which is at most sqrt(2 KL) in all (Pinsker)
     d = torch.where(torch.isfinite(z), z.amax(1, keepdim=True) - z, 0.0)
     ku = 2 * (sum_ulps(c) + sum_ulps(i.size(1)) + 16) * U
     dmax = (p * (1 + d)).sum(1) + 1
