@@ -509,9 +509,12 @@ log_probs_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int6
   write_piece(grad + first * c, piece, (n - first < kRows ? n - first : kRows) * c);
 }
 
-// Rows of more than kNarrowMax classes, a warp per share of a row.
+// Rows of more than kNarrowMax classes, a warp per share of a row. Each logit is
+// read and each gradient written once: bound by memory. Four blocks to an SM (64
+// registers a thread): 4096 x 32768 bf16 94.5 us, 108.6 with the three that the
+// compiler leaves by itself; five, which would spill, 153.
 template <typename T>
-__global__ void __launch_bounds__(kMapThreads)
+__global__ void __launch_bounds__(kMapThreads, 4)
 log_probs_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld,
                           const int64_t* __restrict__ labels, const float* __restrict__ stats,
                           const float* __restrict__ entropy, int top_k,
