@@ -289,7 +289,8 @@ __host__ __device__ constexpr size_t ring_bytes(int threads) {
   return static_cast<size_t>(kRingRounds) * kWideLoads<T> * 16 * threads;
 }
 
-constexpr int64_t kWideMax = (1ll << 31) - 16;  // classes: positions in a row are 32-bit
+// Classes: positions in a row are 32-bit, and loops step past its end by less than 1024.
+constexpr int64_t kWideMax = (1ll << 31) - 1024;
 
 template <typename T>
 struct RowFrame {

@@ -594,7 +594,7 @@ int lp_check(int64_t n, int64_t c, int32_t x_type, int64_t ld, int32_t top_k, co
   CIGN_REQUIRE(top_k <= kLpMaxTop, CIGN_ERR_UNSUPPORTED, "%s: top_k is at most %d", name,
                kLpMaxTop);
   CIGN_REQUIRE(n < (1ll << 31) && c <= kWideMax, CIGN_ERR_UNSUPPORTED,
-               "%s: at most 2^31 - 1 rows of at most 2^31 - 16 classes", name);
+               "%s: at most 2^31 - 1 rows of at most 2^31 - 1024 classes", name);
   return CIGN_OK;
 }
 

@@ -697,7 +697,7 @@ CIGN_API int cign_layer_norm_bwd(int64_t n, int64_t d, int32_t x_type, int32_t p
  *   labels: int64 [n]; negative = no label (log_prob 0, no gradient);
  *     >= c = log_prob NaN.  labels and log_prob may both be NULL.
  *   entropy, stats ([n, 2], 8-byte aligned, for the backward) may be NULL.
- *   n < 2^31, c <= 2^31 - 16.
+ *   n < 2^31, c <= 2^31 - 1024.
  *   A class with logit -inf has probability 0.  A row of -inf only has
  *     log_prob -inf (0 without a label), entropy 0 and gradient 0; a row with
  *     a NaN or +inf gives NaN. */

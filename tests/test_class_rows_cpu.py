@@ -56,6 +56,7 @@ def test_layer_norm_backward_refuses(kw, code):
 @pytest.mark.parametrize("kw,code", [
     (dict(n=-1), INVALID), (dict(c=0), INVALID), (dict(xt=5), INVALID), (dict(ld=7), INVALID), (dict(k=9), INVALID),
     (dict(k=-1), INVALID), (dict(c=100, ld=100, k=65), UNSUPPORTED), (dict(c=1 << 31, ld=1 << 31), UNSUPPORTED),
+    (dict(c=(1 << 31) - 1023, ld=1 << 31), UNSUPPORTED),
     (dict(x=None), NULL), (dict(labels=None), NULL), (dict(k=2), NULL), (dict(k=2, top=P), NULL),
     (dict(stats=ctypes.c_void_p(4100)), ALIGNMENT)])
 def test_log_probs_forward_refuses(kw, code):
