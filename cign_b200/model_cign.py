@@ -342,12 +342,13 @@ class GraphCliffordNet(nn.Module):
         """Without dropout: the nodes' log probability of their labels (if given), entropy and
         top_k best classes.  A teacher's top_log_probs and top_index are what node_loss takes
         (tail "bucket", temperature 1, or "drop")."""
-        training = self.training
+        training = [m for m in self.modules() if m.training]
         self.eval()
         try:
             return node_log_probs(self(x, graph_operator), labels, top_k)
-        finally:
-            self.train(training)
+        finally:  # a part that was in eval mode by itself stays so
+            for m in training:
+                m.training = True
 
 
 def build_model(in_dim: int, hidden_dim: int, out_dim: int, num_layers: int = 4,

@@ -668,7 +668,7 @@ CIGN_API int cign_block_dropout_mask(int64_t count, float p, uint64_t seed,
  *   - `x_type` and `param_type` are CIGN_F32, CIGN_BF16 or CIGN_F16.
  *   - Matrices are row-major with the stated row stride (in elements, at
  *     least the width); pointers need the alignment of one element only.
- *     Outputs have no gaps between rows.
+ *     Outputs have no gaps between rows and do not overlap inputs.
  *   - Statistics, sums and products are float32 (or wider) for every type;
  *     outputs are rounded once. */
 enum { CIGN_F32 = 0, CIGN_BF16 = 1, CIGN_F16 = 2 };

@@ -111,3 +111,26 @@ def test_rows_of_copies_only_what_a_kernel_cannot_read():
         rows, got = _lib.rows_of(t)
         assert got == ld and (rows.data_ptr() == t.data_ptr()) == same or t.numel() == 0
         assert rows.shape == t.shape
+
+
+def test_classify_leaves_the_modes_of_the_parts(monkeypatch):
+    """A part that was put in eval mode by itself stays so, after an error too."""
+    from cign_b200 import model_cign
+    model = model_cign.build_model(in_dim=8, hidden_dim=16, out_dim=3, num_layers=2, hop_scales=(1, 2), gat_heads=2)
+    model.train()
+    next(iter(model.children())).eval()
+    modes = [m.training for m in model.modules()]
+    assert True in modes and False in modes
+    seen = []
+    monkeypatch.setattr(model_cign.GraphCliffordNet, "forward",
+                        lambda self, x, op: seen.append(any(m.training for m in self.modules())))
+    monkeypatch.setattr(model_cign, "node_log_probs", lambda *a: "out")
+    assert model.classify(None, None) == "out" and seen == [False]
+    assert [m.training for m in model.modules()] == modes
+
+    def fail(*a):
+        raise ValueError("stop")
+    monkeypatch.setattr(model_cign, "node_log_probs", fail)
+    with pytest.raises(ValueError, match="stop"):
+        model.classify(None, None)
+    assert [m.training for m in model.modules()] == modes
