@@ -264,7 +264,7 @@ layer_norm_bwd_kernel(int64_t n, int d, const T* __restrict__ gy, int64_t ldg,
     if (gx != nullptr) {
       row_sum2<LANES, BLOCK>(s1, s2, part, slot);
       s1 *= -rs * inv_d;
-      s2 *= -rs * rs * rs * inv_d;
+      s2 = (s2 * rs * inv_d) * (-rs * rs);  // rstd^3 may be out of float32's range
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         Pack<T, V> q;

@@ -128,6 +128,19 @@ def test_far_mean(cuda, d):
     run_case(cuda, 21, d, torch.float32, torch.float32, mean=1000.0)
 
 
+@pytest.mark.parametrize("scale", [1e15, 1e-15])
+@pytest.mark.parametrize("d", [64, 777, 2560, 9000, 20000])
+def test_rows_of_far_magnitude(cuda, d, scale):
+    """Rows whose rstd^3 is no float32 number."""
+    x = (scale * torch.randn(21, d, device=cuda)).requires_grad_()
+    gy = torch.randn(21, d, device=cuda)
+    y = layer_norm(x, eps=0.0)
+    (gx,) = torch.autograd.grad(y, x, gy)
+    r = reference(x, None, None, gy, 0.0)
+    check(y, r["y"], r["ty"], f"y d={d} {scale}")
+    check(gx, r["gx"], r["tgx"], f"grad x d={d} {scale}")
+
+
 @pytest.mark.parametrize("d", [8, 515, 6000])
 def test_rows_without_variance(cuda, d):
     x = torch.full((5, d), 3.0, device=cuda).requires_grad_()
