@@ -132,9 +132,9 @@ __device__ __forceinline__ float exp2_hw(float t) {
 
 // e^(d / T) of two values d <= 0 by the hardware's 2^x, `scale` = log2(e) / T;
 // below 2^-126 zero.  d must be finite (callers raise it to exp_floor(scale),
-// where the result is 0).  For 16-bit logits the argument d scale is rounded to float32, which leaves a
-// relative error of about |d| 2^-23: the terms of a softmax sum weigh e^d, and
-// a gradient is rounded to 16 bits.  For float32 logits what the rounding
+// where the result is 0).  For 16-bit logits the argument d scale is rounded to
+// float32, which leaves a relative error of about |d| 2^-23: the terms of a
+// softmax sum weigh e^d, and a gradient is rounded to 16 bits.  For float32 logits what the rounding
 // drops is put back, so that the small probabilities beside a sure class keep
 // their digits.
 constexpr float kLog2e = 1.44269504f;
@@ -182,7 +182,7 @@ struct RowStat {
 // class lane + G i in register i < E: a row is read once, and the 32 / G rows
 // of a warp are neighbours.  A row costs a warp E of its steps, the sums over
 // the group, one logarithm and what is read once per row, so few lanes and many
-// classes per lane are cheapest (2.45M x 47 float32 forward: 132 us with 4
+// classes per lane are cheapest (2.45M x 47 float32 forward: 137 us with 4
 // lanes, 177 with 8, 159 with 2, whose loads are too scattered).  Up to 512
 // classes this beats a warp that streams the row (200000 rows of 512: forward
 // 102 us and 143 in float32, 125 and 204 in bf16; of 1000: 209 and 199, 338 and
