@@ -5,6 +5,8 @@ Modules named after the reference's (drop-in replacements):
     multihop_csr_pipeline, collapsed_gat, fused_gat_sideops,
     fused_clifford_pack, fused_clifford_switch_pack, fused_clifford_cign_pack,
     fused_clifford_cign_generic, fused_block_ops
+the classification head's row operators:
+    layer_norm, node_log_probs, distill
 plus graph_operator (FixedCSR operator / selected_sparse_powers), model_cign
 (the CIGN caller used by the benchmark) and synth (seeded workloads).
 

@@ -134,9 +134,9 @@ __device__ __forceinline__ float exp2_hw(float t) {
 // below 2^-126 zero.  d must be finite (callers raise it to exp_floor(scale),
 // where the result is 0).  For 16-bit logits the argument d scale is rounded to
 // float32, which leaves a relative error of about |d| 2^-23: the terms of a
-// softmax sum weigh e^d, and a gradient is rounded to 16 bits.  For float32 logits what the rounding
-// drops is put back, so that the small probabilities beside a sure class keep
-// their digits.
+// softmax sum weigh e^d, and a gradient is rounded to 16 bits.  For float32
+// logits what the rounding drops is put back, so that the small probabilities
+// beside a sure class keep their digits.
 constexpr float kLog2e = 1.44269504f;
 __device__ __forceinline__ float exp_floor(float scale) { return -160.0f / scale; }
 constexpr float kExpFloor = -160.0f / kLog2e;  // T = 1
