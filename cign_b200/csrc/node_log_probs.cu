@@ -344,13 +344,103 @@ log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
   }
 }
 
-// Rows of at most E G classes, a group of G lanes per row (class_rows.cuh).  The
-// best classes go by rounds over the lanes' registers, each of E compares and
-// 2 log2 G shuffles: right for a few (a node's best five), not for many
-// (200000 x 400, 40 best: 1.5 ms).  2.45M x 47 float32: 137 us, 3.8 TB/s, bound by
-// issue (61% of the slots) and the latency of the loads, which a prefetching
-// persistent grid did not change.
-template <typename T, int G, int E>
+// The best top_k classes of a narrow row by their keys (0: no class), for more
+// than a few.  The top_k-th largest key is found by bisection, counting the
+// larger ones of the group; it starts at the least of the maxima of top_k sets of
+// classes at least, and ends early where exactly top_k keys are above.  Those
+// classes go to `list`, and a class's place is the number of larger ones.  About
+// as long as 4 rounds over the registers where a warp has one row, 5 with two and
+// 10 with four, whose bisections go on until the last is done; with eight and more
+// the rounds are faster up to top_k = 20 and as fast at 40 (40M float32 logits,
+// select and rounds in us: 512 classes, 5 best 118 and 124, 64 best 184 and 943;
+// 200, 10 best 170 and 238; 100, 10 best 235 and 233, 20 best 290 and 402; 47, 20
+// best 336 and 334, 40 best 512 and 614; 30, 10 best 319 and 189).
+constexpr bool narrow_selects(int G) { return G >= 8; }
+constexpr int narrow_rounds(int G) { return 80 / G > 4 ? 80 / G : 4; }
+template <int G, int E>
+struct NarrowBest {
+  static constexpr int kMost = G * E < kLpMaxTop ? G * E : kLpMaxTop;
+  static constexpr int kStride = kMost + 1;  // groups read from other banks
+  static constexpr int kOwn = kMost / G;     // entries of a lane
+  // f(place, key) for the lane's entries of the best
+  template <typename F>
+  __device__ __forceinline__ static void run(const uint32_t (&key)[E], uint32_t most, int top_k,
+                                             uint64_t* list, F&& f) {
+    const int lane = threadIdx.x & (G - 1);
+    constexpr uint32_t kNone = 0x007ffffeu;  // below the key of -inf
+    uint32_t sets[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < E; ++i) sets[i * 4 / E] = max(sets[i * 4 / E], key[i]);
+    uint32_t lo = 0;
+    if (top_k <= G) {
+      lo = max(max(sets[0], sets[1]), max(sets[2], sets[3]));
+    } else if (top_k <= 2 * G) {
+      lo = min(max(sets[0], sets[1]), max(sets[2], sets[3]));
+    } else if (top_k <= 4 * G) {
+      lo = min(min(sets[0], sets[1]), min(sets[2], sets[3]));
+    }
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) lo = min(lo, __shfl_xor_sync(kFullMask, lo, o));
+    lo = max(lo, kNone + 1) - 1;
+    // more than or exactly top_k keys are above lo, `above` < top_k above hi
+    uint32_t hi = most;
+    int above = 0;
+    while (__any_sync(kFullMask, hi - lo > 1)) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      int count = 0;
+#pragma unroll
+      for (int i = 0; i < E; ++i) count += key[i] > mid ? 1 : 0;
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) count += __shfl_xor_sync(kFullMask, count, o);
+      if (hi - lo > 1) {
+        if (count > top_k) {
+          lo = mid;
+        } else {
+          hi = mid;
+          above = count;
+          if (count == top_k) lo = mid;  // found
+        }
+      }
+    }
+    // the classes above hi, then those at it by their index until top_k are there
+    const unsigned group = group_mask<G>(), before = group & ((1u << (threadIdx.x & 31)) - 1u);
+    int larger = 0, equal = above;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const bool gt = key[i] > hi, eq = key[i] == hi;
+      const unsigned who_gt = __ballot_sync(kFullMask, gt), who_eq = __ballot_sync(kFullMask, eq);
+      const int at = gt ? larger + __popc(who_gt & before) : equal + __popc(who_eq & before);
+      if ((gt || eq) && at < top_k)
+        list[at] = (static_cast<uint64_t>(key[i]) << 32) | static_cast<uint32_t>(~(lane + G * i));
+      larger += __popc(who_gt & group);
+      equal += __popc(who_eq & group);
+    }
+    __syncwarp();
+    uint64_t mine[kOwn];
+    int place[kOwn];
+#pragma unroll
+    for (int r = 0; r < kOwn; ++r) {
+      mine[r] = r * G + lane < top_k ? list[r * G + lane] : 0;
+      place[r] = 0;
+    }
+    for (int j = 0; j < top_k; ++j) {
+      const uint64_t o = list[j];
+#pragma unroll
+      for (int r = 0; r < kOwn; ++r)
+        if (r * G < top_k) place[r] += o > mine[r] ? 1 : 0;
+    }
+#pragma unroll
+    for (int r = 0; r < kOwn; ++r)
+      if (r * G + lane < top_k) f(place[r], mine[r]);
+  }
+};
+
+// Rows of at most E G classes, a group of G lanes per row (class_rows.cuh).
+// 2.45M x 47 float32: 137 us, 3.8 TB/s, bound by issue (61% of the slots) and the
+// latency of the loads, which a prefetching persistent grid did not change.
+// The best classes by rounds over the registers, each E compares and 2 log2 G
+// shuffles, or by NarrowBest (SELECT).
+template <typename T, int G, int E, bool SELECT>
 __global__ void __launch_bounds__(kNarrowThreads)
 log_probs_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_t ld,
                             const int64_t* __restrict__ labels, int top_k, LogProbOut out) {
@@ -394,6 +484,20 @@ log_probs_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int6
 #pragma unroll
   for (int i = 0; i < E; ++i)
     key[i] = i * G < own ? value_key(i % 2 == 0 ? v[i / 2].x : v[i / 2].y) : 0u;
+  if constexpr (SELECT) {
+    using Best = NarrowBest<G, E>;
+    __shared__ uint64_t lists[kNarrowThreads / G * Best::kStride];
+    // a NaN, which m skips, is above all
+    const uint32_t most = a.s == a.s ? value_key(m) : 0xffffffffu;
+    Best::run(key, most, top_k, lists + threadIdx.x / G * Best::kStride,
+              [&](int place, uint64_t k) {
+                if (!live) return;
+                out.top_index[row * top_k + place] = key_index(k);
+                out.top_log_probs[row * top_k + place] =
+                    log_prob_of(key_value(static_cast<uint32_t>(k >> 32)), m, logs);
+              });
+    return;
+  }
   for (int k = 0; k < top_k; ++k) {
     uint32_t best = 0, at_i = 0;
 #pragma unroll
@@ -635,9 +739,13 @@ int cign_node_log_probs_fwd(int64_t n, int64_t c, int32_t x_type, const void* lo
   const LogProbOut out{log_prob, entropy, stats, top_log_probs, top_index};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c <= kNarrowMax) {
-    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c,
-        log_probs_narrow_fwd_kernel<T, G, E><<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
-            n, static_cast<int>(c), static_cast<const T*>(logits), ld, labels, top_k, out)));
+    CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c, {
+      auto kernel = log_probs_narrow_fwd_kernel<T, G, E, false>;
+      if constexpr (narrow_selects(G))
+        if (top_k > narrow_rounds(G)) kernel = log_probs_narrow_fwd_kernel<T, G, E, true>;
+      kernel<<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
+          n, static_cast<int>(c), static_cast<const T*>(logits), ld, labels, top_k, out);
+    }));
     CIGN_CHECK_LAUNCH("log_probs_narrow_fwd_kernel");
     return CIGN_OK;
   }

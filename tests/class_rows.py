@@ -46,6 +46,6 @@ def check(actual, exact, allowed, what):
     # below the smallest normal number the steps do not shrink any further
     tiny = torch.finfo(actual.dtype).smallest_normal * u
     err = torch.where(same, 0.0, (a - e).abs())
-    room = allowed * (1 + u) + u * e.abs() + tiny
+    room = torch.where(same, 1.0, allowed * (1 + u) + u * e.abs() + tiny)
     worst = (err / room).nan_to_num(nan=float("inf")).max().item() if err.numel() else 0.0
     assert worst <= 1.0, f"{what}: {worst:.2f} times the allowed error"

@@ -135,6 +135,37 @@ def test_equal_logits_go_to_the_lower_class(cuda, c):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", [4, 5, 6, 10, 11, 17, 32, 33, 64])
+@pytest.mark.parametrize("c", [65, 97, 128, 129, 193, 256, 257, 385, 512])
+def test_best_classes_of_narrow_rows(cuda, c, k, dtype):
+    """Rows of different kinds side by side in a warp, the last warp not full: plain ones, few values with ties at
+    the border, masked, all masked, NaN, +inf, far magnitudes, all equal, values next to each other."""
+    g = torch.Generator(device=cuda).manual_seed(c * 100 + k)
+    n = 41
+    x = torch.randn(n, c, generator=g, device=cuda)
+    x[1::9] = torch.randint(-2, 3, (x[1::9].size(0), c), generator=g, device=cuda).float()
+    x[2::9] = x[2::9].masked_fill(torch.rand(x[2::9].shape, generator=g, device=cuda) < 0.97, -INF)
+    x[3::9] = -INF
+    x[4::9, 7::30] = float("nan")
+    x[5::9, 11] = INF
+    x[6::9] *= 60000.0
+    x[6::9] = x[6::9].clamp(-65504, 65504)
+    x[7::9] = 0.25
+    x[8::9] = 1.0 + torch.arange(c, device=cuda).flip(0) * torch.finfo(dtype).eps
+    x = x.to(dtype)
+    out = node_log_probs(x, None, k)
+    order = torch.sort(x.float(), dim=1, descending=True, stable=True)[1][:, :k]
+    assert torch.equal(out.top_index, order)
+    z = x.double()
+    best = z.gather(1, order)
+    lp = torch.where(torch.isinf(z).all(1, keepdim=True) & (z < 0).all(1, keepdim=True), -INF,
+                     best - torch.logsumexp(z, 1, keepdim=True))
+    lp = torch.where((torch.isnan(z) | (z == INF)).any(1, keepdim=True), float("nan"), lp)
+    # the sum's roundings, and those of x - m and of the difference to the logarithm
+    check(out.top_log_probs, lp, (c / 256 + 24) * U * (1 + torch.where(torch.isfinite(lp), lp.abs(), 0.0)), "top")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,c,k", [(4, 30, 10), (4, 300, 40), (300, 5000, 64), (2, 70001, 20), (4000, 1500, 50)])
 def test_fewer_classes_left_than_asked_for(cuda, n, c, k, dtype):
     """All but three classes are masked: the best are these, then masked ones by their index."""
