@@ -438,11 +438,11 @@ struct NarrowBest {
 // Rows of at most E G classes, a group of G lanes per row (class_rows.cuh).
 // 2.45M x 47 float32: 137 us, 3.8 TB/s, bound by issue (61% of the slots) and the
 // latency of the loads, which a prefetching persistent grid did not change.
-// One best class (or none) is where the maximum is; a few go by rounds over the
-// registers, each E compares and 2 log2 G shuffles, and more by NarrowBest.  A
-// kernel of its own for each: together they take 64 registers, and the rounds
-// lose 5%.  One best of 100000 x 400: 70 us by the maximum, 88 by a round.
-enum Best { kOneBest, kRounds, kSelect };
+// One best class is where the maximum is; a few go by rounds over the registers,
+// each E compares and 2 log2 G shuffles, and more by NarrowBest.  A kernel of its
+// own for each, as together they take 64 registers (100000 x 400, none: 48 us
+// with 32 registers, 55 with 48; one best: 58 us by the maximum, 88 by a round).
+enum Best { kNoBest, kOneBest, kRounds, kSelect };
 template <typename T, int G, int E, Best BEST>
 __global__ void __launch_bounds__(kNarrowThreads)
 log_probs_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_t ld,
@@ -480,16 +480,22 @@ log_probs_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int6
   a.s = group_sum<G>(s2.x + s2.y) + (group_sum<G>(cnt2.x + cnt2.y) - 1.0f);
   a.t = group_sum<G>(t2.x + t2.y);
   if (live && lane == 0) write_row(out, row, a, y, y >= 0 && y < c ? to_f(x[y]) : 0.0f, c);
-  if (top_k == 0) return;
+  if constexpr (BEST == kNoBest) return;
   const float logs = stat_log(a);
   const bool has_nan = a.s != a.s;  // which m skips
   if constexpr (BEST == kOneBest) {
     // the best class is where the maximum is, or the first NaN
     uint32_t j = 0xffffffffu;
 #pragma unroll
-    for (int i = E - 1; i >= 0; --i) {
-      const float vi = i % 2 == 0 ? v[i / 2].x : v[i / 2].y;
-      if (has_nan ? vi != vi : vi == m) j = lane + G * i;
+    for (int i = E - 1; i >= 0; --i)
+      if ((i % 2 == 0 ? v[i / 2].x : v[i / 2].y) == m) j = lane + G * i;
+    if (has_nan) {  // rarely: not worth registers
+      j = 0xffffffffu;
+#pragma unroll 1
+      for (int i = E - 1; i >= 0; --i) {
+        const float xi = i * G < own ? to_f(x[lane + i * G]) : 0.0f;
+        if (xi != xi) j = lane + G * i;
+      }
     }
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) j = min(j, __shfl_xor_sync(kFullMask, j, o));
@@ -757,8 +763,9 @@ int cign_node_log_probs_fwd(int64_t n, int64_t c, int32_t x_type, const void* lo
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c <= kNarrowMax) {
     CIGN_TYPE_DISPATCH(x_type, T, CIGN_GROUP_DISPATCH(c, {
-      auto kernel = top_k > 1 ? log_probs_narrow_fwd_kernel<T, G, E, kRounds>
-                              : log_probs_narrow_fwd_kernel<T, G, E, kOneBest>;
+      auto kernel = top_k > 1    ? log_probs_narrow_fwd_kernel<T, G, E, kRounds>
+                    : top_k == 1 ? log_probs_narrow_fwd_kernel<T, G, E, kOneBest>
+                                 : log_probs_narrow_fwd_kernel<T, G, E, kNoBest>;
       if constexpr (narrow_selects(G))
         if (top_k > narrow_rounds(G)) kernel = log_probs_narrow_fwd_kernel<T, G, E, kSelect>;
       kernel<<<narrow_grid(n, G), kNarrowThreads, 0, s>>>(
