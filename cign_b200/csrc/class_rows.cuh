@@ -182,10 +182,10 @@ struct RowStat {
 // class lane + G i in register i < E: a row is read once, and the 32 / G rows
 // of a warp are neighbours.  A row costs a warp E of its steps, the sums over
 // the group, one logarithm and what is read once per row, so few lanes and many
-// classes per lane are cheapest (2.45M x 47 float32 forward: 137 us with 4
-// lanes, 177 with 8, 159 with 2, whose loads are too scattered).  Up to 512
+// classes per lane are cheapest (2.45M x 47 float32 forward: 117 us with 4
+// lanes, 166 with 8, 158 with 2, whose loads are too scattered).  Up to 512
 // classes this beats a warp that streams the row (200000 rows of 512: forward
-// 102 us and 143 in float32, 125 and 204 in bf16; of 1000: 209 and 199, 338 and
+// 90 us and 143 in float32, 92 and 204 in bf16; of 1000: 209 and 199, 338 and
 // 207).
 constexpr int kNarrowThreads = 256;
 constexpr int64_t kNarrowMax = 512;

@@ -436,8 +436,8 @@ struct NarrowBest {
 };
 
 // Rows of at most E G classes, a group of G lanes per row (class_rows.cuh).
-// 2.45M x 47 float32: 137 us, 3.8 TB/s, bound by issue (61% of the slots) and the
-// latency of the loads, which a prefetching persistent grid did not change.
+// 2.45M x 47 float32: 117 us, 4.4 TB/s, bound by issue and the latency of the loads,
+// which a prefetching persistent grid did not change.
 // One best class is where the maximum is; a few go by rounds over the registers,
 // each E compares and 2 log2 G shuffles, and more by NarrowBest.  A kernel of its
 // own for each, as together they take 64 registers (100000 x 400, none: 48 us
@@ -595,10 +595,12 @@ __device__ __forceinline__ float special_grad(const LogProbGrads& g, const RowGr
 }
 
 // The gradient of a block's rows is formed in shared memory and written as one
-// piece, as the rows' own starts are not aligned.  2.45M x 47 float32: 200 us,
-// 4.9 TB/s, bound by issue and the latency of the row's statistics and logits.
+// piece, as the rows' own starts are not aligned.  2.45M x 47 float32: 194 us,
+// 5.1 TB/s, bound by issue and the latency of the row's statistics and logits.  Five
+// blocks to an SM, 48 registers a thread (100000 x 400: 61 us, 68 with four, 63 with
+// six, which spill).
 template <typename T, int G, int E>
-__global__ void __launch_bounds__(kNarrowThreads)
+__global__ void __launch_bounds__(kNarrowThreads, 5)
 log_probs_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_t ld,
                             const int64_t* __restrict__ labels, const float* __restrict__ stats,
                             const float* __restrict__ entropy, int top_k,
