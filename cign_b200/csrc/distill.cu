@@ -353,10 +353,10 @@ distill_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
 }
 
 // Rows of more than kNarrowMax classes, a warp per share of a row.  4096 x 32768
-// bf16, 64 kept: 120 us, 4.5 TB/s; the same pass without kept classes is 95 us, the
-// rest is their arithmetic in 64 bits.
+// bf16, 64 kept: 119 us, 4.5 TB/s, 104 with 5; bound by latency and by the kept
+// classes' arithmetic in 64 bits.
 template <typename T>
-__global__ void __launch_bounds__(kMapThreads)
+__global__ void __launch_bounds__(kMapThreads, 4)
 distill_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int64_t ld, Teacher te,
                         float temperature, InvT it, int bucket, const float* __restrict__ stats,
                         const float* __restrict__ g_loss, int64_t g_stride, int split, int warps,
@@ -369,6 +369,20 @@ distill_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
   const T* x = logits + row * ld;
   T* out = grad + row * c;
   const RowShare<T> share(x, out, c, at.rank, split);
+  // the kept classes of this share, gathered so that few lanes' worth of arithmetic
+  // in 64 bits is issued once; before the row, as these loads wait no longer than
+  // those of its statistics (30000 x 2000 float32, 100 kept: 113 us, 120 behind it)
+  uint8_t* mine = entries[threadIdx.x >> 5];
+  const int lane = threadIdx.x & 31;
+  int count = 0;
+  for (int e0 = 0; e0 < te.k; e0 += 32) {
+    const bool here = e0 + lane < te.k && share.holds(teacher_index(te, row, e0 + lane)) &&
+                      teacher_value(te, row, e0 + lane) != -INFINITY;
+    const unsigned who = __ballot_sync(kFullMask, here);
+    if (here) mine[count + __popc(who & ((1u << lane) - 1u))] = static_cast<uint8_t>(e0 + lane);
+    count += __popc(who);
+  }
+  __syncwarp();
   const DistillRow r = load_row(stats + row * kDsStats);
   const float g = g_loss[row * g_stride] * temperature;
   if (r.kind == 2.0f || g == 0.0f || (r.m == -INFINITY && r.logs == r.logs)) {
@@ -402,26 +416,12 @@ distill_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
       }
     });
   }
-  // the kept classes of this share, gathered first so that few lanes' worth of
-  // arithmetic in 64 bits is issued once
-  uint8_t* mine = entries[threadIdx.x >> 5];
-  const int lane = threadIdx.x & 31;
-  int count = 0;
-  for (int e0 = 0; e0 < te.k; e0 += 32) {
-    const bool here = e0 + lane < te.k && share.holds(teacher_index(te, row, e0 + lane)) &&
-                      teacher_value(te, row, e0 + lane) != -INFINITY;
-    const unsigned who = __ballot_sync(kFullMask, here);
-    if (here) mine[count + __popc(who & ((1u << lane) - 1u))] = static_cast<uint8_t>(e0 + lane);
-    count += __popc(who);
-  }
-  __syncwarp();  // also orders the writes of the gradient above before those below
+  __syncwarp();  // orders the writes above before those below
   for (int i = lane; i < count; i += 32) {
-    const int e = mine[i];
-    const int64_t idx = teacher_index(te, row, e);
-    const double lp = (static_cast<double>(to_f(x[idx])) - r.m) * it.full -
-                      static_cast<double>(r.logs);
-    out[idx] = from_f<T>(
-        g * kept_gradient(te, row, c, idx, teacher_value(te, row, e), lp, r, bucket, it));
+    const int idx0 = static_cast<int>(teacher_index(te, row, mine[i]));
+    const float v0 = teacher_value(te, row, mine[i]);
+    const double lp = (static_cast<double>(to_f(x[idx0])) - r.m) * it.full - static_cast<double>(r.logs);
+    out[idx0] = from_f<T>(g * kept_gradient(te, row, c, idx0, v0, lp, r, bucket, it));
   }
 }
 
