@@ -428,7 +428,7 @@ distill_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
 // Rows of at most E G classes, a group of G lanes per row (class_rows.cuh).
 // The kept classes of a row are bits in shared memory; lane l takes the
 // teacher's entries l, l + G, ...  169343 x 47 float32, 5 kept: 31 us, 1.5 TB/s,
-// bound by issue (69% of the slots): the 64-bit arithmetic and the logarithms of
+// bound by issue (71% of the slots): the 64-bit arithmetic and the logarithms of
 // 5 entries and a row weigh as much as its 47 classes.
 template <typename T, int G, int E>
 __global__ void __launch_bounds__(kNarrowThreads)
