@@ -67,17 +67,19 @@ __device__ __forceinline__ float divergence_term(float q, float d) {
 }
 
 // What the forward keeps of a row for the backward.  Outside the kept classes
-// the gradient is T g p_j (W - r / p_rest) = T g spread e^(log p_j + lift): lift
-// is 0 but where p_rest is too small to divide by.
+// the gradient is T g p_j (W - r / p_rest).  Where r / p_rest is above e it is
+// formed as T g r (W p_rest / r - 1) (p_j / p_rest), the last of which needs the
+// distance to the rest's own maximum only, however far that is below the row's.
 struct DistillRow {
   float m;       // maximum of the logits
   float logs;    // log sum e^((x - m) / T)
-  float spread;
+  float spread;  // the gradient of the other classes is T g spread e^((x - base) / T - base_log)
   float w1;      // W - 1
   float tmax;    // tail "drop": maximum and log sum of the teacher's values
   float tlog;
-  float lift;
   float kind;    // 0; 1: a class is kept twice; 2: the row has no kept class
+  __device__ __forceinline__ float base(bool bucket) const { return bucket ? tmax : m; }
+  __device__ __forceinline__ float base_log(bool bucket) const { return bucket ? tlog : logs; }
 };
 
 __device__ __forceinline__ double log_q(float v, const DistillRow& r, bool bucket,
@@ -108,30 +110,53 @@ __device__ __forceinline__ float kept_gradient(const Teacher& te, int64_t row, i
 __device__ __forceinline__ DistillRow load_row(const float* stats) {
   const float4 a = reinterpret_cast<const float4*>(stats)[0];
   const float4 b = reinterpret_cast<const float4*>(stats)[1];
-  return DistillRow{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  return DistillRow{a.x, a.y, a.z, a.w, b.x, b.y, b.z};
 }
 
-// The row's loss and statistics from the sum over its entries; log_rest is
-// log p_rest.
-__device__ __forceinline__ void finish_row(DistillRow r, float sum, float mass_r, float log_rest,
-                                           bool none, bool bad, bool dup, float temperature,
-                                           float* loss, float* stats) {
-  const float w = 1.0f + r.w1;
+// T^2 as a factor of a row's terms and one of their sum: below 1 the terms have
+// it, so that a far one of them, up to 10^42 before, stays a float32 number.
+__device__ __forceinline__ float term_scale(float temperature) {
+  return temperature < 1.0f ? temperature * temperature : 1.0f;
+}
+__device__ __forceinline__ float sum_scale(float temperature) {
+  return temperature < 1.0f ? 1.0f : temperature * temperature;
+}
+
+// The row's loss and statistics from the sum over its entries, whose terms have
+// term_scale; rest_m and rest_log are the maximum and log sum of the rest alone.
+__device__ __forceinline__ void finish_row(DistillRow r, float sum, float mass_r, float rest_m,
+                                           float rest_log, const InvT& it, bool bucket, bool none,
+                                           bool bad, bool dup, float temperature, float* loss,
+                                           float* stats) {
+  const float w = 1.0f + r.w1, ts = term_scale(temperature);
+  // log p_rest
+  const float log_rest = rest_m == -INFINITY ? -INFINITY
+                         : rest_m == r.m     ? rest_log - r.logs
+                                             : rest_log + scaled(rest_m - r.m, it) - r.logs;
   r.spread = w;
-  r.lift = 0.0f;
+  if (bucket) {
+    r.tmax = r.m;
+    r.tlog = r.logs;
+  }
   if (mass_r != 0.0f) {
     const float d = logf(mass_r) - log_rest;
-    sum += divergence_term(mass_r, d);
-    if (d < 40.0f) {
+    if (!(d >= 1e30f) || rest_m == -INFINITY) {
+      sum += ts * divergence_term(mass_r, d);
+    } else {
+      sum += static_cast<float>(
+          ts * (mass_r * ((static_cast<double>(r.m) - static_cast<double>(rest_m)) * it.full)));
+    }
+    if (d < 1.0f) {
       r.spread = w - expf(d);
-    } else if (log_rest > -INFINITY) {
-      r.spread = w * expf(-d) - 1.0f;
-      r.lift = d;
+    } else if (rest_m > -INFINITY) {
+      r.spread = (w * expf(-d) - 1.0f) * mass_r;
+      r.tmax = rest_m;
+      r.tlog = rest_log;
     }
   } else {
-    sum += expf(log_rest);
+    sum += ts * expf(log_rest);
   }
-  float l = temperature * temperature * (sum + r.w1);
+  float l = sum_scale(temperature) * fmaf(ts, r.w1, sum);
   if (r.m == -INFINITY && r.logs == r.logs) l = INFINITY;  // the student has no class left
   if (none) l = 0.0f;
   if (bad) l = r.logs = r.spread = __int_as_float(0x7fffffff);
@@ -139,7 +164,7 @@ __device__ __forceinline__ void finish_row(DistillRow r, float sum, float mass_r
   *loss = l;
   if (stats) {
     reinterpret_cast<float4*>(stats)[0] = make_float4(r.m, r.logs, r.spread, r.w1);
-    reinterpret_cast<float4*>(stats)[1] = make_float4(r.tmax, r.tlog, r.lift, r.kind);
+    reinterpret_cast<float4*>(stats)[1] = make_float4(r.tmax, r.tlog, r.kind, 0.0f);
   }
 }
 
@@ -332,11 +357,9 @@ distill_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
   r.m = st.m;
   r.logs = st.m == INFINITY ? __int_as_float(0x7fffffff) : log1pf(st.s);
   rest.m = __shfl_sync(kFullMask, rest.m, 0);
-  const float log_rest = rest.m == -INFINITY
-                             ? -INFINITY
-                             : log1pf(rest.s + (rest.cnt - 1.0f)) +
-                                   (rest.m == r.m ? 0.0f : scaled(rest.m - r.m, it)) - r.logs;
+  const float rest_log = log1pf(rest.s + (rest.cnt - 1.0f));
   const float mass_r = bucket ? rest_mass(mass, sh.distinct == c, r.w1) : (r.w1 = 0.0f);
+  const float ts = term_scale(temperature);
   float sum = 0.0f;
   for (int e = lane; e < te.k; e += 32) {
     if (sh.index[e] < 0) continue;
@@ -344,12 +367,12 @@ distill_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
     const double lp = (static_cast<double>(sh.x[e]) - r.m) * it.full - static_cast<double>(r.logs);
     const float p = expf(static_cast<float>(lq));
     const float d = static_cast<float>(lq - lp);
-    sum += first_of(e) ? divergence_term(p, d) : p * (d - 1.0f);
+    sum += ts * (first_of(e) ? divergence_term(p, d) : p * (d - 1.0f));
   }
   sum = warp_sum(sum);
   if (lane == 0)
-    finish_row(r, sum, mass_r, log_rest, sh.distinct == 0, sh.bad != 0, dup, temperature,
-               loss + row, stats ? stats + row * kDsStats : nullptr);
+    finish_row(r, sum, mass_r, rest.m, rest_log, it, bucket, sh.distinct == 0, sh.bad != 0, dup,
+               temperature, loss + row, stats ? stats + row * kDsStats : nullptr);
 }
 
 // Rows of more than kNarrowMax classes, a warp per share of a row.  4096 x 32768
@@ -394,7 +417,8 @@ distill_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
   }
   const F2 f = both(g * r.spread);
   const F2 scale = both(kLog2e * it.hi);
-  const F2 shift = both(-(r.m * it.hi + (r.logs - r.lift)) * kLog2e);
+  const float base = r.base(bucket), base_log = r.base_log(bucket);
+  const F2 shift = both(-(base * it.hi + base_log) * kLog2e);
   if (sizeof(T) == 2 && !(fabsf(shift.x) > 8192.0f)) {
     // one operation on the logit; the rounding of the shift, 2^-11 log 2 at
     // most, is below the gradient's
@@ -409,8 +433,8 @@ distill_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
     share.template run<true>([&](auto& v) {
 #pragma unroll
       for (auto& p : v) {
-        const F2 d = add2(p, both(-r.m));
-        F2 a{scaled(d.x, it) - (r.logs - r.lift), scaled(d.y, it) - (r.logs - r.lift)};
+        const F2 d = add2(p, both(-base));
+        F2 a{scaled(d.x, it) - base_log, scaled(d.y, it) - base_log};
         a = F2{max_nan(a.x, kExpFloor), max_nan(a.y, kExpFloor)};
         p = mul2(exp_neg2<T>(a, kLog2e), f);
       }
@@ -548,12 +572,12 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
   const float s = low ? s_kept + (c_kept - 1.0f) + (s_rest + c_rest) * expf(fall)
                       : s_kept + s_rest + (c_kept + c_rest - 1.0f);
   r.logs = m == INFINITY ? __int_as_float(0x7fffffff) : log1pf(s);
-  const float log_rest =
-      m_rest == -INFINITY ? -INFINITY : log1pf(s_rest + (c_rest - 1.0f)) + fall - r.logs;
+  const float rest_log = log1pf(s_rest + (c_rest - 1.0f));
 #pragma unroll
   for (int o = G / 2; o > 0; o >>= 1) mass += __shfl_xor_sync(kFullMask, mass, o);
   const float mass_r =
       bucket ? rest_mass(mass, distinct == static_cast<float>(c), r.w1) : (r.w1 = 0.0f);
+  const float ts = term_scale(temperature);
   float sum = 0.0f;
   for (int e = lane; e < te.k; e += G) {
     const Entry t = entry(e);
@@ -566,11 +590,11 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
     const double lp = (static_cast<double>(t.x) - m) * it.full - static_cast<double>(r.logs);
     const float q = expf(static_cast<float>(lq));
     const float d = static_cast<float>(lq - lp);
-    sum += first ? divergence_term(q, d) : q * (d - 1.0f);
+    sum += ts * (first ? divergence_term(q, d) : q * (d - 1.0f));
   }
   sum = group_sum<G>(sum);
-  if (live && lane == 0) finish_row(r, sum, mass_r, log_rest, distinct == 0.0f, bad, dup,
-                                    temperature, loss + row,
+  if (live && lane == 0) finish_row(r, sum, mass_r, m_rest, rest_log, it, bucket,
+                                    distinct == 0.0f, bad, dup, temperature, loss + row,
                                     stats ? stats + row * kDsStats : nullptr);
 }
 
@@ -599,10 +623,11 @@ distill_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
   const DistillRow r = load_row(stats + row * kDsStats);
   const float g = g_loss[row * g_stride] * temperature;
   const bool zero = r.kind == 2.0f || g == 0.0f || (r.m == -INFINITY && r.logs == r.logs);
-  const F2 f = both(g * r.spread), shift = both(-(r.logs - r.lift));
+  const F2 f = both(g * r.spread), shift = both(-r.base_log(bucket));
+  const float base = r.base(bucket);
 #pragma unroll
   for (int i = 0; i < E / 2; ++i) {
-    const F2 d = add2(v[i], both(-r.m));
+    const F2 d = add2(v[i], both(-base));
     F2 a = add2(F2{scaled(d.x, it), scaled(d.y, it)}, shift);
     a = F2{max_nan(a.x, kExpFloor), max_nan(a.y, kExpFloor)};
     const F2 w = mul2(exp_neg2<T>(a, kLog2e), f);
