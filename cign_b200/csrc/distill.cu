@@ -13,7 +13,8 @@
 // with d_i = log q_i - log p_{c_i}: the added sum p - sum q is W - 1 exactly,
 // because sum over kept p + p_rest = 1, and an error of the row's log sum
 // cancels in first order.  W p_j - q_j is q_j (expm1(-d_j) + (W - 1) e^-d_j).
-// d and r are formed in 64 bits from the float32 values.
+// d and r are formed in 64 bits from the float32 values.  Where d is far below 0
+// the terms are formed as p - q + q d and W p - q: e^-d alone may overflow.
 #include <cooperative_groups.h>
 
 #include "class_rows.cuh"
@@ -66,6 +67,28 @@ __device__ __forceinline__ float divergence_term(float q, float d) {
   return q * (expm1f(-d) + d);
 }
 
+// The student's probability is e^8 times the teacher's and more: e^-d, which may
+// be no float32 number while q is 0, is left out, and p - q loses nothing.
+constexpr float kFarBelow = -8.0f;
+
+// A class that the student all but masks: in 64 bits, so that q = 0 is a
+// probability that no product with d = -log p makes visible.
+__device__ __noinline__ float far_above_term(double lq, double lp, bool first, float scale) {
+  const double q = exp(lq), p = first ? exp(lp) : 0.0;
+  return static_cast<float>(scale * (p - q + (q > 0.0 ? q * (lq - lp) : 0.0)));
+}
+
+// An entry's part of the loss, p - q + q d with q = e^lq, p = e^lp, d = lq - lp,
+// times `scale`; p counts with the first entry of a class.
+__device__ __forceinline__ float entry_term(double lq, double lp, bool first, float scale) {
+  const float q = expf(static_cast<float>(lq));
+  const float d = static_cast<float>(lq - lp);
+  if (d < kFarBelow)
+    return scale * ((first ? expf(static_cast<float>(lp)) - q : -q) + (q > 0.0f ? q * d : 0.0f));
+  if (!(d < 1e4f)) return far_above_term(lq, lp, first, scale);  // NaN too
+  return scale * (first ? divergence_term(q, d) : q * (d - 1.0f));
+}
+
 // What the forward keeps of a row for the backward.  Outside the kept classes
 // the gradient is T g p_j (W - r / p_rest).  Where r / p_rest is above e it is
 // formed as T g r (W p_rest / r - 1) (p_j / p_rest), the last of which needs the
@@ -89,12 +112,14 @@ __device__ __forceinline__ double log_q(float v, const DistillRow& r, bool bucke
 }
 
 // W p - q of a kept class: q the sum of its entries.
-__device__ __forceinline__ float kept_gradient(const Teacher& te, int64_t row, int64_t c,
-                                               int64_t idx, float v, double lp,
-                                               const DistillRow& r, bool bucket, const InvT& it) {
+__device__ __forceinline__ float kept_gradient(const Teacher& te, int64_t row, int64_t idx,
+                                               float v, double lp, const DistillRow& r,
+                                               bool bucket, const InvT& it) {
   const double lq = log_q(v, r, bucket, it);
   if (r.kind == 0.0f) {
     const float d = static_cast<float>(lq - lp);
+    if (d < kFarBelow)
+      return (1.0f + r.w1) * expf(static_cast<float>(lp)) - expf(static_cast<float>(lq));
     return expf(static_cast<float>(lq)) *
            (expm1f(-d) + (r.w1 != 0.0f ? r.w1 * expf(-d) : 0.0f));
   }
@@ -365,9 +390,7 @@ distill_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
     if (sh.index[e] < 0) continue;
     const double lq = log_q(sh.value[e], r, bucket, it);
     const double lp = (static_cast<double>(sh.x[e]) - r.m) * it.full - static_cast<double>(r.logs);
-    const float p = expf(static_cast<float>(lq));
-    const float d = static_cast<float>(lq - lp);
-    sum += ts * (first_of(e) ? divergence_term(p, d) : p * (d - 1.0f));
+    sum += entry_term(lq, lp, first_of(e), ts);
   }
   sum = warp_sum(sum);
   if (lane == 0)
@@ -445,7 +468,7 @@ distill_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
     const int idx0 = static_cast<int>(teacher_index(te, row, mine[i]));
     const float v0 = teacher_value(te, row, mine[i]);
     const double lp = (static_cast<double>(to_f(x[idx0])) - r.m) * it.full - static_cast<double>(r.logs);
-    out[idx0] = from_f<T>(g * kept_gradient(te, row, c, idx0, v0, lp, r, bucket, it));
+    out[idx0] = from_f<T>(g * kept_gradient(te, row, idx0, v0, lp, r, bucket, it));
   }
 }
 
@@ -588,9 +611,7 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
         first = teacher_index(te, row, q) != t.idx || teacher_value(te, row, q) == -INFINITY;
     const double lq = log_q(t.v, r, bucket, it);
     const double lp = (static_cast<double>(t.x) - m) * it.full - static_cast<double>(r.logs);
-    const float q = expf(static_cast<float>(lq));
-    const float d = static_cast<float>(lq - lp);
-    sum += ts * (first ? divergence_term(q, d) : q * (d - 1.0f));
+    sum += entry_term(lq, lp, first, ts);
   }
   sum = group_sum<G>(sum);
   if (live && lane == 0) finish_row(r, sum, mass_r, m_rest, rest_log, it, bucket,
@@ -642,7 +663,7 @@ distill_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
       if (idx < 0 || idx >= c || tv == -INFINITY) continue;
       const double lp = (static_cast<double>(to_f(x[idx])) - r.m) * it.full -
                         static_cast<double>(r.logs);
-      out[idx] = from_f<T>(g * kept_gradient(te, row, c, idx, tv, lp, r, bucket, it));
+      out[idx] = from_f<T>(g * kept_gradient(te, row, idx, tv, lp, r, bucket, it));
     }
   }
   write_piece(grad + first * c, piece, (n - first < kRows ? n - first : kRows) * c);

@@ -72,7 +72,10 @@ def distill_top_logits(logits: torch.Tensor, teacher_values: torch.Tensor,
     class, compared with the student's probability of all the other classes.
 
     A node without entries has loss 0 and gradient 0; a student row of -inf
-    only has loss inf and gradient 0.  The gradient flows to logits (once: a
+    only has loss inf and gradient 0.  A kept class that the student masks
+    (-inf) gives loss inf, unless the teacher's probability of it is 0 in 64
+    bits (its logarithm below about -745, as a mask of -1e4 leaves it): then
+    the class takes no part.  The gradient flows to logits (once: a
     second derivative raises); the teacher's tensors are constants."""
     if logits.device.type != "cuda" or logits.dtype not in _lib.TYPE_CODES:
         raise TypeError("logits must be CUDA float32, bfloat16 or float16")

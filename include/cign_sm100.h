@@ -725,7 +725,9 @@ CIGN_API int cign_node_log_probs_bwd(int64_t n, int64_t c, int32_t x_type, const
  *   tail 1 ("bucket"): values are the teacher's log probabilities at T; what
  *     they leave of 1 is one more class, compared with the student's
  *     probability of all classes that are not kept.
- *   A row without entries has loss 0 and gradient 0.
+ *   A row without entries has loss 0 and gradient 0.  A kept class with logit
+ *     -inf gives loss inf, or takes no part if the teacher's probability of it
+ *     is 0 in 64 bits.
  *   loss [n]; stats [n, 8] (16-byte aligned, for the backward) or NULL.
  *   n < 2^31, c <= 2^20, 1e-3 <= temperature <= 1e6. */
 CIGN_API int cign_distill_fwd(int64_t n, int64_t c, int32_t x_type, const void* logits, int64_t ld,
