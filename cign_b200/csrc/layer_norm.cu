@@ -9,9 +9,18 @@
 // Statistics, products and sums are float32 whatever the element type; y and
 // the gradients are rounded once.
 //
+// The variance is formed from differences.  The mean m is a float32 number, which
+// for a row of level l leaves l 2^-24 rstd and more in xh: nothing beside the other
+// roundings where l is of the spread's size, but all digits of a row whose level is
+// far above its spread.  Such a row (far_level) takes one more sum, delta = <e> with
+// e = x - m, which is exact where x is near m:
+//   var = <e^2> - delta^2,  xh = (e - delta) rstd
+// The backward forms delta again from the m that it is given.  A row that is not far
+// pays a comparison; the sum for every row took 3 to 6% more time (24492 x 2560
+// float32: 83 + 121 us, 81 + 115 without; 103 + 138 where every row is far).
+//
 // Both passes are bound by memory: a row is read once into registers, the
-// statistics are formed there (the variance from differences, so a far mean
-// costs no digits), and the result is written.  A thread holds the same
+// statistics are formed there, and the result is written.  A thread holds the same
 // columns of every row that it meets, so weight, bias and the two sums of the
 // backward stay in registers over all rows of a persistent block, which writes
 // one partial sum of the parameter gradients at its end; a second kernel adds
@@ -27,6 +36,8 @@ namespace {
 constexpr int kLnGroupThreads = 256;  // block of the kernels with several rows per block
 constexpr int kLnBlockThreads = 512;  // of a block that holds one row; the widest rows take twice that
 constexpr int kLnMaxBlocks = 1776;    // partial sums of the parameter gradients (148 SMs x 12)
+// Wider rows leave the parameter gradients to a kernel of their own.
+constexpr int64_t kLnBlockColumns = 16 * kLnBlockThreads;
 constexpr int kLnWideThreads = 256;
 constexpr int kLnWideWarps = kLnWideThreads / 32;
 constexpr int64_t kLnMaxColumns = 65535ll * kLnWideThreads;  // the grid's second dimension
@@ -104,7 +115,36 @@ __device__ __forceinline__ void load_row(Pack<T, V> (&q)[NV], const T* r, int lo
     q[i] = load_pack<T, V>(r + (i < NV - SLACK ? i : (i < loads ? i : loads - 1)) * lanes * V);
 }
 
-// y, and mean and rstd for the backward.  24492 x 2560 float32: 80 us, 6.3 TB/s,
+// Whether the level of a row is above twice its spread; below, the mean's
+// roundings leave no more than twice their relative size in xh.
+__device__ __forceinline__ bool far_level(float mu, float rs) { return fabsf(mu * rs) > 2.0f; }
+// The same for any row of a warp, whose rows' sums are formed together.
+template <int BLOCK>
+__device__ __forceinline__ bool any_far(bool far) {
+  return BLOCK != 0 ? far : __any_sync(kFullMask, far);
+}
+// delta of the row at xr, 0 if the row is not far.  Reads the row again, as the
+// registers of a kernel that kept it for this would cost every row more.
+template <typename T, int V, int LANES, int BLOCK>
+__device__ __forceinline__ float row_delta(const T* xr, int d, float mu, bool far, float* part,
+                                           int& slot) {
+  float s = 0.0f;
+#pragma unroll 1
+  for (int i = LnLanes<LANES, BLOCK>::lane(); i < d / V; i += LnLanes<LANES, BLOCK>::count()) {
+    const Pack<T, V> q = load_pack<T, V>(xr + i * V);
+#pragma unroll
+    for (int e = 0; e < V; ++e) s += to_f(q.e[e]) - mu;
+  }
+  s = row_sum<LANES, BLOCK>(s, part, slot) * (1.0f / static_cast<float>(d));
+  return far ? s : 0.0f;
+}
+// The variance from <e^2> and delta, not below 0 (NaN stays).
+__device__ __forceinline__ float variance(float sq, float delta) {
+  const float v = fmaf(-delta, delta, sq);
+  return v < 0.0f ? 0.0f : v;
+}
+
+// y, and m and rstd for the backward.  24492 x 2560 float32: 80 us, 6.3 TB/s,
 // bound by memory.  131072 x 1024 bf16: 96 us, 5.6 TB/s, and 200003 x 301 fp16,
 // whose rows start anywhere and are read by elements: 68 us, 3.5 TB/s; both
 // bound by the instructions they issue and by the latency that the resident
@@ -112,9 +152,10 @@ __device__ __forceinline__ void load_row(Pack<T, V> (&q)[NV], const T* r, int lo
 // loads of elements.)
 // At most 80 registers: left alone, the compiler gives the 16-element bf16 row
 // 98 and fewer blocks are resident (131072 x 1024: 110 us, 96 us with 80; 64
-// spill, 111 us).
+// spill, 111 us).  72 for a block's rows of 12 elements per thread, which take no
+// more but for the far rows (40000 x 1301 float32: 73 us, 77 with 80).
 template <typename T, int V, int NV, int SLACK, int LANES, int BLOCK>
-__global__ void __maxnreg__(BLOCK == 2 ? 64 : 80)
+__global__ void __maxnreg__(BLOCK == 2 ? 64 : V == 1 && NV == 12 && BLOCK == 1 ? 72 : 80)
 layer_norm_fwd_kernel(int64_t n, int d, const T* __restrict__ x, int64_t ldx,
                       const void* __restrict__ w, const void* __restrict__ b, int32_t param_type,
                       float eps, T* __restrict__ y, float* __restrict__ mean,
@@ -162,7 +203,7 @@ layer_norm_fwd_kernel(int64_t n, int d, const T* __restrict__ x, int64_t ldx,
     }
     if (row + step < n) xp += step * ldx;
     load_row<T, V, NV, SLACK>(next, xp, loads, lanes);
-    const float mu = row_sum<LANES, BLOCK>(s, part, slot) * inv_d;
+    float mu = row_sum<LANES, BLOCK>(s, part, slot) * inv_d;
     float v = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -174,7 +215,15 @@ layer_norm_fwd_kernel(int64_t n, int d, const T* __restrict__ x, int64_t ldx,
       }
       v += i < NV - SLACK || i < own ? a : 0.0f;
     }
-    const float rs = rsqrtf(row_sum<LANES, BLOCK>(v, part, slot) * inv_d + eps);
+    v = row_sum<LANES, BLOCK>(v, part, slot) * inv_d;
+    float rs = rsqrtf(v + eps), shift = 0.0f;
+    if (any_far<BLOCK>(far_level(mu, rs))) {
+      const float delta = row_delta<T, V, LANES, BLOCK>(x + (live ? row : n - 1) * ldx, d, mu,
+                                                        far_level(mu, rs), part, slot);
+      rs = rsqrtf(variance(v, delta) + eps);
+      shift = -delta * rs;
+      mu += delta;
+    }
     if (live && lane == 0 && mean != nullptr) {
       mean[row] = mu;
       rstd[row] = rs;
@@ -183,14 +232,14 @@ layer_norm_fwd_kernel(int64_t n, int d, const T* __restrict__ x, int64_t ldx,
     for (int i = 0; i < NV; ++i) {
       Pack<T, V> q;
 #pragma unroll
-      for (int e = 0; e < V; ++e) q.e[e] = from_f<T>(fmaf(xv[i][e] * rs, wv[i][e], bv[i][e]));
+      for (int e = 0; e < V; ++e) q.e[e] = from_f<T>(fmaf(fmaf(xv[i][e], rs, shift), wv[i][e], bv[i][e]));
       if (live && (i < NV - SLACK || i < own)) store_pack<T, V>(yp + i * lanes * V, q);
     }
   }
 }
 
-// grad x, and partial: [gridDim.x, 2, d] sums of g xh and g over the block's rows,
-// or NULL.  The weights and both sums of a thread's columns are in registers, so
+// grad x; partial: [gridDim.x, 2, d] sums of g xh and g over the block's rows, or
+// NULL; deltas (BLOCK 2): those of the rows, or NULL.  The weights and both sums of a thread's columns are in registers, so
 // that x and g are read once for all three gradients: 24492 x 2560 float32 115 us,
 // 6.5 TB/s, bound by memory; 131072 x 1024 bf16 146 us, 5.5 TB/s, bound by latency
 // (24% of the warps are resident at 121 registers a thread).
@@ -204,11 +253,14 @@ layer_norm_bwd_kernel(int64_t n, int d, const T* __restrict__ gy, int64_t ldg,
                       const T* __restrict__ x, int64_t ldx, const void* __restrict__ w,
                       int32_t param_type, const float* __restrict__ mean,
                       const float* __restrict__ rstd, T* __restrict__ gx,
-                      float* __restrict__ partial) {
+                      float* __restrict__ partial, float* __restrict__ deltas) {
   using L = LnLanes<LANES, BLOCK>;
   __shared__ __align__(16) float2 part[64];
-  if (BLOCK != 0 && threadIdx.x < 32)
+  __shared__ __align__(16) float part1[64];  // of take_delta: a barrier lies between any two uses of a set
+  if (BLOCK != 0 && threadIdx.x < 32) {
     part[threadIdx.x] = part[32 + threadIdx.x] = make_float2(0.0f, 0.0f);
+    part1[threadIdx.x] = part1[32 + threadIdx.x] = 0.0f;
+  }
   if (BLOCK != 0) __syncthreads();
   extern __shared__ float columns[];  // BLOCK == 0: [rows of the block, LANES * NV * V]
   int slot = 0;
@@ -246,7 +298,7 @@ layer_norm_bwd_kernel(int64_t n, int d, const T* __restrict__ gy, int64_t ldg,
     const bool live = BLOCK != 0 || row < n;
     if (!kAhead) ask();
     const float mu = mu_next, rs = rs_next;
-    // with e = x - mean and h = g rstd: u = g w, u xh = rstd u e, g xh = h e and
+    // with e = x - m - delta and h = g rstd: u = g w, u xh = rstd u e, g xh = h e and
     // grad_x = h w - rstd <u> - e rstd^3 <u e>.  Loads behind the last repeat it:
     // they have w = 0 and their sums are dropped.
     float ev[NV][V], hv[NV][V];
@@ -254,9 +306,22 @@ layer_norm_bwd_kernel(int64_t n, int d, const T* __restrict__ gy, int64_t ldg,
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
+      for (int e = 0; e < V; ++e) ev[i][e] = to_f(xn[i].e[e]) - mu;
+    float delta = 0.0f;
+    if (any_far<BLOCK>(far_level(mu, rs))) {
+      delta = row_delta<T, V, LANES, BLOCK>(x + (live ? row : n - 1) * ldx, d, mu,
+                                            far_level(mu, rs), part1, slot);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) ev[i][e] -= delta;
+    }
+    if (BLOCK == 2 && lane == 0 && deltas != nullptr) deltas[row] = delta;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
       for (int e = 0; e < V; ++e) {
         const float g = to_f(gn[i].e[e]);
-        ev[i][e] = to_f(xn[i].e[e]) - mu;
         hv[i][e] = g * rs;
         const float u = g * wv[i][e];
         s1 += u;
@@ -349,6 +414,14 @@ layer_norm_param_sum_kernel(int blocks, int64_t d, const float* __restrict__ par
   }
 }
 
+// delta of the block's row.
+template <typename T>
+__device__ __forceinline__ float wide_delta(const T* xr, int64_t d, float mu, float* part) {
+  float s = 0.0f;
+  for (int64_t j = threadIdx.x; j < d; j += kLnWideThreads) s += to_f(xr[j]) - mu;
+  return block_sum<kLnWideWarps>(s, part) * (1.0f / static_cast<float>(d));
+}
+
 // Rows that do not fit the registers of one block: a block per row, which
 // reads the row again for each of its sums (from L2).  2000 x 40000 float32: 305 us,
 // 2.1 TB/s of the bytes that must move, bound by the latency of single loads; the
@@ -371,41 +444,53 @@ layer_norm_wide_fwd_kernel(int64_t n, int64_t d, const T* __restrict__ x, int64_
     const float a = to_f(xr[j]) - mu;
     v = fmaf(a, a, v);
   }
-  const float rs = rsqrtf(block_sum<kLnWideWarps>(v, part) * inv_d + eps);
+  v = block_sum<kLnWideWarps>(v, part) * inv_d;
+  float rs = rsqrtf(v + eps), delta = 0.0f;
+  if (far_level(mu, rs)) {
+    delta = wide_delta(xr, d, mu, part);
+    rs = rsqrtf(variance(v, delta) + eps);
+  }
   if (threadIdx.x == 0 && mean != nullptr) {
-    mean[row] = mu;
+    mean[row] = mu + delta;
     rstd[row] = rs;
   }
+  const float shift = -delta * rs;
   for (int64_t j = threadIdx.x; j < d; j += kLnWideThreads) {
-    const float xh = (to_f(xr[j]) - mu) * rs;
+    const float xh = fmaf(to_f(xr[j]) - mu, rs, shift);
     y[row * d + j] = from_f<T>(fmaf(xh, load_param(w, param_type, j, 1.0f),
                                     load_param(b, param_type, j, 0.0f)));
   }
 }
 
+// grad x and the rows' deltas; either may be NULL.
 template <typename T>
 __global__ void __launch_bounds__(kLnWideThreads)
 layer_norm_wide_bwd_kernel(int64_t n, int64_t d, const T* __restrict__ gy, int64_t ldg,
                            const T* __restrict__ x, int64_t ldx, const void* __restrict__ w,
                            int32_t param_type, const float* __restrict__ mean,
-                           const float* __restrict__ rstd, T* __restrict__ gx) {
+                           const float* __restrict__ rstd, T* __restrict__ gx,
+                           float* __restrict__ deltas) {
   __shared__ float part[kLnWideWarps];
   const float inv_d = 1.0f / static_cast<float>(d);
   const int64_t row = blockIdx.x;
   const T* xr = x + row * ldx;
   const T* gr = gy + row * ldg;
   const float mu = mean[row], rs = rstd[row];
+  const float delta = far_level(mu, rs) ? wide_delta(xr, d, mu, part) : 0.0f;
+  if (threadIdx.x == 0 && deltas != nullptr) deltas[row] = delta;
+  if (gx == nullptr) return;
+  const float shift = -delta * rs;
   float s1 = 0.0f, s2 = 0.0f;
   for (int64_t j = threadIdx.x; j < d; j += kLnWideThreads) {
     const float u = to_f(gr[j]) * load_param(w, param_type, j, 1.0f);
     s1 += u;
-    s2 = fmaf(u, (to_f(xr[j]) - mu) * rs, s2);
+    s2 = fmaf(u, fmaf(to_f(xr[j]) - mu, rs, shift), s2);
   }
   s1 = block_sum<kLnWideWarps>(s1, part) * inv_d;
   s2 = block_sum<kLnWideWarps>(s2, part) * inv_d;
   for (int64_t j = threadIdx.x; j < d; j += kLnWideThreads) {
     const float u = to_f(gr[j]) * load_param(w, param_type, j, 1.0f);
-    const float xh = (to_f(xr[j]) - mu) * rs;
+    const float xh = fmaf(to_f(xr[j]) - mu, rs, shift);
     gx[row * d + j] = from_f<T>(rs * (u - s1 - xh * s2));
   }
 }
@@ -418,7 +503,7 @@ __global__ void __launch_bounds__(kLnWideThreads)
 layer_norm_wide_param_kernel(int64_t n, int64_t d, int64_t chunk, const T* __restrict__ gy,
                              int64_t ldg, const T* __restrict__ x, int64_t ldx,
                              const float* __restrict__ mean, const float* __restrict__ rstd,
-                             float* __restrict__ partial) {
+                             const float* __restrict__ deltas, float* __restrict__ partial) {
   const int64_t j = (static_cast<int64_t>(blockIdx.y) * kLnWideThreads + threadIdx.x) * V;
   if (j >= d) return;
   const int64_t r0 = blockIdx.x * chunk;
@@ -429,7 +514,7 @@ layer_norm_wide_param_kernel(int64_t n, int64_t d, int64_t chunk, const T* __res
   constexpr int kG = V == 1 ? 8 : 4;  // rows whose loads are in flight together
   for (int64_t rb = r0; rb < r1; rb += kG) {
     Pack<T, V> g[kG], v[kG];
-    float mu[kG], rs[kG];
+    float mu[kG], rs[kG], delta[kG];
 #pragma unroll
     for (int u = 0; u < kG; ++u) {
       const int64_t r = rb + u < r1 ? rb + u : r1 - 1;
@@ -437,6 +522,7 @@ layer_norm_wide_param_kernel(int64_t n, int64_t d, int64_t chunk, const T* __res
       v[u] = load_pack<T, V>(x + r * ldx + j);
       mu[u] = mean[r];
       rs[u] = rstd[r];
+      delta[u] = deltas[r];
     }
 #pragma unroll
     for (int u = 0; u < kG; ++u)
@@ -444,7 +530,7 @@ layer_norm_wide_param_kernel(int64_t n, int64_t d, int64_t chunk, const T* __res
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const float ge = to_f(g[u].e[e]);
-          aw[e] = fmaf(ge, (to_f(v[u].e[e]) - mu[u]) * rs[u], aw[e]);
+          aw[e] = fmaf(ge, (to_f(v[u].e[e]) - mu[u] - delta[u]) * rs[u], aw[e]);
           ab[e] += ge;
         }
       }
@@ -593,6 +679,9 @@ int64_t resident_blocks(int threads, size_t smem) {
   return static_cast<int64_t>(per_sm) * sm_count();
 }
 
+// Of the widest rows' workspace, a multiple of 16 bytes.
+int64_t delta_floats(int64_t n) { return (n + 3) / 4 * 4; }
+
 int64_t ln_wide_chunk(int64_t n) {
   const int64_t c = (n + kLnMaxBlocks - 1) / kLnMaxBlocks;
   return c < 16 ? 16 : c;
@@ -633,21 +722,24 @@ int ln_fwd(int64_t n, int64_t d, const T* x, int64_t ldx, const void* w, const v
 template <typename T>
 int ln_bwd(int64_t n, int64_t d, const T* gy, int64_t ldg, const T* x, int64_t ldx, const void* w,
            int32_t param_type, const float* mean, const float* rstd, T* gx, void* gw, void* gb,
-           float* partial, cudaStream_t s) {
+           float* ws, cudaStream_t s) {
   const void* ptrs[] = {x, gy, gx};
   const int64_t lds[] = {ldx, ldg, d};
   const LnPlan plan = ln_plan<T>(n, d, ptrs, lds, 3);
   const bool params = gw != nullptr || gb != nullptr;
   // the parameter gradients of the widest rows, by columns
-  const bool apart = !plan.shape.fits || plan.shape.lanes > kLnBlockThreads;
+  const bool apart = d > kLnBlockColumns;  // where ln_plan takes more than kLnBlockThreads, or none
+  // the workspace: the rows' deltas where the parameter gradients read them, then partial sums
+  float* deltas = params && apart ? ws : nullptr;
+  float* partial = params && apart ? ws + delta_floats(n) : ws;
   int sums = 0;
-  if (!plan.shape.fits) {
-    if (gx) {
+  if (!plan.shape.fits || (apart && gx == nullptr)) {
+    if (gx || params) {
       layer_norm_wide_bwd_kernel<T><<<static_cast<unsigned>(n), kLnWideThreads, 0, s>>>(
-          n, d, gy, ldg, x, ldx, w, param_type, mean, rstd, gx);
+          n, d, gy, ldg, x, ldx, w, param_type, mean, rstd, gx, deltas);
       CIGN_CHECK_LAUNCH("layer_norm_wide_bwd_kernel");
     }
-  } else if (gx || (params && !apart)) {
+  } else if (gx || params) {
     CIGN_LN_DISPATCH(T, plan, {
       constexpr auto kernel = layer_norm_bwd_kernel<T, V, NV, SLACK, LANES, BLOCK>;
       const size_t smem = BLOCK != 0 ? 0 : kLnGroupThreads * NV * V * sizeof(float);
@@ -656,7 +748,7 @@ int ln_bwd(int64_t n, int64_t d, const T* gy, int64_t ldg, const T* x, int64_t l
       sums = static_cast<int>(plan.blocks < resident ? plan.blocks : resident);
       kernel<<<sums, plan.threads, smem, s>>>(n, static_cast<int>(d), gy, ldg, x, ldx, w,
                                               param_type, mean, rstd, gx,
-                                              params && !apart ? partial : nullptr);
+                                              params && !apart ? partial : nullptr, deltas);
     });
     CIGN_CHECK_LAUNCH("layer_norm_bwd_kernel");
   }
@@ -668,10 +760,10 @@ int ln_bwd(int64_t n, int64_t d, const T* gy, int64_t ldg, const T* x, int64_t l
     if (plan.wide)
       layer_norm_wide_param_kernel<T, 16 / sizeof(T)>
           <<<dim3(sums, cols), kLnWideThreads, 0, s>>>(n, d, chunk, gy, ldg, x, ldx, mean, rstd,
-                                                       partial);
+                                                       deltas, partial);
     else
       layer_norm_wide_param_kernel<T, 1><<<dim3(sums, cols), kLnWideThreads, 0, s>>>(
-          n, d, chunk, gy, ldg, x, ldx, mean, rstd, partial);
+          n, d, chunk, gy, ldg, x, ldx, mean, rstd, deltas, partial);
     CIGN_CHECK_LAUNCH("layer_norm_wide_param_kernel");
   }
   if (params) {
@@ -709,7 +801,8 @@ int cign_layer_norm_fwd(int64_t n, int64_t d, int32_t x_type, int32_t param_type
 
 size_t cign_layer_norm_bwd_workspace_bytes(int64_t n, int64_t d) {
   if (n <= 0 || d <= 0) return 0;
-  return 2 * static_cast<size_t>(n < kLnMaxBlocks ? n : kLnMaxBlocks) * d * sizeof(float);
+  return (2 * static_cast<size_t>(n < kLnMaxBlocks ? n : kLnMaxBlocks) * d +
+          (d > kLnBlockColumns ? delta_floats(n) : 0)) * sizeof(float);
 }
 
 int cign_layer_norm_bwd(int64_t n, int64_t d, int32_t x_type, int32_t param_type, const void* gy,

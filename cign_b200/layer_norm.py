@@ -7,7 +7,10 @@ dropout or an addend) and ``jk_norm`` the output norm over the block states
 deeper model's output norm, half-precision rows, rows of a wider buffer, norms
 without weight or bias.  Statistics and sums are float32 for every type, the
 weight and bias gradients are summed in a fixed order, and y, grad x, grad
-weight and grad bias are rounded once.
+weight and grad bias are rounded once.  A row whose level is far above its
+spread keeps its digits: what the mean's own rounding leaves is taken out.
+Rows with a spread above about 1e19, whose squares leave float32's range, come
+out as the bias.
 """
 from __future__ import annotations
 
