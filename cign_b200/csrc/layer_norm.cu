@@ -686,6 +686,10 @@ int64_t ln_wide_chunk(int64_t n) {
   const int64_t c = (n + kLnMaxBlocks - 1) / kLnMaxBlocks;
   return c < 16 ? 16 : c;
 }
+int64_t ln_wide_sums(int64_t n) {
+  const int64_t chunk = ln_wide_chunk(n);
+  return (n + chunk - 1) / chunk;
+}
 
 int ln_check(int64_t n, int64_t d, int32_t x_type, int32_t param_type, const char* name) {
   CIGN_REQUIRE(n >= 0 && d > 0, CIGN_ERR_INVALID_ARGUMENT, "%s: bad sizes", name);
@@ -754,7 +758,7 @@ int ln_bwd(int64_t n, int64_t d, const T* gy, int64_t ldg, const T* x, int64_t l
   }
   if (params && apart) {
     const int64_t chunk = ln_wide_chunk(n);
-    sums = static_cast<int>((n + chunk - 1) / chunk);
+    sums = static_cast<int>(ln_wide_sums(n));
     const int64_t loads = plan.wide ? d / (16 / sizeof(T)) : d;
     const unsigned cols = static_cast<unsigned>((loads + kLnWideThreads - 1) / kLnWideThreads);
     if (plan.wide)
@@ -801,8 +805,10 @@ int cign_layer_norm_fwd(int64_t n, int64_t d, int32_t x_type, int32_t param_type
 
 size_t cign_layer_norm_bwd_workspace_bytes(int64_t n, int64_t d) {
   if (n <= 0 || d <= 0) return 0;
-  return (2 * static_cast<size_t>(n < kLnMaxBlocks ? n : kLnMaxBlocks) * d +
-          (d > kLnBlockColumns ? delta_floats(n) : 0)) * sizeof(float);
+  // grad w and grad b of every partial sum: one per persistent block, or per chunk of rows
+  const bool apart = d > kLnBlockColumns;
+  const int64_t sums = apart ? ln_wide_sums(n) : n < kLnMaxBlocks ? n : kLnMaxBlocks;
+  return (2 * static_cast<size_t>(sums) * d + (apart ? delta_floats(n) : 0)) * sizeof(float);
 }
 
 int cign_layer_norm_bwd(int64_t n, int64_t d, int32_t x_type, int32_t param_type, const void* gy,
