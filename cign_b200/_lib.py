@@ -12,6 +12,7 @@ from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t
 from pathlib import Path
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 LIB_PATH = Path(__file__).resolve().parent / "libcign_sm100.so"
@@ -309,6 +310,14 @@ def once(backward):
     def run(ctx, *grads):
         return (refusing if torch.is_grad_enabled() else backward)(ctx, *grads)
     return staticmethod(run)
+
+
+def refuse_tangents(name: str, *tensors) -> None:
+    """Raises where a tensor is dual (forward-mode differentiation): for calls that
+    leave the autograd node out, which would raise, and would lose the tangent."""
+    for t in tensors:
+        if t is not None and unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 class DeviceGuard:

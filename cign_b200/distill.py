@@ -76,7 +76,8 @@ def distill_top_logits(logits: torch.Tensor, teacher_values: torch.Tensor,
     (-inf) gives loss inf, unless the teacher's probability of it is 0 in 64
     bits (its logarithm below about -745, as a mask of -1e4 leaves it): then
     the class takes no part.  The gradient flows to logits (once: a
-    second derivative raises); the teacher's tensors are constants."""
+    second derivative raises, as forward mode does); the teacher's tensors are
+    constants."""
     if logits.device.type != "cuda" or logits.dtype not in _lib.TYPE_CODES:
         raise TypeError("logits must be CUDA float32, bfloat16 or float16")
     if teacher_values.device != logits.device or teacher_values.dtype not in _lib.TYPE_CODES:
@@ -101,6 +102,7 @@ def distill_top_logits(logits: torch.Tensor, teacher_values: torch.Tensor,
         raise ValueError(f"tail must be 'drop' or 'bucket', got {tail!r}")
     if torch.is_grad_enabled() and logits.requires_grad:
         return _DistillFn.apply(logits, teacher_values, teacher_index, temperature, _TAILS[tail])
+    _lib.refuse_tangents("distill_top_logits", logits, teacher_values)
     rows, ld = _lib.rows_of(logits)
     values, ld_v = _lib.rows_of(teacher_values)
     index, ld_i = _lib.rows_of(teacher_index)

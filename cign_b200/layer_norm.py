@@ -79,7 +79,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     x: CUDA float32, bfloat16 or float16, any leading dimensions; the rows may
     lie in a wider buffer.  weight, bias: [D] or None, both of one type, x's or
     float32.  Gradients flow to x, weight and bias (once: a second derivative
-    raises)."""
+    raises, as forward mode does)."""
     if x.device.type != "cuda" or x.dtype not in _lib.TYPE_CODES:
         raise TypeError("x must be CUDA float32, bfloat16 or float16")
     if x.dim() < 1 or x.size(-1) < 1:
@@ -104,6 +104,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                                     or (bias is not None and bias.requires_grad)):
         y = _LayerNormFn.apply(rows, weight, bias, eps)
     else:
+        _lib.refuse_tangents("layer_norm", x, weight, bias)
         rows, ldx = _lib.rows_of(rows)
         y = _forward(rows, ldx, weight, bias, eps, False)[0]
     return y if x.dim() == 2 else y.view(x.shape)

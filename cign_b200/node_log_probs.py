@@ -88,7 +88,7 @@ def node_log_probs(logits: torch.Tensor, labels: Optional[torch.Tensor] = None,
     Logits of -inf mask classes.  A row that masks all of them has log_prob
     -inf (0 without a label), entropy 0 and gradient 0; a row with NaN or +inf
     gives NaN.  Gradients flow from log_prob, entropy and top_log_probs to
-    logits (once: a second derivative raises)."""
+    logits (once: a second derivative raises, as forward mode does)."""
     if logits.device.type != "cuda" or logits.dtype not in _lib.TYPE_CODES:
         raise TypeError("logits must be CUDA float32, bfloat16 or float16")
     if logits.dim() != 2 or logits.size(1) < 1:
@@ -105,5 +105,6 @@ def node_log_probs(logits: torch.Tensor, labels: Optional[torch.Tensor] = None,
         raise ValueError(f"top_k must be between 0 and min(C, {MAX_TOP}), got {top_k}")
     if torch.is_grad_enabled() and logits.requires_grad:
         return NodeLogProbs(*_NodeLogProbsFn.apply(logits, labels, top_k))
+    _lib.refuse_tangents("node_log_probs", logits)
     rows, ld = _lib.rows_of(logits)
     return NodeLogProbs(*_forward(rows, ld, labels, top_k, False)[:4])
