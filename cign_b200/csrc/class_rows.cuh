@@ -151,6 +151,21 @@ __device__ __forceinline__ F2 exp_neg2(F2 d, float scale) {
   return e;
 }
 
+// e^((x - m) / T - logs) of 16-bit logits as 2^(x scale + shift), one operation on
+// the logit: the constant part -(m scale + logs log2(e)) is rounded to `shift`, and
+// 2^left is a factor of what the exponentials are multiplied with.  A shift of 8192
+// is rounded by 2^-12, which would be 2^-12.5 of a probability.
+struct OneStep {
+  float shift, left;
+  __device__ __forceinline__ OneStep(float m, float logs, float scale) {
+    const double s = -(static_cast<double>(m) * scale + static_cast<double>(logs) * 1.4426950408889634);
+    shift = static_cast<float>(s);
+    left = static_cast<float>(s - shift);
+  }
+  // far ones are not finite, or their left not small
+  __device__ __forceinline__ bool near() const { return fabsf(shift) <= 8192.0f; }
+};
+
 // 1 - e^x for x <= 0, with its digits where x is near 0 (the series to x^8 is
 // exact to float32 for x > -1/2); p = e^x is given.
 __device__ __forceinline__ float one_minus_exp(float x, float p) {

@@ -439,17 +439,16 @@ distill_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
     return;
   }
   const F2 f = both(g * r.spread);
-  const F2 scale = both(kLog2e * it.hi);
   const float base = r.base(bucket), base_log = r.base_log(bucket);
-  const F2 shift = both(-(base * it.hi + base_log) * kLog2e);
-  if (sizeof(T) == 2 && !(fabsf(shift.x) > 8192.0f)) {
-    // one operation on the logit; the rounding of the shift, 2^-11 log 2 at
-    // most, is below the gradient's
+  const OneStep one(base, base_log, kLog2e * it.hi);
+  if (sizeof(T) == 2 && one.near()) {
+    const F2 scale = both(kLog2e * it.hi), shift = both(one.shift);
+    const F2 f2 = both(f.x * exp2_hw(one.left));
     share.template run<true>([&](auto& v) {
 #pragma unroll
       for (auto& p : v) {
         const F2 a = fma2(p, scale, shift);
-        p = mul2(F2{exp2_hw(a.x), exp2_hw(a.y)}, f);
+        p = mul2(F2{exp2_hw(a.x), exp2_hw(a.y)}, f2);
       }
     });
   } else {

@@ -682,17 +682,18 @@ log_probs_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
   }
   // -p G - gh p (lp + H) = p (A + B lp)
   const F2 A = both(-(r.all + r.gh * r.H)), B = both(-r.gh);
-  const F2 scale = both(kLog2e), shift = both(-(st.x + st.y) * kLog2e);
-  if (sizeof(T) == 2 && !(fabsf(shift.x) > 8192.0f)) {
-    // e^lp by one operation on the logit; the rounding of the shift, 2^-11 log 2
-    // at most, is below the gradient's
-    const F2 B2 = both(B.x * 0.693147181f);
+  const OneStep one(st.x, st.y, kLog2e);
+  if (sizeof(T) == 2 && one.near()) {
+    // with the exponent's a = (lp / log 2) - left: p (A + B lp) = 2^a 2^left (A + B2 (a + left))
+    const float back = exp2_hw(one.left), B1 = B.x * 0.693147181f;
+    const F2 scale = both(kLog2e), shift = both(one.shift);
+    const F2 B2 = both(B1 * back), A2 = both(fmaf(B1, one.left, A.x) * back);
     if (r.gh == 0.0f) {
       share.template run<true>([&](auto& v) {
 #pragma unroll
         for (auto& p : v) {
           const F2 a = fma2(p, scale, shift);
-          p = mul2(F2{exp2_hw(a.x), exp2_hw(a.y)}, A);
+          p = mul2(F2{exp2_hw(a.x), exp2_hw(a.y)}, A2);
         }
       });
     } else {
@@ -701,7 +702,7 @@ log_probs_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
         for (auto& p : v) {
           F2 a = fma2(p, scale, shift);
           a = F2{max_nan(a.x, -160.0f), max_nan(a.y, -160.0f)};  // -inf: p = 0
-          p = mul2(F2{exp2_hw(a.x), exp2_hw(a.y)}, fma2(B2, a, A));
+          p = mul2(F2{exp2_hw(a.x), exp2_hw(a.y)}, fma2(B2, a, A2));
         }
       });
     }
