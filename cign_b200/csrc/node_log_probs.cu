@@ -299,7 +299,7 @@ log_probs_wide_fwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, in
         for (int k = i * per_slot; k < (i + 1) * per_slot && k < rounds; ++k) {
           const int g = frame.g0 + from + kThreads * (k * L + lane / V);
           const bool in = lane < L * V && g < frame.g1;
-          const int f = g * V + lane % V;
+          const int f = in ? g * V + lane % V : frame.shift;  // behind the row it could pass 32 bits
           kept.add(in ? class_key(to_f(frame.base[f]), f - frame.shift) : 0, in, top_k);
         }
       }
