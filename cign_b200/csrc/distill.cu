@@ -521,7 +521,7 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
   __syncwarp();
   // teacher: kept classes, maximum
   bool bad = false, dup = false;
-  float tmax = -INFINITY, nan = 0.0f;
+  float tmax = -INFINITY;
   float distinct = 0.0f;
   for (int e = lane; e < te.k; e += G) {
     const Entry t = entry(e);
@@ -532,7 +532,6 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
     dup |= !first;
     distinct += first ? 1.0f : 0.0f;
     tmax = fmaxf(tmax, t.v);
-    if (t.v != t.v) nan = t.v;
   }
   const unsigned mine = group_mask<G>();
   bad = __ballot_sync(kFullMask, bad) & mine;
@@ -551,7 +550,7 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
     else if (t.v == r.tmax) tcnt += 1.0f;
     else tsum += expf(scaled(t.v - r.tmax, it));
   }
-  r.tlog = log1pf(group_sum<G>(tsum + nan) + (group_sum<G>(tcnt) - 1.0f));
+  r.tlog = log1pf(group_sum<G>(tsum) + (group_sum<G>(tcnt) - 1.0f));
   // student: the sums over the classes that are not kept and over the kept ones,
   // relative to their own maxima: that of the rest may be far below the row's
   float m = -INFINITY, m_rest = -INFINITY;

@@ -75,6 +75,20 @@ def test_both_mask_the_same_class(cuda):
 
 
 @pytest.mark.parametrize("tail", ["drop", "bucket"])
+@pytest.mark.parametrize("c", [6, 60, 900, 20000])
+def test_a_value_that_is_no_number_makes_its_row_so(cuda, c, tail):
+    x, v, i, _ = make(cuda, 9, c, 3, torch.float32, tail, 1.0)
+    v[1, 0] = v[2, 2] = float("nan")
+    v[3] = float("nan")
+    v[4, 1], i[4, 1] = float("nan"), -1  # absent
+    x.requires_grad_()
+    loss = distill_top_logits(x, v, i, 1.0, tail)
+    (grad,) = torch.autograd.grad(loss, x, torch.ones(9, device=cuda))
+    assert torch.isnan(loss).tolist() == [r in (1, 2, 3) for r in range(9)]
+    assert torch.isnan(grad).any(1).tolist() == [r in (1, 2, 3) for r in range(9)]
+
+
+@pytest.mark.parametrize("tail", ["drop", "bucket"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("c", [6, 60, 900])
 @pytest.mark.parametrize("temp", [0.005, 0.02, 0.05])
