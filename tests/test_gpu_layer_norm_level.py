@@ -78,3 +78,33 @@ def test_rows_of_one_value_are_the_bias(cuda, d):
     assert room < 1e-3
     assert layer_norm(x, eps=EPS).abs().max() <= room
     assert (layer_norm(x, None, b, EPS) - b).abs().max() <= room + 8 * U
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,d", [(41, 8), (5003, 37), (4001, 96), (77, 301), (1003, 520), (3001, 777), (601, 2560), (333, 5003),
+                                 (99, 9000), (49, 16001), (31, 40000)])
+def test_far_rows_leave_their_neighbours_alone(cuda, n, d, dtype):
+    """Far rows among others, in one warp and one after the other in a block: the others are bit for bit what they
+    are without them, and the far ones right."""
+    g = torch.Generator(device=cuda).manual_seed(n)
+    x = torch.randn(n, d, generator=g, device=cuda).to(dtype)
+    far = torch.rand(n, generator=g, device=cuda) < 0.3
+    far[0] = True
+    y0_in = torch.where(far[:, None], (12345.0 + x.float()).to(dtype), x).requires_grad_()
+    w = (1 + 0.1 * torch.randn(d, generator=g, device=cuda)).requires_grad_()
+    gy = torch.randn(n, d, generator=g, device=cuda).to(dtype)
+    x.requires_grad_()
+    clean, mixed = layer_norm(x, w), layer_norm(y0_in, w)
+    (gx_clean,) = torch.autograd.grad(clean, x, gy)
+    gx, gw = torch.autograd.grad(mixed, (y0_in, w), gy)
+    assert torch.equal(mixed[~far], clean[~far]) and torch.equal(gx[~far], gx_clean[~far])
+    r = reference(y0_in[far], w, torch.zeros_like(w), gy[far], EPS)
+    check(mixed[far], r["y"], r["ty"], f"y n={n} d={d} {dtype}")
+    check(gx[far], r["gx"], r["tgx"], f"grad x n={n} d={d} {dtype}")
+    z = y0_in.detach().double()
+    e = z - z.mean(1, keepdim=True)
+    xh = e * (e.pow(2).mean(1, keepdim=True) + EPS).rsqrt()
+    gd = gy.double()
+    k = (sum_ulps(d) + n / 64 + 90) * U
+    # rows that are not far: the mean's roundings, k of a mean of at most twice the spread
+    check(gw, (gd * xh).sum(0), k * (gd.abs() * (3 + xh.abs())).sum(0), f"grad w n={n} d={d} {dtype}")
