@@ -123,17 +123,25 @@ template <int BLOCK>
 __device__ __forceinline__ bool any_far(bool far) {
   return BLOCK != 0 ? far : __any_sync(kFullMask, far);
 }
-// delta of the row at xr, 0 if the row is not far.  Reads the row again, as the
-// registers of a kernel that kept it for this would cost every row more.
-template <typename T, int V, int LANES, int BLOCK>
-__device__ __forceinline__ float row_delta(const T* xr, int d, float mu, bool far, float* part,
-                                           int& slot) {
+// delta of a row, 0 if it is not far: from the lanes' e where a warp holds rows, and
+// from the row at xr, read again, where a block does, whose kernels would need more
+// registers for every row otherwise.
+template <typename T, int V, int NV, int SLACK, int LANES, int BLOCK>
+__device__ __forceinline__ float row_delta(const float (&e)[NV][V], int own, const T* xr, int d,
+                                           float mu, bool far, float* part, int& slot) {
   float s = 0.0f;
-#pragma unroll 1
-  for (int i = LnLanes<LANES, BLOCK>::lane(); i < d / V; i += LnLanes<LANES, BLOCK>::count()) {
-    const Pack<T, V> q = load_pack<T, V>(xr + i * V);
+  if constexpr (BLOCK == 0) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) s += to_f(q.e[e]) - mu;
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += i < NV - SLACK || i < own ? e[i][j] : 0.0f;
+  } else {
+#pragma unroll 1
+    for (int i = LnLanes<LANES, BLOCK>::lane(); i < d / V; i += LnLanes<LANES, BLOCK>::count()) {
+      const Pack<T, V> q = load_pack<T, V>(xr + i * V);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += to_f(q.e[j]) - mu;
+    }
   }
   s = row_sum<LANES, BLOCK>(s, part, slot) * (1.0f / static_cast<float>(d));
   return far ? s : 0.0f;
@@ -218,8 +226,8 @@ layer_norm_fwd_kernel(int64_t n, int d, const T* __restrict__ x, int64_t ldx,
     v = row_sum<LANES, BLOCK>(v, part, slot) * inv_d;
     float rs = rsqrtf(v + eps), shift = 0.0f;
     if (any_far<BLOCK>(far_level(mu, rs))) {
-      const float delta = row_delta<T, V, LANES, BLOCK>(x + (live ? row : n - 1) * ldx, d, mu,
-                                                        far_level(mu, rs), part, slot);
+      const float delta = row_delta<T, V, NV, SLACK, LANES, BLOCK>(
+          xv, own, x + row * ldx, d, mu, far_level(mu, rs), part, slot);
       rs = rsqrtf(variance(v, delta) + eps);
       shift = -delta * rs;
       mu += delta;
@@ -309,8 +317,8 @@ layer_norm_bwd_kernel(int64_t n, int d, const T* __restrict__ gy, int64_t ldg,
       for (int e = 0; e < V; ++e) ev[i][e] = to_f(xn[i].e[e]) - mu;
     float delta = 0.0f;
     if (any_far<BLOCK>(far_level(mu, rs))) {
-      delta = row_delta<T, V, LANES, BLOCK>(x + (live ? row : n - 1) * ldx, d, mu,
-                                            far_level(mu, rs), part1, slot);
+      delta = row_delta<T, V, NV, SLACK, LANES, BLOCK>(ev, own, x + row * ldx, d, mu,
+                                                       far_level(mu, rs), part1, slot);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
