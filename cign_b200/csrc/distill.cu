@@ -206,7 +206,7 @@ __device__ __forceinline__ float rest_mass(double mass, bool all_kept, float& w1
 // Rows of more than kNarrowMax classes: a team of W warps per row, with W = 8 a
 // cluster of blocks where rows are few.  The kept classes are bits in shared
 // memory, at their places in the row's frame, so that a thread finds those of
-// its 16 bytes in one byte or half of one.  4096 x 32768 bf16, 64 kept: 91 us, 3.0
+// its 16 bytes in one byte or half of one.  4096 x 32768 bf16, 64 kept: 93 us, 2.9
 // TB/s, bound by issue (67% of the slots), as the forward of node_log_probs.cu with
 // a read of the bits per 16 bytes; 777 x 10007 fp16: 14 us, and 16 x 1000 float32:
 // 5.8 us, latency: the row, then one warp's arithmetic on the entries.
@@ -473,7 +473,7 @@ distill_wide_bwd_kernel(int64_t n, int64_t c, const T* __restrict__ logits, int6
 
 // Rows of at most E G classes, a group of G lanes per row (class_rows.cuh).
 // The kept classes of a row are bits in shared memory; lane l takes the
-// teacher's entries l, l + G, ...  169343 x 47 float32, 5 kept: 31 us, 1.5 TB/s,
+// teacher's entries l, l + G, ...  169343 x 47 float32, 5 kept: 33 us, 1.5 TB/s,
 // bound by issue (71% of the slots): the 64-bit arithmetic and the logarithms of
 // 5 entries and a row weigh as much as its 47 classes.
 template <typename T, int G, int E>
@@ -617,7 +617,7 @@ distill_narrow_fwd_kernel(int64_t n, int c, const T* __restrict__ logits, int64_
                                     stats ? stats + row * kDsStats : nullptr);
 }
 
-// 169343 x 47 float32, 5 kept: 20 us, 4.0 TB/s from L2 and DRAM, bound by issue and
+// 169343 x 47 float32, 5 kept: 21 us, 4.0 TB/s from L2 and DRAM, bound by issue and
 // the latency of the entries.
 template <typename T, int G, int E>
 __global__ void __launch_bounds__(kNarrowThreads)

@@ -152,9 +152,9 @@ __device__ __forceinline__ float variance(float sq, float delta) {
   return v < 0.0f ? 0.0f : v;
 }
 
-// y, and m and rstd for the backward.  24492 x 2560 float32: 80 us, 6.3 TB/s,
-// bound by memory.  131072 x 1024 bf16: 96 us, 5.6 TB/s, and 200003 x 301 fp16,
-// whose rows start anywhere and are read by elements: 68 us, 3.5 TB/s; both
+// y, and m and rstd for the backward.  24492 x 2560 float32: 81 us, 6.2 TB/s,
+// bound by memory.  131072 x 1024 bf16: 97 us, 5.5 TB/s, and 200003 x 301 fp16,
+// whose rows start anywhere and are read by elements: 69 us, 3.5 TB/s; both
 // bound by the instructions they issue and by the latency that the resident
 // warps leave open.  (16-byte loads shifted into place were slower than the
 // loads of elements.)
@@ -249,11 +249,11 @@ layer_norm_fwd_kernel(int64_t n, int d, const T* __restrict__ x, int64_t ldx,
 // grad x; partial: [gridDim.x, 2, d] sums of g xh and g over the block's rows, or
 // NULL; deltas (BLOCK 2): those of the rows, or NULL.  The weights and both sums of a thread's columns are in registers, so
 // that x and g are read once for all three gradients: 24492 x 2560 float32 115 us,
-// 6.5 TB/s, bound by memory; 131072 x 1024 bf16 146 us, 5.5 TB/s, bound by latency
+// 6.5 TB/s, bound by memory; 131072 x 1024 bf16 148 us, 5.4 TB/s, bound by latency
 // (24% of the warps are resident at 121 registers a thread).
 // Rows that take more than kLnBlockThreads threads (BLOCK 2) leave these to a
 // kernel of their own: with them a thread would need more than the 64 registers
-// that a block of 1024 has (5093 x 10080 fp16: 90 us, and 51 for the other; bound by
+// that a block of 1024 has (5093 x 10080 fp16: 92 us, and 52 for the other; bound by
 // the latency of a row's loads and two barriers with one block to an SM).
 template <typename T, int V, int NV, int SLACK, int LANES, int BLOCK>
 __global__ void __launch_bounds__(BLOCK ? BLOCK * kLnBlockThreads : kLnGroupThreads)
@@ -431,9 +431,9 @@ __device__ __forceinline__ float wide_delta(const T* xr, int64_t d, float mu, fl
 }
 
 // Rows that do not fit the registers of one block: a block per row, which
-// reads the row again for each of its sums (from L2).  2000 x 40000 float32: 305 us,
-// 2.1 TB/s of the bytes that must move, bound by the latency of single loads; the
-// backward 350 us, 2.7 TB/s.
+// reads the row again for each of its sums (from L2).  2000 x 40000 float32: 315 us,
+// 2.0 TB/s of the bytes that must move, bound by the latency of single loads; the
+// backward 354 us, 2.7 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(kLnWideThreads)
 layer_norm_wide_fwd_kernel(int64_t n, int64_t d, const T* __restrict__ x, int64_t ldx,
@@ -505,7 +505,7 @@ layer_norm_wide_bwd_kernel(int64_t n, int64_t d, const T* __restrict__ gy, int64
 
 // Partial sums of the parameter gradients over a chunk of rows, rows in order;
 // a thread has V neighbouring columns.  It reads x and g once more: 5093 x 10080
-// fp16 51 us, 4.0 TB/s; 2000 x 40000 float32 107 us, 6.0 TB/s.
+// fp16 52 us, 4.0 TB/s; 2000 x 40000 float32 107 us, 6.0 TB/s.
 template <typename T, int V>
 __global__ void __launch_bounds__(kLnWideThreads)
 layer_norm_wide_param_kernel(int64_t n, int64_t d, int64_t chunk, const T* __restrict__ gy,

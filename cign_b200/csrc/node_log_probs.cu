@@ -188,8 +188,8 @@ __device__ __forceinline__ void find_floor(WideShared<W>& sh, float most, int sl
   team_sync<W>();
 }
 
-// 4096 x 32768 bf16: 71 us, 3.8 TB/s; 2048 x 32768 float32: 64 us, 4.2 TB/s;
-// 2048 x 65537 bf16 with 20 best classes: 87 us, 3.1 TB/s.  Bound by issue (65%
+// 4096 x 32768 bf16: 71 us, 3.8 TB/s; 2048 x 32768 float32: 65 us, 4.1 TB/s;
+// 2048 x 65537 bf16 with 20 best classes: 88 us, 3.1 TB/s.  Bound by issue (65%
 // of the slots, DRAM 38-46%): per pair of logits two conversions, one fma for the
 // exponents, two exponentials, an add and an fma for the sums, and the compares
 // of the maximum.  3 x 100003 float32 with 8 best classes, eight blocks to a row:
@@ -655,7 +655,7 @@ log_probs_narrow_bwd_kernel(int64_t n, int c, const T* __restrict__ logits, int6
 // Rows of more than kNarrowMax classes, a warp per share of a row. Each logit is
 // read and each gradient written once: bound by memory where the logits are float32
 // (2048 x 32768: 88 us, 6.1 TB/s).  Four blocks to an SM (64 registers a thread):
-// 4096 x 32768 bf16 94.5 us, 5.7 TB/s; 108.6 us with the three that the compiler
+// 4096 x 32768 bf16 96 us, 5.6 TB/s; 109 us with the three that the compiler
 // leaves by itself; five, which spill, 153.
 template <typename T>
 __global__ void __launch_bounds__(kMapThreads, 4)

@@ -71,6 +71,10 @@ def distill_top_logits(logits: torch.Tensor, teacher_values: torch.Tensor,
     probabilities at the temperature, and what they leave of 1 is one more
     class, compared with the student's probability of all the other classes.
 
+    The student's log sum is float32: at temperatures far above the logits'
+    spread, where p and q are nearly equal, the gradient of a kept class,
+    temperature * (p - q), is known to about temperature * 2^-22.
+
     A node without entries has loss 0 and gradient 0; a student row of -inf
     only has loss inf and gradient 0.  A kept class that the student masks
     (-inf) gives loss inf, unless the teacher's probability of it is 0 in 64
