@@ -240,17 +240,19 @@ layer_norm_fwd_kernel(int64_t n, int d, const T* __restrict__ x, int64_t ldx,
     for (int i = 0; i < NV; ++i) {
       Pack<T, V> q;
 #pragma unroll
-      for (int e = 0; e < V; ++e) q.e[e] = from_f<T>(fmaf(fmaf(xv[i][e], rs, shift), wv[i][e], bv[i][e]));
+      for (int e = 0; e < V; ++e)
+        q.e[e] = from_f<T>(fmaf(fmaf(xv[i][e], rs, shift), wv[i][e], bv[i][e]));
       if (live && (i < NV - SLACK || i < own)) store_pack<T, V>(yp + i * lanes * V, q);
     }
   }
 }
 
 // grad x; partial: [gridDim.x, 2, d] sums of g xh and g over the block's rows, or
-// NULL; deltas (BLOCK 2): those of the rows, or NULL.  The weights and both sums of a thread's columns are in registers, so
-// that x and g are read once for all three gradients: 24492 x 2560 float32 115 us,
-// 6.5 TB/s, bound by memory; 131072 x 1024 bf16 148 us, 5.4 TB/s, bound by latency
-// (24% of the warps are resident at 121 registers a thread).
+// NULL; deltas (BLOCK 2): those of the rows, or NULL.  The weights and both sums of
+// a thread's columns are in registers, so that x and g are read once for all three
+// gradients: 24492 x 2560 float32 115 us, 6.5 TB/s, bound by memory; 131072 x 1024
+// bf16 148 us, 5.4 TB/s, bound by latency (24% of the warps are resident at 121
+// registers a thread).
 // Rows that take more than kLnBlockThreads threads (BLOCK 2) leave these to a
 // kernel of their own: with them a thread would need more than the 64 registers
 // that a block of 1024 has (5093 x 10080 fp16: 92 us, and 52 for the other; bound by
@@ -264,7 +266,8 @@ layer_norm_bwd_kernel(int64_t n, int d, const T* __restrict__ gy, int64_t ldg,
                       float* __restrict__ partial, float* __restrict__ deltas) {
   using L = LnLanes<LANES, BLOCK>;
   __shared__ __align__(16) float2 part[64];
-  __shared__ __align__(16) float part1[64];  // of take_delta: a barrier lies between any two uses of a set
+  // row_delta's: between two uses of one set lies a barrier of its own or row_sum2's
+  __shared__ __align__(16) float part1[64];
   if (BLOCK != 0 && threadIdx.x < 32) {
     part[threadIdx.x] = part[32 + threadIdx.x] = make_float2(0.0f, 0.0f);
     part1[threadIdx.x] = part1[32 + threadIdx.x] = 0.0f;
